@@ -18,10 +18,12 @@ MAX_PLANES = 256  # EKV_MAX_PLANES
 MAX_LAYERS = 128  # EKV_MAX_LAYERS
 SHARED_INLINE_MAX = 512  # EKV_SHARED_INLINE_MAX
 SHADOW_MAX_LAYERS = 128  # EKV_SHADOW_MAX_LAYERS
+ATTENTION_MAX_BATCH = 4096  # EKV_ATTENTION_MAX_BATCH
 
 _p = ct.c_void_p
 _i32 = ct.c_int
 _i64 = ct.c_int64
+_f32 = ct.c_float
 _u64p = ct.POINTER(ct.c_uint64)
 _i64p = ct.POINTER(ct.c_int64)
 
@@ -177,6 +179,27 @@ _KERNELS = {
         _p,
     ],
     "ekv_shadow_reset": [_u64p, _i32, _i64, _p, _i32, _i64, _i32, _p],
+    "ekv_extend_block_tables": [
+        _p, _i64, _i64, _i64,
+        _p, _i32, _p, _i32, _p, _i32, _i64,
+        _p, _i64, _i64, _i64,
+        _p, _p, _p, _p, _p,
+        _i32, _p,
+    ],
+    "ekv_append_rows": [
+        _u64p, _u64p, _i32, _i64, _i64, _i64,
+        _p, _i32, _i64, _i64,
+        _i32, _p,
+    ],
+    "ekv_shared_prefix_workspace": [_i64, _i64, _i32, _i32, _i32, _i32, _i64p],
+    "ekv_shared_prefix_attention": [
+        _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64,
+        _i32, _i32, _i32, _i32, _i64, _i64,
+        _p, _i32, _i64, _i64, _i64, _i64,
+        _p, _i32, _p, _i32, _p, _i32, _i64, _i64, _f32,
+        _p, _i64, _i64, _p, _i64, _i64,
+        _p, _i64, _i32, _p,
+    ],
 }
 
 _VMM = {

@@ -499,6 +499,80 @@ int ekv_shadow_reset(
     const uint64_t* initialized, int n_layers, int64_t capacity, const void* locations, int loc_esize, int64_t n,
     int device, void* stream);
 
+/*
+ * Block tables and slot maps of a serving step, from the requests' lengths.  No
+ * reference counterpart (its engine's allocator hands out slots on the host).
+ * Request b < batch holds L = max(lengths[b], 0) tokens in row rows[b] (rows NULL:
+ * b) of block_tables [table_rows, table_width] (int32 pages of page_size
+ * positions) and gains n = new_tokens[b].  It is active when its row exists,
+ * n > 0 and L + n <= table_width * page_size, and then needs
+ * ceil((L + n) / page_size) - ceil(L / page_size) pages.  Active requests are
+ * granted in batch order while the sum of their pages stays <= n_free and the
+ * sum of their tokens <= max_tokens; the first that does not fit and all after
+ * it get nothing.  A granted request's new table entries are the next entries of
+ * free_pages, its token i has position t = L + i and slot
+ * page(t / page_size) * page_size + t % page_size (-1 where the page is negative
+ * or the slot does not fit 31 bits).  Outputs (int32): query_starts [batch + 1]
+ * (running token count), slot_map and positions [max_tokens] (-1 behind the last
+ * token), new_lengths [batch] (L + granted tokens, at most 2^31 - 1), pages_used
+ * [1].  Outputs must not overlap inputs; active rows must be distinct.  Index
+ * vectors are contiguous; table_width * page_size < 2^31.
+ */
+int ekv_extend_block_tables(
+    int32_t* block_tables, int64_t table_rows, int64_t table_width, int64_t table_row_stride,
+    const void* rows, int rows_esize, const void* lengths, int lengths_esize,
+    const void* new_tokens, int new_esize, int64_t batch,
+    const int32_t* free_pages, int64_t n_free, int64_t page_size, int64_t max_tokens,
+    int32_t* query_starts, int32_t* slot_map, int32_t* positions, int32_t* new_lengths, int32_t* pages_used,
+    int device, void* stream);
+
+/*
+ * Row append: for i < tokens with 0 <= slot_map[i] < slots and every plane p,
+ *     dst[p] + slot_map[i]*dst_row_stride_bytes <- src[p] + i*src_row_stride_bytes
+ * (row_bytes each); other tokens are skipped.  src / dst are HOST arrays of n_planes
+ * device addresses (n_planes <= EKV_MAX_PLANES).  Slots must be distinct.  No
+ * reference counterpart.
+ */
+int ekv_append_rows(
+    const uint64_t* src, const uint64_t* dst, int n_planes, int64_t row_bytes,
+    int64_t src_row_stride_bytes, int64_t dst_row_stride_bytes,
+    const void* slot_map, int map_esize, int64_t tokens, int64_t slots,
+    int device, void* stream);
+
+/*
+ * Attention of a batch whose requests share a prefix.  No reference counterpart (its
+ * engine's attention reads the rows).  Query token n is the i-th of the n_b =
+ * query_starts[b+1] - query_starts[b] new tokens of request b (query_starts NULL:
+ * tokens == batch, b = n, n_b = 1) and sees the positions
+ * t < lengths[b] - n_b + i + 1.  Position t is read from slot page * page_size +
+ * t % page_size, page = block_tables[row, t / page_size], with row = source_row for
+ * t < shared_tokens and rows[b] (NULL: b) otherwise; positions without a slot in
+ * [0, slots) are skipped.  For query head h and KV head h * kv_heads / query_heads:
+ *     out[n, h, :] = sum_t exp(scale * q.k_t) v_t / sum_t exp(scale * q.k_t)
+ *     lse[n, h] = log sum_t exp(scale * q.k_t)          (lse may be NULL)
+ * and 0 / -infinity for a token that sees nothing.  Tokens of no request are not
+ * written.  dtype is that of query, planes and out; head_dim 64 or 128; strides in
+ * elements, the head dimension contiguous, every row 16-byte aligned.  batch is at
+ * most EKV_ATTENTION_MAX_BATCH.  workspace: ekv_shared_prefix_workspace's bytes,
+ * 256-byte aligned device memory that no other call uses at the same time.
+ */
+#define EKV_BF16 0
+#define EKV_FP16 1
+#define EKV_ATTENTION_MAX_BATCH 4096
+int ekv_shared_prefix_workspace(
+    int64_t tokens, int64_t batch, int query_heads, int kv_heads, int head_dim, int device, int64_t* bytes);
+int ekv_shared_prefix_attention(
+    const void* query, int64_t q_token_stride, int64_t q_head_stride,
+    const void* k_plane, int64_t k_slot_stride, int64_t k_head_stride,
+    const void* v_plane, int64_t v_slot_stride, int64_t v_head_stride, int64_t slots,
+    int dtype, int head_dim, int query_heads, int kv_heads, int64_t tokens, int64_t batch,
+    const void* block_tables, int table_esize, int64_t table_rows, int64_t table_width, int64_t table_row_stride,
+    int64_t page_size, const void* rows, int rows_esize, const void* lengths, int lengths_esize,
+    const void* query_starts, int starts_esize, int64_t shared_tokens, int64_t source_row, float scale,
+    void* out, int64_t o_token_stride, int64_t o_head_stride,
+    float* lse, int64_t lse_token_stride, int64_t lse_head_stride,
+    void* workspace, int64_t workspace_bytes, int device, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
