@@ -5,16 +5,44 @@
 // source request's table row, every other through the request's own:
 //     o = sum_j exp(scale q.k_j) v_j / sum_j exp(scale q.k_j),   lse = log sum_j exp(scale q.k_j).
 //
-// prefix_rows_kernel: one warp per (token, query head) walks its tokens in order with a
-// running maximum and sum in 32 bits (one pass over K and V); the head dimension is
-// spread over the lanes, a score is one warp reduction.
-#include "common.cuh"
+// The work is a list of ITEMS, one per KV head and row tile (up to 256 query rows that read
+// the same keys, a row being a token and one of the head's query heads):
+//   * prefix items: row tiles over ALL tokens of the batch against the P shared positions;
+//   * own items: row tiles of one request against its positions from P on.
+// An item is a run of 128-position tiles.  Its cost is kItemCost + kTileCost per tile; the
+// total is cut into one equal share per SM (attention_kernel runs one block per SM), so an
+// item may be spread over several blocks, each of which leaves a partial result (running
+// maximum, sum and unscaled output in 32 bits).  Every block derives its share from the
+// lengths by itself (one scan over the requests), so lengths may change under a captured
+// graph, and memory-bound own items run beside the compute-bound prefix items.
+// combine_kernel joins the partial results of each row.
+//
+// attention_kernel, one tile: S = Q K^T and O += P V on the tensor cores (tcgen05, 128 rows x
+// 128 positions, 32-bit sums in tensor memory), a softmax thread per row between them.
+// Roles by warp: 0-3 and 4-7 softmax of row tile halves ("slots") 0 and 1; 8-11 gather the K and V rows
+// into swizzled shared memory (cp.async, 16 bytes a lane, whole rows; slots resolved through
+// the table, zeros for positions without one); 12 issues the products.  A 256-row item uses both slots
+// on the same K and V; smaller items alternate between them, so one's softmax runs beside
+// the other's products.  The maximum a row's weights refer to is raised only when the tile's
+// maximum passes it by 2^8 (kRaise), which makes rescaling O rare; sums stay exact to 32 bits since the
+// weights are bounded by 2^8.  Weights are rounded to the 16-bit type for the second product
+// (its operand type), the row sum is taken of the unrounded ones.
+#include "tensor.cuh"
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
 namespace ekv {
 namespace {
+
+constexpr int kRows = 128;           // rows of a slot (tensor-memory lanes)
+constexpr int kTile = 128;           // positions of a tile
+constexpr int kThreads = 512;
+constexpr int kMaxEntries = EKV_ATTENTION_MAX_ROW_TILES;
+constexpr int kItemCost = 1;         // an item's start, in units of which ...
+constexpr int kTileCost = 2;         // ... a tile is kTileCost
+constexpr int kMaskRing = 8;          // more than the stages of any layout plus 1 (see the gather role)
+constexpr float kRaise = 8.f;
 
 struct AttentionParams {
     const void* query;
@@ -27,16 +55,53 @@ struct AttentionParams {
     const void* lengths;
     const void* starts;  // null: token b is request b's only one
     int64_t q_token, q_head, k_slot, k_head, v_slot, v_head, o_token, o_head, lse_token, lse_head;
-    int64_t slots, table_rows, table_width, table_stride, page_size;
+    int64_t slots, table_rows, table_width, table_stride;
     int64_t tokens, batch, shared, source_row;
-    int query_heads, group;
+    uint32_t page_size;
+    int page_log2;  // -1: not a power of two
+    int kv_heads, group;
     int table_es, rows_es, len_es, starts_es;
     float scale_log2;  // scale * log2(e)
+    // Derived: rows per KV head, prefix row tiles, prefix tiles.
+    int64_t head_rows, prefix_row_tiles, prefix_tiles;
+    int blocks;
+    // Workspace.
+    float* prefix_out;   // [kv_heads][head_rows][dim]: an item's first part
+    float2* prefix_stat; // (maximum, sum)
+    float* own_out;
+    float2* own_stat;
+    float* next_out;     // [blocks][256][dim]: the part a block continues
+    float2* next_stat;
+    uint32_t* plan_cost; // [kMaxEntries + 1]
+    uint32_t* plan_first;  // [batch + 1]: each request's first entry
+    uint32_t* failed;    // [blocks]
 };
 
-// Request of query token n, with the tokens that n sees; false for a token of no request.
-__device__ __forceinline__ bool request_of(const AttentionParams& p, int64_t n, int64_t& b, int64_t& seen) {
-    int64_t fresh = 1, at = 0;
+// ---------------------------------------------------------------- requests
+
+struct Request {
+    int64_t begin;  // first query token
+    int64_t fresh;  // query tokens
+    int32_t length;
+};
+
+__device__ __forceinline__ Request request_at(const AttentionParams& p, int64_t b) {
+    Request r;
+    r.begin = b;
+    r.fresh = 1;
+    if (p.starts) {
+        r.begin = load_index(p.starts, p.starts_es, b);
+        r.fresh = load_index(p.starts, p.starts_es, b + 1) - r.begin;
+        if (r.begin < 0 || r.fresh < 0 || r.fresh > p.tokens - r.begin) r.fresh = 0;
+    }
+    const int64_t length = load_index(p.lengths, p.len_es, b);
+    r.length = static_cast<int32_t>(length < 0 ? 0 : (length > INT32_MAX ? INT32_MAX : length));
+    return r;
+}
+
+// Request of query token n and its place in it; false for a token of no request.
+__device__ __forceinline__ bool request_of(const AttentionParams& p, int64_t n, int64_t& b, Request& r) {
+    if (n >= p.tokens) return false;
     b = n;
     if (p.starts) {
         int64_t low = 0, high = p.batch + 1;
@@ -49,20 +114,16 @@ __device__ __forceinline__ bool request_of(const AttentionParams& p, int64_t n, 
             }
         }
         if (low >= p.batch) return false;
-        const int64_t begin = load_index(p.starts, p.starts_es, low), end = load_index(p.starts, p.starts_es, low + 1);
-        if (n < begin || n >= end) return false;
         b = low;
-        fresh = end - begin;
-        at = n - begin;
     }
-    seen = load_index(p.lengths, p.len_es, b) - fresh + at + 1;
-    return true;
+    r = request_at(p, b);
+    return n >= r.begin && n < r.begin + r.fresh;
 }
 
-// Slot of token j of table row `row`, or -1 where the table has none inside the planes.
-__device__ __forceinline__ int64_t slot_of(const AttentionParams& p, int64_t row, int64_t j) {
+// Slot of position j of table row `row`, or -1 where there is none inside the planes.
+__device__ __forceinline__ int64_t slot_of(const AttentionParams& p, int64_t row, uint32_t j) {
     if (row < 0 || row >= p.table_rows) return -1;
-    const int64_t index = j / p.page_size;
+    const uint32_t index = p.page_log2 >= 0 ? j >> p.page_log2 : j / p.page_size;
     if (index >= p.table_width) return -1;
     const int64_t page = load_index(p.tables, p.table_es, row * p.table_stride + index);
     if (page < 0 || page >= p.slots) return -1;
@@ -70,72 +131,792 @@ __device__ __forceinline__ int64_t slot_of(const AttentionParams& p, int64_t row
     return slot < p.slots ? slot : -1;
 }
 
-__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
-__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
-__device__ __forceinline__ void from_float(float x, __nv_bfloat16& y) { y = __float2bfloat16_rn(x); }
-__device__ __forceinline__ void from_float(float x, __half& y) { y = __float2half_rn(x); }
+// ---------------------------------------------------------------- the list of items
+
+// One entry per row tile of a request's own part, in shared memory; the items of an entry are
+// its KV heads.
+struct Plan {
+    uint32_t cost[kMaxEntries + 1];  // running cost of one head
+    int32_t end[kMaxEntries];        // positions the tile's last row sees
+    uint16_t request[kMaxEntries];
+    uint16_t row_tile[kMaxEntries];
+    int64_t scratch[kThreads / 32];
+    uint32_t entries;
+};
+
+__device__ __forceinline__ uint32_t item_cost(int64_t tiles) {
+    return tiles > 0 ? static_cast<uint32_t>(kItemCost + kTileCost * tiles) : 0u;
+}
+
+// Index (in the request) of the last token of a row tile.
+__device__ __forceinline__ int64_t last_token(int64_t row_tile, int64_t fresh, int group) {
+    const int64_t last = (row_tile * 2 * kRows + 2 * kRows - 1) / group;
+    return last < fresh ? last : fresh - 1;
+}
+
+// Exclusive scan over the block; `total` is the sum of all.
+__device__ __forceinline__ int64_t block_scan(int64_t value, int64_t& total, int64_t* scratch) {
+    const unsigned lane = lane_id(), warp = threadIdx.x >> 5;
+    int64_t sum = value;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t up = __shfl_up_sync(0xffffffffu, sum, d);
+        if (lane >= d) sum += up;
+    }
+    if (lane == 31) scratch[warp] = sum;
+    __syncthreads();
+    int64_t before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kThreads / 32; ++w) {
+        if (w == warp) before = total;
+        total += scratch[w];
+    }
+    __syncthreads();
+    return before + sum - value;
+}
+
+__device__ __forceinline__ void build_plan(const AttentionParams& p, Plan& plan) {
+    int64_t entries = 0;
+    for (int64_t first = 0; first < p.batch; first += kThreads) {
+        const int64_t b = first + threadIdx.x;
+        Request r{0, 0, 0};
+        if (b < p.batch) r = request_at(p, b);
+        const int64_t tiles = (r.fresh * p.group + 2 * kRows - 1) / (2 * kRows);
+        int64_t total;
+        const int64_t at = entries + block_scan(tiles, total, plan.scratch);
+        if (b < p.batch) {
+            if (blockIdx.x == 0) p.plan_first[b] = static_cast<uint32_t>(at < kMaxEntries ? at : kMaxEntries);
+            for (int64_t t = 0; t < tiles && at + t < kMaxEntries; ++t) {
+                const int64_t seen = r.length - r.fresh + last_token(t, r.fresh, p.group) + 1;
+                plan.request[at + t] = static_cast<uint16_t>(b);
+                plan.row_tile[at + t] = static_cast<uint16_t>(t);
+                plan.end[at + t] = static_cast<int32_t>(seen);
+            }
+        }
+        entries += total;
+    }
+    if (entries > kMaxEntries) entries = kMaxEntries;  // only for query_starts that are not ascending
+    __syncthreads();
+    const int64_t reach = p.table_width * p.page_size;
+    uint32_t running = 0;
+    for (int64_t first = 0; first < entries; first += kThreads) {
+        const int64_t e = first + threadIdx.x;
+        uint32_t cost = 0;
+        if (e < entries) {
+            const int64_t end = plan.end[e] < reach ? plan.end[e] : reach;
+            cost = item_cost((end - p.shared + kTile - 1) / kTile);
+            if (end <= p.shared) cost = 0;
+        }
+        int64_t total;
+        const uint32_t at = running + static_cast<uint32_t>(block_scan(cost, total, plan.scratch));
+        if (e < entries) {
+            plan.cost[e] = at;
+            if (blockIdx.x == 0) p.plan_cost[e] = at;
+        }
+        running += static_cast<uint32_t>(total);
+    }
+    if (threadIdx.x == 0) {
+        plan.cost[entries] = running;
+        plan.entries = static_cast<uint32_t>(entries);
+        if (blockIdx.x == 0) {
+            p.plan_cost[entries] = running;
+            p.plan_first[p.batch] = static_cast<uint32_t>(entries);
+        }
+    }
+    __syncthreads();
+}
+
+// Block `block`'s share of [0, total) begins here.
+__device__ __forceinline__ int64_t share_begin(int64_t block, int64_t total, int blocks) {
+    return total * block / blocks;  // below 2^63: the total is below 2^49
+}
+
+// First tile at or behind position x of an item that begins at `start` (its tile t > 0 lies at
+// start + kItemCost + t * kTileCost).
+__device__ __forceinline__ int64_t first_tile(int64_t x, int64_t start, int64_t tiles) {
+    if (x <= start) return 0;
+    int64_t t = (x - start - kItemCost + kTileCost - 1) / kTileCost;
+    if (t < 1) t = 1;
+    return t < tiles ? t : tiles;
+}
+
+struct Item {
+    bool prefix;
+    bool first;          // this block has the item's first tile
+    int head;
+    int rows;            // rows of the item, up to 256
+    int64_t request;     // own items
+    int64_t row;         // first row: of the head (prefix) or of the request (own)
+    int64_t low, high;   // tiles of this block
+    int64_t begin, end;  // positions of the whole item
+};
+
+struct Walk {
+    int64_t start, stop;  // this block's share
+    int64_t prefix_cost, prefix_items;
+    int64_t index;        // next prefix item
+    uint32_t entry;
+    int head;
+};
+
+__device__ __forceinline__ Walk begin_walk(const AttentionParams& p, const Plan& plan) {
+    Walk w;
+    w.prefix_cost = item_cost(p.prefix_tiles);
+    w.prefix_items = p.prefix_tiles ? p.prefix_row_tiles * p.kv_heads : 0;
+    const int64_t prefix_total = w.prefix_cost * w.prefix_items;
+    const int64_t total = prefix_total + static_cast<int64_t>(plan.cost[plan.entries]) * p.kv_heads;
+    w.start = share_begin(blockIdx.x, total, p.blocks);
+    w.stop = share_begin(blockIdx.x + 1, total, p.blocks);
+    w.index = w.prefix_items;
+    w.entry = 0;
+    w.head = 0;
+    if (w.start < prefix_total) {
+        w.index = w.start / w.prefix_cost;
+    } else if (plan.entries) {
+        // Last entry that begins at or before the share's start.
+        const int64_t x = w.start - prefix_total;
+        uint32_t low = 0, high = plan.entries;
+        while (high - low > 1) {
+            const uint32_t mid = (low + high) >> 1;
+            if (static_cast<int64_t>(plan.cost[mid]) * p.kv_heads <= x) {
+                low = mid;
+            } else {
+                high = mid;
+            }
+        }
+        w.entry = low;
+        const int64_t cost = plan.cost[low + 1] - plan.cost[low];
+        if (cost) w.head = static_cast<int>((x - static_cast<int64_t>(plan.cost[low]) * p.kv_heads) / cost);
+    }
+    return w;
+}
+
+// The next item of which this block has a tile; false at the end of its share.
+__device__ __forceinline__ bool next_item(const AttentionParams& p, const Plan& plan, Walk& w, Item& item) {
+    while (w.index < w.prefix_items) {
+        const int64_t start = w.index * w.prefix_cost;
+        if (start >= w.stop) return false;
+        const int64_t i = w.index++;
+        item.low = first_tile(w.start, start, p.prefix_tiles);
+        item.high = first_tile(w.stop, start, p.prefix_tiles);
+        if (item.low >= item.high) continue;
+        const int64_t tile = i % p.prefix_row_tiles;
+        item.prefix = true;
+        item.first = item.low == 0;
+        item.head = static_cast<int>(i / p.prefix_row_tiles);
+        item.row = tile * 2 * kRows;
+        item.rows = static_cast<int>(p.head_rows - item.row < 2 * kRows ? p.head_rows - item.row : 2 * kRows);
+        item.begin = 0;
+        item.end = p.shared;
+        return true;
+    }
+    const int64_t prefix_total = w.prefix_cost * w.prefix_items;
+    while (w.entry < plan.entries) {
+        const int64_t cost = plan.cost[w.entry + 1] - plan.cost[w.entry];
+        const int64_t start = prefix_total + static_cast<int64_t>(plan.cost[w.entry]) * p.kv_heads + w.head * cost;
+        if (cost && start >= w.stop) return false;
+        const uint32_t e = w.entry;
+        const int head = w.head;
+        if (!cost || ++w.head >= p.kv_heads) {
+            ++w.entry;
+            w.head = 0;
+        }
+        if (!cost) continue;
+        const int64_t tiles = (cost - kItemCost) / kTileCost;
+        item.low = first_tile(w.start, start, tiles);
+        item.high = first_tile(w.stop, start, tiles);
+        if (item.low >= item.high) continue;
+        const int64_t reach = p.table_width * p.page_size;
+        item.prefix = false;
+        item.first = item.low == 0;
+        item.head = head;
+        item.request = plan.request[e];
+        item.row = static_cast<int64_t>(plan.row_tile[e]) * 2 * kRows;
+        const int64_t left = (p.starts ? request_at(p, item.request).fresh : 1) * p.group - item.row;
+        item.rows = static_cast<int>(left < 2 * kRows ? left : 2 * kRows);
+        item.begin = p.shared;
+        item.end = plan.end[e] < reach ? plan.end[e] : reach;
+        return true;
+    }
+    return false;
+}
+
+// The query token and head of an item's row, and the positions it sees (all in [0, 2^31)).
+__device__ __forceinline__ bool row_of(const AttentionParams& p, const Item& item, int r, int64_t& token, int& head,
+                                       int64_t& seen) {
+    seen = 0;
+    if (r >= item.rows) return false;
+    const int64_t local = item.row + r;
+    const int64_t at = local / p.group;
+    head = item.head * p.group + static_cast<int>(local - at * p.group);
+    Request request;
+    if (item.prefix) {
+        token = at;
+        int64_t b;
+        if (!request_of(p, token, b, request)) return false;
+    } else {
+        request = request_at(p, item.request);
+        token = request.begin + at;
+    }
+    seen = request.length - request.fresh + (token - request.begin) + 1;
+    return true;
+}
+
+// ---------------------------------------------------------------- the kernel
+
+template <int kDim>
+struct Layout {
+    static constexpr int kStages = kDim == 128 ? 2 : 4;
+    static constexpr uint32_t kBlock = kTile * 128;            // 128 rows of 128 bytes
+    static constexpr uint32_t kOperand = kBlock * (kDim / 64); // 128 rows of the head dimension
+    static constexpr uint32_t kQuery = 0;
+    static constexpr uint32_t kKeys = 2 * kOperand;
+    static constexpr uint32_t kValues = kKeys + kStages * kOperand;
+    static constexpr uint32_t kPlan = kValues + kStages * kOperand;
+    static constexpr uint32_t kMasks = kPlan + ((sizeof(Plan) + 15) / 16) * 16;
+    static constexpr uint32_t kBarriers = kMasks + kMaskRing * 16;
+    // k_full, k_empty, v_full, v_empty (stages each); q_full, q_empty, s_full, p_full, o_full (slots each); drain.
+    static constexpr int kBarrierCount = 4 * kStages + 5 * 2 + 1;
+    static constexpr uint32_t kTail = kBarriers + kBarrierCount * 8;
+    static constexpr uint32_t kBytes = kTail + 16;  // tensor-memory address, failed flag
+};
+
+template <typename T>
+struct Kind;
+template <>
+struct Kind<__nv_bfloat16> {
+    static constexpr bool kBf16 = true;
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+};
+template <>
+struct Kind<__half> {
+    static constexpr bool kBf16 = false;
+    static __device__ __forceinline__ uint32_t pack(float a, float b) {
+        const __half2 v = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+};
 
 template <typename T, int kDim>
-__global__ void __launch_bounds__(128) prefix_rows_kernel(const __grid_constant__ AttentionParams p) {
-    constexpr int kPer = kDim / 32;
-    grid_dependency_wait();
-    allow_dependents();
-    const int64_t item = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    const int64_t n = item / p.query_heads;
-    const int head = static_cast<int>(item - n * p.query_heads);
+__global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_constant__ AttentionParams p) {
+    using L = Layout<kDim>;
+    extern __shared__ __align__(1024) uint8_t shared[];
+    Plan& plan = *reinterpret_cast<Plan*>(shared + L::kPlan);
+    volatile uint32_t* masks = reinterpret_cast<uint32_t*>(shared + L::kMasks);
+    volatile uint32_t* failed = reinterpret_cast<uint32_t*>(shared + L::kTail + 4);
+    const uint32_t base = shared_address(shared);
+    const int warp = threadIdx.x >> 5;
     const unsigned lane = lane_id();
-    int64_t b, seen;
-    if (n >= p.tokens || !request_of(p, n, b, seen)) return;
-    const int64_t row = p.rows ? load_index(p.rows, p.rows_es, b) : b;
-    const int kv_head = head / p.group;
-    const T* q = static_cast<const T*>(p.query) + n * p.q_token + head * p.q_head;
-    const T* k = static_cast<const T*>(p.k_plane) + kv_head * p.k_head;
-    const T* v = static_cast<const T*>(p.v_plane) + kv_head * p.v_head;
-    float query[kPer], acc[kPer];
-#pragma unroll
-    for (int i = 0; i < kPer; ++i) {
-        query[i] = to_float(q[lane + 32 * i]);
-        acc[i] = 0.f;
-    }
-    float top = -INFINITY, total = 0.f;
-    for (int64_t j = 0; j < seen; ++j) {
-        const int64_t slot = slot_of(p, j < p.shared ? p.source_row : row, j);
-        if (slot < 0) {
-            if (j / p.page_size >= p.table_width) break;
-            continue;
+
+    const uint32_t barriers = base + L::kBarriers;
+    const auto k_full = [&](int s) { return barriers + 8 * s; };
+    const auto k_empty = [&](int s) { return barriers + 8 * (L::kStages + s); };
+    const auto v_full = [&](int s) { return barriers + 8 * (2 * L::kStages + s); };
+    const auto v_empty = [&](int s) { return barriers + 8 * (3 * L::kStages + s); };
+    const auto slot_barrier = [&](int which, int s) { return barriers + 8 * (4 * L::kStages + 2 * which + s); };
+    const auto q_full = [&](int s) { return slot_barrier(0, s); };
+    const auto q_empty = [&](int s) { return slot_barrier(1, s); };
+    const auto s_full = [&](int s) { return slot_barrier(2, s); };
+    const auto p_full = [&](int s) { return slot_barrier(3, s); };
+    const auto o_full = [&](int s) { return slot_barrier(4, s); };
+    const uint32_t drain = barriers + 8 * (L::kBarrierCount - 1);
+
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < L::kStages; ++s) {
+            barrier_init(k_full(s), 4);
+            barrier_init(k_empty(s), 1);
+            barrier_init(v_full(s), 4);
+            barrier_init(v_empty(s), 1);
         }
-        float score = 0.f;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) score = fmaf(query[i], to_float(k[slot * p.k_slot + lane + 32 * i]), score);
-#pragma unroll
-        for (int d = 16; d; d >>= 1) score += __shfl_xor_sync(0xffffffffu, score, d);
-        score *= p.scale_log2;
-        const float higher = fmaxf(top, score);
-        const float rescale = top == -INFINITY ? 0.f : exp2f(top - higher);
-        const float weight = higher == -INFINITY ? 0.f : exp2f(score - higher);
-        top = higher;
-        total = total * rescale + weight;
-#pragma unroll
-        for (int i = 0; i < kPer; ++i) {
-            acc[i] = fmaf(weight, to_float(v[slot * p.v_slot + lane + 32 * i]), acc[i] * rescale);
+        for (int s = 0; s < 2; ++s) {
+            barrier_init(q_full(s), 4);
+            barrier_init(q_empty(s), 1);
+            barrier_init(s_full(s), 1);
+            barrier_init(p_full(s), 4);
+            barrier_init(o_full(s), 1);
         }
+        barrier_init(drain, 1);
+        *failed = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        fence_async_shared();
     }
-    T* o = static_cast<T*>(p.out) + n * p.o_token + head * p.o_head;
+    if (warp == 12) tensor_alloc(base + L::kTail, 512);
+    grid_dependency_wait();
+    tensor_fence_before();
+    build_plan(p, plan);  // ends with __syncthreads
+    tensor_fence_after();
+    const uint32_t tensor = *reinterpret_cast<volatile uint32_t*>(shared + L::kTail);
+
+    Walk walk = begin_walk(p, plan);
+    Item item;
+    int turn = 0;  // slot of the next item of up to 128 rows
+
+    if (warp < 8) {
+        // ------------------------------------------------------------ softmax of slot `slot`
+        const int slot = warp >> 2;
+        const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 tensor-memory lanes a warp
+        const uint32_t scores = tensor + lanes + slot * kTile;
+        const uint32_t output = tensor + lanes + 256 + slot * 128;
+        uint32_t uses = 0, ends = 0, tile_count = 0;
+        const int r = (warp & 3) * 32 + lane;
+        while (next_item(p, plan, walk, item)) {
+            const bool both = item.rows > kRows;
+            const int mine = both ? slot : turn;
+            turn ^= 1;
+            if (mine != slot) {
+                tile_count += static_cast<uint32_t>(item.high - item.low);
+                continue;
+            }
+            const int item_row = (both ? slot * kRows : 0) + r;
+            int64_t token = 0, seen;
+            int head = 0;
+            const bool present = row_of(p, item, item_row, token, head, seen);
+            if (!present) seen = INT64_MAX;  // computed with the others and dropped
+            const bool idle = (both ? slot * kRows : 0) + (warp & 3) * 32 >= item.rows;  // no row in this warp
+            float top = -INFINITY, total = 0.f;
+            for (int64_t t = item.low; t < item.high; ++t, ++tile_count) {
+                if (!__all_sync(0xffffffffu, barrier_wait(s_full(slot), uses & 1, failed))) goto finish;
+                ++uses;
+                tensor_fence_after();
+                if (!idle) {
+                    const int64_t position = item.begin + t * kTile;
+                    // Positions this row sees here: those that have a slot, up to its last.
+                    const int64_t left = seen - position;
+                    uint32_t bits[4];
+                    uint32_t all = 0xffffffffu;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) from_float(total == 0.f ? 0.f : acc[i] / total, o[lane + 32 * i]);
-    if (p.lse && lane == 0) {
-        p.lse[n * p.lse_token + head * p.lse_head] =
-            total == 0.f ? -INFINITY : (top + log2f(total)) * 0.69314718055994531f;
+                    for (int c = 0; c < 4; ++c) {
+                        const int64_t mine_left = left - 32 * c;
+                        const uint32_t limit =
+                            mine_left >= 32 ? 0xffffffffu : (mine_left <= 0 ? 0u : (1u << mine_left) - 1u);
+                        bits[c] = masks[(tile_count % kMaskRing) * 4 + c] & limit;
+                        all &= bits[c];
+                    }
+                    const bool whole = __all_sync(0xffffffffu, all == 0xffffffffu);
+                    float high = -INFINITY;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t s[32];
+                        tensor_load32(scores + 32 * c, s);
+                        tensor_wait_load();
+                        if (whole) {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) high = fmaxf(high, __uint_as_float(s[j]));
+                        } else {
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) {
+                                high = fmaxf(high, bits[c] >> j & 1u ? __uint_as_float(s[j]) : -INFINITY);
+                            }
+                        }
+                    }
+                    high *= p.scale_log2;
+                    const bool raise = present && (high > top + kRaise || (top == -INFINITY && high > -INFINITY));
+                    if (__any_sync(0xffffffffu, raise)) {
+                        const float before = top;
+                        if (raise) top = high;
+                        const float factor = raise ? (before == -INFINITY ? 0.f : exp2_approx(before - top)) : 1.f;
+                        total *= factor;
+                        if (t > item.low) {
+                            // The products of this slot's earlier tiles are complete (s_full).
+#pragma unroll 1
+                            for (int c = 0; c < kDim / 32; ++c) {
+                                uint32_t o[32];
+                                tensor_load32(output + 32 * c, o);
+                                tensor_wait_load();
+#pragma unroll
+                                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * factor);
+                                tensor_store32(output + 32 * c, o);
+                            }
+                        }
+                    }
+                    const float shift = top == -INFINITY ? 0.f : top;
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        uint32_t s[32], weights[16];
+                        tensor_load32(scores + 32 * c, s);
+                        tensor_wait_load();
+#pragma unroll
+                        for (int j = 0; j < 32; j += 2) {
+                            float a = exp2_approx(fmaf(__uint_as_float(s[j]), p.scale_log2, -shift));
+                            float b = exp2_approx(fmaf(__uint_as_float(s[j + 1]), p.scale_log2, -shift));
+                            if (!whole) {
+                                a = bits[c] >> j & 1u ? a : 0.f;
+                                b = bits[c] >> (j + 1) & 1u ? b : 0.f;
+                            }
+                            total += a + b;
+                            weights[j / 2] = Kind<T>::pack(a, b);
+                        }
+                        tensor_store16(scores + 16 * c, weights);
+                    }
+                    tensor_wait_store();
+                }
+                tensor_fence_before();
+                __syncwarp();
+                if (lane == 0) barrier_arrive(p_full(slot));
+            }
+            if (!__all_sync(0xffffffffu, barrier_wait(o_full(slot), ends & 1, failed))) goto finish;
+            ++ends;
+            tensor_fence_after();
+            if (!idle) {
+                float* partial;
+                float2* stat;
+                if (item.first) {
+                    // Rows of a head in token order: for an own item behind those of its request's first token.
+                    const int64_t row = item.head * p.head_rows +
+                                        (item.prefix ? item.row + item_row
+                                                     : token * p.group + (head - item.head * p.group));
+                    partial = (item.prefix ? p.prefix_out : p.own_out) + row * kDim;
+                    stat = (item.prefix ? p.prefix_stat : p.own_stat) + row;
+                } else {
+                    const int64_t row = static_cast<int64_t>(blockIdx.x) * 2 * kRows + item_row;
+                    partial = p.next_out + row * kDim;
+                    stat = p.next_stat + row;
+                }
+#pragma unroll 1
+                for (int c = 0; c < kDim / 32; ++c) {
+                    uint32_t o[32];
+                    tensor_load32(output + 32 * c, o);
+                    tensor_wait_load();
+                    if (present) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4) {
+                            *reinterpret_cast<uint4*>(partial + 32 * c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                        }
+                    }
+                }
+                if (present) *stat = make_float2(top, total);
+                tensor_fence_before();
+            }
+        }
+    } else if (warp < 12) {
+        // ------------------------------------------------------------ gather
+        const int part = warp - 8;  // rows 32 * part .. of every operand
+        constexpr int kLanes = kDim / 8;        // lanes a row (16 bytes each)
+        constexpr int kAtOnce = 32 / kLanes;    // rows a step
+        const int chunk = lane % kLanes, sub = lane / kLanes;
+        const char* k_plane = static_cast<const char*>(p.k_plane);
+        const char* v_plane = static_cast<const char*>(p.v_plane);
+        constexpr int kGroups = 2 * L::kStages;  // most copy groups in flight
+        uint32_t signals[kGroups] = {};          // barriers of the groups in flight, oldest first
+        int pending = 0;
+        uint32_t k_uses = 0, q_uses[2] = {0, 0};
+        // Complete the oldest group and tell its barrier.
+        const auto signal_oldest = [&]() {
+            switch (pending) {
+                case 1: copies_wait<0>(); break;
+                case 2: copies_wait<1>(); break;
+                case 3: copies_wait<2>(); break;
+                case 4: copies_wait<3>(); break;
+                case 5: copies_wait<4>(); break;
+                case 6: copies_wait<5>(); break;
+                case 7: copies_wait<6>(); break;
+                default: copies_wait<7>(); break;
+            }
+            fence_async_shared();
+            __syncwarp();
+            if (lane == 0) barrier_arrive(signals[0]);
+#pragma unroll
+            for (int i = 0; i + 1 < kGroups; ++i) signals[i] = signals[i + 1];
+            --pending;
+        };
+        // Wait for room, telling what has arrived meanwhile (the room may depend on it).
+        const auto acquire = [&](uint32_t barrier, uint32_t parity) {
+            if (pending == kGroups) signal_oldest();
+            while (!__all_sync(0xffffffffu, barrier_try(barrier, parity))) {
+                if (pending) {
+                    signal_oldest();
+                } else if (!__all_sync(0xffffffffu, barrier_wait(barrier, parity, failed))) {
+                    return false;
+                }
+            }
+            return true;
+        };
+        const auto launched = [&](uint32_t barrier) {
+            copies_commit();
+#pragma unroll
+            for (int i = 0; i < kGroups; ++i) {
+                if (i == pending) signals[i] = barrier;
+            }
+            ++pending;
+        };
+        const auto target = [&](uint32_t operand, int row) {
+            return operand + (chunk >> 3) * L::kBlock + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+        };
+        while (next_item(p, plan, walk, item)) {
+            const bool both = item.rows > kRows;
+            const int64_t first_token = item.prefix ? 0 : request_at(p, item.request).begin;
+            // Queries of the slots the item uses.
+            for (int half = 0; half < (both ? 2 : 1); ++half) {
+                const int slot = both ? half : turn;
+                if (!acquire(q_empty(slot), (q_uses[slot] & 1) ^ 1)) goto finish;
+                ++q_uses[slot];
+                const uint32_t operand = base + L::kQuery + slot * L::kOperand;
+                for (int i = 0; i < 32; i += kAtOnce) {
+                    const int row = part * 32 + i + sub;
+                    if (half * kRows + part * 32 + i >= item.rows) break;
+                    const int64_t local = item.row + half * kRows + row;
+                    if (half * kRows + row < item.rows) {
+                        const int64_t at = local / p.group;
+                        const int head = item.head * p.group + static_cast<int>(local - at * p.group);
+                        const int64_t token = first_token + at;
+                        const char* source = static_cast<const char*>(p.query) +
+                                             2 * (token * p.q_token + head * p.q_head) + 16 * chunk;
+                        copy16_async(target(operand, row), source, 16);
+                    }
+                }
+                launched(q_full(slot));
+            }
+            turn ^= 1;
+            const int64_t table_row =
+                item.prefix ? p.source_row : (p.rows ? load_index(p.rows, p.rows_es, item.request) : item.request);
+            const char* keys = k_plane + 2 * item.head * p.k_head + 16 * chunk;
+            const char* values = v_plane + 2 * item.head * p.v_head + 16 * chunk;
+            for (int64_t t = item.low; t < item.high; ++t, ++k_uses) {
+                const int64_t position = item.begin + t * kTile + part * 32 + lane;
+                const int64_t own = position < item.end ? slot_of(p, table_row, static_cast<uint32_t>(position)) : -1;
+                const uint32_t there = __ballot_sync(0xffffffffu, own >= 0);
+                const int stage = k_uses % L::kStages;
+                const uint32_t parity = ((k_uses / L::kStages) & 1) ^ 1;
+                if (!acquire(k_empty(stage), parity)) goto finish;
+                if (lane == 0) masks[(k_uses % kMaskRing) * 4 + part] = there;
+                const int found = static_cast<int>(own);
+                uint32_t operand = base + L::kKeys + stage * L::kOperand;
+#pragma unroll 8
+                for (int i = 0; i < 32; i += kAtOnce) {
+                    const int row = i + sub;
+                    const int slot = __shfl_sync(0xffffffffu, found, row);
+                    const char* source = slot >= 0 ? keys + 2 * (slot * p.k_slot) : static_cast<const char*>(p.query);
+                    copy16_async(target(operand, part * 32 + row), source, slot >= 0 ? 16 : 0);
+                }
+                launched(k_full(stage));
+                if (!acquire(v_empty(stage), parity)) goto finish;
+                operand = base + L::kValues + stage * L::kOperand;
+#pragma unroll 8
+                for (int i = 0; i < 32; i += kAtOnce) {
+                    const int row = i + sub;
+                    const int slot = __shfl_sync(0xffffffffu, found, row);
+                    const char* source = slot >= 0 ? values + 2 * (slot * p.v_slot) : static_cast<const char*>(p.query);
+                    copy16_async(target(operand, part * 32 + row), source, slot >= 0 ? 16 : 0);
+                }
+                launched(v_full(stage));
+            }
+        }
+        while (pending) signal_oldest();
+    } else if (warp == 12 && lane == 0) {
+        // ------------------------------------------------------------ products
+        constexpr uint32_t kScoreProduct = mma_descriptor(Kind<T>::kBf16, kRows, kTile, false);
+        constexpr uint32_t kOutputProduct = mma_descriptor(Kind<T>::kBf16, kRows, kDim, true);
+        uint32_t k_uses = 0, q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
+        // The second product of a tile is issued after the first one of the next, unless both
+        // use the same slot (whose scores it reads).
+        struct {
+            bool waiting;
+            int slot;
+            uint32_t uses;  // of the K and V stages
+            bool begins, ends, opens, closes;  // first / last tile of the item; first / last slot of the tile
+        } later{};
+        const auto second = [&]() {
+            later.waiting = false;
+            const int slot = later.slot, stage = later.uses % L::kStages;
+            if (!barrier_wait(p_full(slot), p_uses[slot] & 1, failed)) return false;
+            ++p_uses[slot];
+            if (later.opens && !barrier_wait(v_full(stage), (later.uses / L::kStages) & 1, failed)) return false;
+            tensor_fence_after();
+            const uint64_t values = shared_operand(base + L::kValues + stage * L::kOperand, L::kBlock);
+            const uint32_t d = tensor + 256 + slot * 128, weights = tensor + slot * kTile;
+#pragma unroll
+            for (int k = 0; k < kTile / 16; ++k) {
+                mma_tensor(d, weights + 8 * k, values + k * (16 * 128 >> 4), kOutputProduct, !later.begins || k > 0);
+            }
+            if (later.closes) mma_commit(v_empty(stage));
+            if (later.ends) mma_commit(o_full(slot));
+            return true;
+        };
+        bool fine = true;
+        while (fine && next_item(p, plan, walk, item)) {
+            const bool both = item.rows > kRows;
+            const int only = turn;
+            turn ^= 1;
+            for (int64_t t = item.low; fine && t < item.high; ++t, ++k_uses) {
+                const int stage = k_uses % L::kStages;
+                for (int half = 0; half < (both ? 2 : 1); ++half) {
+                    const int slot = both ? half : only;
+                    if (later.waiting && later.slot == slot && !(fine = second())) break;
+                    if (half == 0 && !(fine = barrier_wait(k_full(stage), (k_uses / L::kStages) & 1, failed))) break;
+                    if (t == item.low) {
+                        if (!(fine = barrier_wait(q_full(slot), q_uses[slot] & 1, failed))) break;
+                        ++q_uses[slot];
+                    }
+                    tensor_fence_after();
+                    const uint64_t queries = shared_operand(base + L::kQuery + slot * L::kOperand, 16);
+                    const uint64_t keys = shared_operand(base + L::kKeys + stage * L::kOperand, 16);
+#pragma unroll
+                    for (int k = 0; k < kDim / 16; ++k) {
+                        const uint32_t step = (k / 4) * (L::kBlock >> 4) + (k % 4) * 2;
+                        mma_shared(tensor + slot * kTile, queries + step, keys + step, kScoreProduct, k > 0);
+                    }
+                    mma_commit(s_full(slot));
+                    const bool last = !both || half == 1;
+                    if (last) mma_commit(k_empty(stage));
+                    if (t + 1 == item.high) mma_commit(q_empty(slot));
+                    if (later.waiting && !(fine = second())) break;
+                    later.waiting = true;
+                    later.slot = slot;
+                    later.uses = k_uses;
+                    later.begins = t == item.low;
+                    later.ends = t + 1 == item.high;
+                    later.opens = half == 0;
+                    later.closes = last;
+                }
+            }
+        }
+        if (fine && later.waiting) fine = second();
+        // Nothing may still use tensor memory when it is freed, whatever happened above.
+        mma_commit(drain);
+        volatile uint32_t ran_out = 0;
+        barrier_wait(drain, 0, &ran_out);
+    }
+finish:
+    copies_wait<0>();
+    __syncthreads();
+    allow_dependents();
+    if (threadIdx.x == 0) p.failed[blockIdx.x] = *failed;
+    if (warp == 12) {
+        __syncwarp();
+        tensor_free(tensor, 512);
     }
 }
 
+// ---------------------------------------------------------------- joining the parts
+
+// A warp per token and query head: the parts (m_i, l_i, O_i) of a row join as
+// sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i with m = max m_i.
 template <typename T, int kDim>
-void launch_rows(const AttentionParams& p, cudaStream_t stream) {
-    const int64_t items = p.tokens * p.query_heads;
-    const int64_t grid = (items + 3) / 4;
-    require(grid <= INT32_MAX, "too many query rows");
-    launch_dependent(prefix_rows_kernel<T, kDim>, dim3(static_cast<unsigned>(grid)), dim3(128), 0, stream,
+__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ AttentionParams p) {
+    constexpr int kPer = kDim / 32;
+    grid_dependency_wait();
+    allow_dependents();
+    const int64_t query_heads = static_cast<int64_t>(p.kv_heads) * p.group;
+    const int64_t index = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
+    const int64_t n = index / query_heads;
+    const int head = static_cast<int>(index - n * query_heads);
+    const unsigned lane = lane_id();
+    int64_t b;
+    Request request;
+    if (!request_of(p, n, b, request)) return;
+    const int kv_head = head / p.group, g = head - kv_head * p.group;
+    float top = -INFINITY, total = 0.f;
+    float acc[kPer] = {};
+    uint32_t bad = 0;  // a wait ran out in a block whose part is needed
+    const auto join = [&](int64_t block, const float* out, const float2* stat, int64_t row) {
+        const float2 part = stat[row];
+        bad |= p.failed[block];
+        if (part.y == 0.f) return;  // the row sees nothing there
+        const float higher = fmaxf(top, part.x);
+        const float mine = top == -INFINITY ? 0.f : exp2_approx(top - higher), its = exp2_approx(part.x - higher);
+        top = higher;
+        total = total * mine + part.y * its;
+        const float* values = out + row * kDim + lane * kPer;
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * mine + values[i] * its;
+    };
+    const int64_t prefix_cost = item_cost(p.prefix_tiles);
+    const int64_t prefix_items = p.prefix_tiles ? p.prefix_row_tiles * p.kv_heads : 0;
+    const int64_t prefix_total = prefix_cost * prefix_items;
+    const uint32_t first_entry = p.plan_first[b];
+    const int64_t local = (n - request.begin) * p.group + g;
+    const int64_t entry = first_entry + local / (2 * kRows);
+    const int64_t entries_end = p.plan_first[p.batch];
+    const int64_t total_cost = prefix_total + static_cast<int64_t>(p.plan_cost[entries_end]) * p.kv_heads;
+    const auto join_item = [&](int64_t start, int64_t tiles, const float* out, const float2* stat, int64_t row, int r) {
+        if (tiles <= 0) return;
+        int64_t block = ((start + 1) * p.blocks - 1) / total_cost;  // the share that holds `start`
+        join(block, out, stat, row);
+        int64_t done = first_tile(share_begin(block + 1, total_cost, p.blocks), start, tiles);
+        while (done < tiles) {
+            ++block;
+            const int64_t high = first_tile(share_begin(block + 1, total_cost, p.blocks), start, tiles);
+            if (high > done) join(block, p.next_out, p.next_stat, block * 2 * kRows + r);
+            done = high;
+        }
+    };
+    const int64_t head_row = n * p.group + g;
+    join_item(prefix_cost * (kv_head * p.prefix_row_tiles + head_row / (2 * kRows)), prefix_items ? p.prefix_tiles : 0,
+              p.prefix_out, p.prefix_stat, kv_head * p.head_rows + head_row, static_cast<int>(head_row % (2 * kRows)));
+    if (entry < entries_end) {
+        const int64_t cost = p.plan_cost[entry + 1] - p.plan_cost[entry];
+        join_item(prefix_total + static_cast<int64_t>(p.plan_cost[entry]) * p.kv_heads + kv_head * cost,
+                  cost ? (cost - kItemCost) / kTileCost : 0, p.own_out, p.own_stat, kv_head * p.head_rows + head_row,
+                  static_cast<int>(local % (2 * kRows)));
+    }
+    const float scale = bad ? NAN : (total == 0.f ? 0.f : 1.f / total);
+    T* o = static_cast<T*>(p.out) + n * p.o_token + head * p.o_head + lane * kPer;
+#pragma unroll
+    for (int i = 0; i < kPer; i += 2) {
+        *reinterpret_cast<uint32_t*>(o + i) = Kind<T>::pack(acc[i] * scale, acc[i + 1] * scale);
+    }
+    if (p.lse && lane == 0) {
+        p.lse[n * p.lse_token + head * p.lse_head] =
+            bad ? NAN : (total == 0.f ? -INFINITY : (top + log2f(total)) * 0.69314718055994531f);
+    }
+}
+
+// ---------------------------------------------------------------- host side
+
+struct Workspace {
+    int64_t prefix_out, own_out, next_out, prefix_stat, own_stat, next_stat, plan_cost, plan_first, failed, bytes;
+};
+
+Workspace workspace_of(int64_t tokens, int64_t batch, int64_t query_heads, int64_t dim, int64_t blocks) {
+    Workspace w{};
+    int64_t at = 0;
+    const auto take = [&](int64_t bytes) {
+        const int64_t here = at;
+        at += (bytes + 255) / 256 * 256;
+        return here;
+    };
+    const int64_t rows = tokens * query_heads, next = blocks * 2 * kRows;
+    w.prefix_out = take(rows * dim * 4);
+    w.own_out = take(rows * dim * 4);
+    w.next_out = take(next * dim * 4);
+    w.prefix_stat = take(rows * 8);
+    w.own_stat = take(rows * 8);
+    w.next_stat = take(next * 8);
+    w.plan_cost = take((kMaxEntries + 2) * 4);
+    w.plan_first = take((batch + 1) * 4);
+    w.failed = take(blocks * 4);
+    w.bytes = at;
+    return w;
+}
+
+template <typename T, int kDim>
+void launch(const AttentionParams& p, int device, cudaStream_t stream) {
+    using L = Layout<kDim>;
+    static_assert(L::kBytes <= 232448, "shared memory of one block");
+    cuda_check(cudaFuncSetAttribute(attention_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes),
+               "attention shared memory");
+    launch_dependent(attention_kernel<T, kDim>, dim3(static_cast<unsigned>(p.blocks)), dim3(kThreads), L::kBytes, stream,
                      "shared_prefix_attention launch", p);
+    const int64_t warps = p.tokens * p.kv_heads * p.group;
+    launch_dependent(combine_kernel<T, kDim>, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0, stream,
+                     "shared_prefix_attention join", p);
+    (void)device;
+}
+
+void check_shape(int64_t tokens, int64_t batch, int query_heads, int kv_heads, int head_dim) {
+    require(tokens >= 0 && batch >= 0, "negative attention dimensions");
+    require(head_dim == 64 || head_dim == 128, "head_dim must be 64 or 128");
+    require(kv_heads >= 1 && query_heads >= 1 && query_heads % kv_heads == 0,
+            "query_heads must be a positive multiple of kv_heads");
+    require(query_heads <= 65535, "more than 65535 query heads");
+    const int64_t group = query_heads / kv_heads;
+    require(batch <= kMaxEntries && tokens <= INT32_MAX / query_heads &&
+                batch + (tokens * group + 2 * kRows - 1) / (2 * kRows) <= kMaxEntries,
+            "more than EKV_ATTENTION_MAX_ROW_TILES row tiles in one call");
 }
 
 }  // namespace
@@ -146,10 +927,8 @@ extern "C" int ekv_shared_prefix_workspace(int64_t tokens, int64_t batch, int qu
     using namespace ekv;
     return guarded([&] {
         require(bytes != nullptr, "null pointer argument");
-        require(tokens >= 0 && batch >= 0 && query_heads >= 0 && kv_heads >= 0, "negative attention dimensions");
-        (void)head_dim;
-        (void)device;
-        *bytes = 0;
+        check_shape(tokens, batch, query_heads, kv_heads, head_dim);
+        *bytes = tokens && batch ? workspace_of(tokens, batch, query_heads, head_dim, sm_count(device)).bytes : 0;
     });
 }
 
@@ -166,13 +945,12 @@ extern "C" int ekv_shared_prefix_attention(
     void* workspace, int64_t workspace_bytes, int device, void* stream) {
     using namespace ekv;
     return guarded([&] {
-        require(tokens >= 0 && batch >= 0 && slots >= 0 && table_rows >= 0 && table_width >= 0,
-                "negative attention dimensions");
+        require(slots >= 0 && slots <= INT32_MAX && table_rows >= 0 && table_width >= 0 && tokens >= 0 && batch >= 0,
+                "negative attention dimensions, or more than 2^31 - 1 slots");
         require(dtype == EKV_BF16 || dtype == EKV_FP16, "dtype must be EKV_BF16 or EKV_FP16");
-        require(head_dim == 64 || head_dim == 128, "head_dim must be 64 or 128");
-        require(kv_heads >= 1 && query_heads >= 1 && query_heads % kv_heads == 0,
-                "query_heads must be a positive multiple of kv_heads");
+        check_shape(tokens, batch, query_heads, kv_heads, head_dim);
         require(page_size >= 1 && page_size <= INT32_MAX, "page_size outside [1, 2^31)");
+        require(table_width <= INT32_MAX / page_size, "a table row covers more than 2^31 - 1 positions");
         require(shared_tokens >= 0 && shared_tokens <= table_width * page_size,
                 "shared_tokens outside the table's positions");
         require(!shared_tokens || (source_row >= 0 && source_row < table_rows), "source row is outside the block table");
@@ -190,9 +968,18 @@ extern "C" int ekv_shared_prefix_attention(
         if (rows) check_esize(rows_esize, "rows");
         check_esize(lengths_esize, "lengths");
         if (query_starts) check_esize(starts_esize, "query_starts");
-        (void)workspace;
-        (void)workspace_bytes;
+        const int group = query_heads / kv_heads;
+        const int64_t head_rows = tokens * group;
+        // The plan's running cost of one head is held in 32 bits.
+        const int64_t most_tiles = (table_width * page_size + kTile - 1) / kTile;
+        const int64_t most_entries = batch + (head_rows + 2 * kRows - 1) / (2 * kRows);
+        require((most_tiles * kTileCost + kItemCost) <= static_cast<int64_t>(UINT32_MAX) / most_entries,
+                "the block table is too wide for this batch");
         bind_device(device);
+        const int blocks = sm_count(device);
+        const Workspace w = workspace_of(tokens, batch, query_heads, head_dim, blocks);
+        require(workspace != nullptr && workspace_bytes >= w.bytes, "workspace is too small");
+        require(reinterpret_cast<uint64_t>(workspace) % 256 == 0, "workspace must be 256-byte aligned");
         AttentionParams p{};
         p.query = query;
         p.k_plane = k_plane;
@@ -217,23 +1004,42 @@ extern "C" int ekv_shared_prefix_attention(
         p.table_rows = table_rows;
         p.table_width = table_width;
         p.table_stride = table_row_stride;
-        p.page_size = page_size;
+        p.page_size = static_cast<uint32_t>(page_size);
+        p.page_log2 = -1;
+        for (int bit = 0; bit < 31; ++bit) {
+            if (page_size == int64_t{1} << bit) p.page_log2 = bit;
+        }
         p.tokens = tokens;
         p.batch = batch;
         p.shared = shared_tokens;
         p.source_row = source_row;
-        p.query_heads = query_heads;
-        p.group = query_heads / kv_heads;
+        p.kv_heads = kv_heads;
+        p.group = group;
         p.table_es = table_esize;
         p.rows_es = rows_esize;
         p.len_es = lengths_esize;
         p.starts_es = starts_esize;
         p.scale_log2 = scale * 1.4426950408889634f;
+        p.head_rows = head_rows;
+        p.prefix_row_tiles = (head_rows + 2 * kRows - 1) / (2 * kRows);
+        p.prefix_tiles = (shared_tokens + kTile - 1) / kTile;
+        p.blocks = blocks;
+        char* at = static_cast<char*>(workspace);
+        p.prefix_out = reinterpret_cast<float*>(at + w.prefix_out);
+        p.own_out = reinterpret_cast<float*>(at + w.own_out);
+        p.next_out = reinterpret_cast<float*>(at + w.next_out);
+        p.prefix_stat = reinterpret_cast<float2*>(at + w.prefix_stat);
+        p.own_stat = reinterpret_cast<float2*>(at + w.own_stat);
+        p.next_stat = reinterpret_cast<float2*>(at + w.next_stat);
+        p.plan_cost = reinterpret_cast<uint32_t*>(at + w.plan_cost);
+        p.plan_first = reinterpret_cast<uint32_t*>(at + w.plan_first);
+        p.failed = reinterpret_cast<uint32_t*>(at + w.failed);
         const auto cstream = static_cast<cudaStream_t>(stream);
         if (dtype == EKV_BF16) {
-            head_dim == 128 ? launch_rows<__nv_bfloat16, 128>(p, cstream) : launch_rows<__nv_bfloat16, 64>(p, cstream);
+            head_dim == 128 ? launch<__nv_bfloat16, 128>(p, device, cstream)
+                            : launch<__nv_bfloat16, 64>(p, device, cstream);
         } else {
-            head_dim == 128 ? launch_rows<__half, 128>(p, cstream) : launch_rows<__half, 64>(p, cstream);
+            head_dim == 128 ? launch<__half, 128>(p, device, cstream) : launch<__half, 64>(p, device, cstream);
         }
         check_launch("shared_prefix_attention launch");
     });

@@ -1,0 +1,157 @@
+// sm_100a tensor-core, tensor-memory and barrier primitives (inline PTX).
+#pragma once
+
+#include "common.cuh"
+
+namespace ekv {
+
+// ---------------------------------------------------------------- mbarriers
+
+__device__ __forceinline__ uint32_t shared_address(const void* pointer) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(pointer));
+}
+
+__device__ __forceinline__ void barrier_init(uint32_t barrier, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(barrier), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ void barrier_arrive(uint32_t barrier) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(barrier) : "memory");
+}
+
+__device__ __forceinline__ bool barrier_try(uint32_t barrier, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(barrier), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
+__device__ __forceinline__ uint64_t device_nanoseconds() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+
+// Nanoseconds after which a wait inside a kernel gives up.
+constexpr uint64_t kWaitLimit = 4000000000ull;
+
+// Wait for the phase of `parity` to complete.  False (and *failed set) when kWaitLimit passes or
+// another thread of the block has given up.
+__device__ __forceinline__ bool barrier_wait(uint32_t barrier, uint32_t parity, volatile uint32_t* failed) {
+    for (int i = 0; i < 64; ++i) {
+        if (barrier_try(barrier, parity)) return true;
+    }
+    const uint64_t begin = device_nanoseconds();
+    while (true) {
+        for (int i = 0; i < 256; ++i) {
+            if (barrier_try(barrier, parity)) return true;
+        }
+        if (*failed) return false;
+        if (device_nanoseconds() - begin > kWaitLimit) {
+            *failed = 1;
+            return false;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- proxies and asynchronous copies
+
+__device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// 16 bytes global -> shared; zeros when `bytes` is 0 (then nothing is read).
+__device__ __forceinline__ void copy16_async(uint32_t target, const void* source, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(target), "l"(source), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void copies_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+
+// ---------------------------------------------------------------- tensor memory
+
+__device__ __forceinline__ void tensor_alloc(uint32_t shared_slot, uint32_t columns) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(shared_slot), "r"(columns)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+}
+__device__ __forceinline__ void tensor_free(uint32_t address, uint32_t columns) {
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(address), "r"(columns));
+}
+__device__ __forceinline__ void tensor_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tensor_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
+__device__ __forceinline__ void tensor_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tensor_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+#define EKV_R8(r, i) "=r"(r[i]), "=r"(r[i + 1]), "=r"(r[i + 2]), "=r"(r[i + 3]), "=r"(r[i + 4]), "=r"(r[i + 5]), "=r"(r[i + 6]), "=r"(r[i + 7])
+#define EKV_I8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
+
+// This lane's 32 consecutive columns (the warp's 32 lanes are tensor-memory lanes).
+__device__ __forceinline__ void tensor_load32(uint32_t address, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : EKV_R8(r, 0), EKV_R8(r, 8), EKV_R8(r, 16), EKV_R8(r, 24)
+        : "r"(address));
+}
+__device__ __forceinline__ void tensor_store32(uint32_t address, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::EKV_I8(r, 0),
+        EKV_I8(r, 8), EKV_I8(r, 16), EKV_I8(r, 24), "r"(address)
+        : "memory");
+}
+__device__ __forceinline__ void tensor_store16(uint32_t address, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::EKV_I8(
+            r, 0),
+        EKV_I8(r, 8), "r"(address)
+        : "memory");
+}
+
+// ---------------------------------------------------------------- matrix products
+
+// Instruction descriptor of a 16-bit product with 32-bit accumulation (M x N).
+__host__ __device__ constexpr uint32_t mma_descriptor(bool bf16, int m, int n, bool b_rows_are_k) {
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | (b_rows_are_k ? 1u << 16 : 0u) |
+           (static_cast<uint32_t>(n >> 3) << 17) | (static_cast<uint32_t>(m >> 4) << 24);
+}
+
+// Shared-memory operand of 128-byte rows, swizzled by 128 bytes, in blocks of 8 rows (1024
+// bytes).  `block_stride`: bytes from one 128-byte wide column block to the next (used where a
+// row of 128 bytes runs along the operand's outer dimension).
+__device__ __forceinline__ uint64_t shared_operand(uint32_t address, uint32_t block_stride) {
+    return static_cast<uint64_t>((address & 0x3ffffu) >> 4) | (static_cast<uint64_t>(block_stride >> 4) << 16) |
+           (static_cast<uint64_t>(1024 >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+__device__ __forceinline__ void mma_shared(uint32_t d, uint64_t a, uint64_t b, uint32_t descriptor, bool accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}" ::"r"(d),
+        "l"(a), "l"(b), "r"(descriptor), "r"(static_cast<uint32_t>(accumulate))
+        : "memory");
+}
+// The left operand in tensor memory (two 16-bit values to a column).
+__device__ __forceinline__ void mma_tensor(uint32_t d, uint32_t a, uint64_t b, uint32_t descriptor, bool accumulate) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}" ::"r"(d),
+        "r"(a), "l"(b), "r"(descriptor), "r"(static_cast<uint32_t>(accumulate))
+        : "memory");
+}
+// One arrival at `barrier` when every product this thread has issued is complete.
+__device__ __forceinline__ void mma_commit(uint32_t barrier) {
+    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(barrier) : "memory");
+}
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+}  // namespace ekv

@@ -20,7 +20,7 @@ import math
 
 import torch
 
-from ._lib import call, index_esize, require_cuda, stream_handle
+from ._lib import ATTENTION_MAX_ROW_TILES, call, index_esize, require_cuda, stream_handle
 from .block_tables import _vector
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}  # EKV_BF16, EKV_FP16
@@ -88,6 +88,8 @@ def _bind(query, k_plane, v_plane, block_tables, lengths, page_size, shared_toke
     starts_es = 8 if query_starts is None else _vector(query_starts, "query_starts", batch + 1)
     if query_starts is None and tokens != batch:
         raise ValueError("without query_starts every request has one query token")
+    if batch + -(-tokens * query_heads // kv_heads // 256) > ATTENTION_MAX_ROW_TILES:
+        raise ValueError("more requests and query tokens than one call takes")
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
     if not 0.0 < scale < 3.0e38:
         raise ValueError("scale must be positive and finite")
@@ -136,6 +138,7 @@ def shared_prefix_attention(query: torch.Tensor, k_plane: torch.Tensor, v_plane:
     slot (a negative page, one outside the planes, past the table) is skipped.  A query token
     that sees no position gets zeros and a log-sum-exp of minus infinity.
 
+    One call takes up to ``ATTENTION_MAX_ROW_TILES`` (2048) row tiles: one per request and 256 query rows of a KV head.
     ``scale`` defaults to ``1 / sqrt(dim)``; ``lse`` is float32 [tokens, query_heads], the natural
     logarithm of the sum of the exponentials.  Scores, maxima, sums and outputs are held in 32 bits.
     """

@@ -552,13 +552,16 @@ int ekv_append_rows(
  *     lse[n, h] = log sum_t exp(scale * q.k_t)          (lse may be NULL)
  * and 0 / -infinity for a token that sees nothing.  Tokens of no request are not
  * written.  dtype is that of query, planes and out; head_dim 64 or 128; strides in
- * elements, the head dimension contiguous, every row 16-byte aligned.  batch is at
- * most EKV_ATTENTION_MAX_BATCH.  workspace: ekv_shared_prefix_workspace's bytes,
- * 256-byte aligned device memory that no other call uses at the same time.
+ * elements, the head dimension contiguous, every row 16-byte aligned.  batch +
+ * ceil(tokens * query_heads / kv_heads / 256) is at most
+ * EKV_ATTENTION_MAX_ROW_TILES.  workspace: ekv_shared_prefix_workspace's bytes of
+ * 256-byte aligned device memory that no other call uses at the same time; its
+ * content need not be initialised or kept.  The waits inside the kernel are bounded
+ * (4 s); rows that one running out affects are NaN.
  */
 #define EKV_BF16 0
 #define EKV_FP16 1
-#define EKV_ATTENTION_MAX_BATCH 4096
+#define EKV_ATTENTION_MAX_ROW_TILES 2048
 int ekv_shared_prefix_workspace(
     int64_t tokens, int64_t batch, int query_heads, int kv_heads, int head_dim, int device, int64_t* bytes);
 int ekv_shared_prefix_attention(

@@ -112,6 +112,9 @@ def _attend():
     (dict(rows=torch.zeros(2, dtype=torch.int32)), ValueError, "3 entries"),
     (dict(query_starts=torch.zeros(3, dtype=torch.int32)), ValueError, "4 entries"),
     (dict(lengths=torch.ones(2, dtype=torch.int32)), ValueError, "one query token"),
+    (dict(query=torch.zeros(1 << 18, 4, 1, dtype=torch.bfloat16).expand(-1, -1, 64)), ValueError, "last dimension"),
+    (dict(lengths=torch.ones(2049, dtype=torch.int32), query=torch.zeros(2049, 4, 64, dtype=torch.bfloat16)), ValueError,
+     "one call takes"),
     (dict(scale=0.0), ValueError, "scale"),
     (dict(scale=float("nan")), ValueError, "scale"),
     (dict(scale=float("inf")), ValueError, "scale"),
@@ -154,6 +157,8 @@ def _attention_args(**change):
     (dict(source=3), b"source row"), (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale"),
     (dict(batch=2), b"one query token"), (dict(query=None), b"null pointer"), (dict(query=4098), b"16-byte"),
     (dict(ks=(127, 64)), b"16-byte"), (dict(table_es=2), b"element size"),
+    (dict(tokens=2049, batch=2049), b"ROW_TILES"), (dict(tokens=1 << 20, starts=4096), b"ROW_TILES"),
+    (dict(width=1 << 30, page=1, tokens=2000, batch=2000), b"too wide"),
 ])
 def test_c_entry_refuses_before_touching_a_device(change, message, library_path):
     from ekv_b200 import _lib
@@ -161,6 +166,7 @@ def test_c_entry_refuses_before_touching_a_device(change, message, library_path)
     lib = _lib.library(str(library_path))
     assert lib.ekv_shared_prefix_attention(*_attention_args(**change)) == -1
     assert message in lib.ekv_error(), lib.ekv_error()
+    assert lib.ekv_bitmap_and(None, 1, 0, None, 0, None) == 0 and lib.ekv_error() == b""  # the next call clears it
 
 
 def test_other_c_entries_refuse_and_pass_empty_work(library_path):
@@ -180,8 +186,8 @@ def test_other_c_entries_refuse_and_pass_empty_work(library_path):
     assert lib.ekv_append_rows(planes, planes, 257, 16, 16, 16, p, 4, 1, 1, 0, None) == -1 and b"plane" in lib.ekv_error()
     assert lib.ekv_append_rows(planes, planes, 1, 16, 16, 16, None, 4, 1, 1, 0, None) == -1 and b"null" in lib.ekv_error()
     assert lib.ekv_append_rows(planes, planes, 1, 16, 16, 16, p, 2, 1, 1, 0, None) == -1 and b"element" in lib.ekv_error()
-    assert lib.ekv_append_rows(planes, planes, 1, 16, 16, 16, None, 4, 0, 1, 0, None) == 0
     assert lib.ekv_append_rows(planes, planes, 1, -1, 16, 16, p, 4, 1, 1, 0, None) == -1
+    assert lib.ekv_append_rows(planes, planes, 1, 16, 16, 16, None, 4, 0, 1, 0, None) == 0
 
 
 def test_restatement_known_answers():
