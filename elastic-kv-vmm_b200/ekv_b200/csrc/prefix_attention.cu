@@ -21,7 +21,11 @@
 // 128 positions, 32-bit sums in tensor memory), a softmax thread per row between them.
 // Roles by warp: 0-3 and 4-7 softmax of row tile halves ("slots") 0 and 1; 8-11 gather the K and V rows
 // into swizzled shared memory (cp.async, 16 bytes a lane, whole rows; slots resolved through
-// the table, zeros for positions without one); 12 issues the products.  A 256-row item uses both slots
+// the table, zeros for positions without one); 12 and 13 issue the products of slots 0 and 1 (one
+// thread each, so that the waits and commits of one fall beside the other's products); 14 walks the
+// block's items and hands them to the others through a small ring; 15 passes on what the gather
+// has written, with the fence between ordinary writes and the tensor cores' reads.
+// A 256-row item uses both slots
 // on the same K and V; smaller items alternate between them, so one's softmax runs beside
 // the other's products.  The maximum a row's weights refer to is raised only when the tile's
 // maximum passes it by 2^8 (kRaise), which makes rescaling O rare; sums stay exact to 32 bits since the
@@ -37,11 +41,20 @@ namespace {
 
 constexpr int kRows = 128;           // rows of a slot (tensor-memory lanes)
 constexpr int kTile = 128;           // positions of a tile
-constexpr int kThreads = 512;
+constexpr int kGatherWarps = 4;
+constexpr int kGatherRows = kTile / kGatherWarps;  // rows of a tile one gather warp copies, one a lane to look up
+static_assert(kGatherRows == 32, "a lane resolves one row");
+constexpr int kThreads = 256 + 32 * kGatherWarps + 128;
+// Registers a thread: 512 threads start with 128; the softmax warps take what the others give
+// up, for the row of scores each of their threads holds.
+constexpr int kStartRegisters = 128, kSoftmaxRegisters = 184, kGatherRegisters = 72, kIssueRegisters = 72;
+static_assert(256 * kSoftmaxRegisters + 32 * kGatherWarps * kGatherRegisters + 128 * kIssueRegisters <=
+                  kThreads * kStartRegisters, "more registers than the block starts with");
 constexpr int kMaxEntries = EKV_ATTENTION_MAX_ROW_TILES;
 constexpr int kItemCost = 1;         // an item's start, in units of which ...
 constexpr int kTileCost = 2;         // ... a tile is kTileCost
-constexpr int kMaskRing = 8;          // more than the stages of any layout plus 1 (see the gather role)
+constexpr int kMaskRing = 8;         // more than the stages of any layout
+constexpr int kItemRing = 4;
 constexpr float kRaise = 8.f;
 
 struct AttentionParams {
@@ -56,14 +69,15 @@ struct AttentionParams {
     const void* starts;  // null: token b is request b's only one
     int64_t q_token, q_head, k_slot, k_head, v_slot, v_head, o_token, o_head, lse_token, lse_head;
     int64_t slots, table_rows, table_width, table_stride;
-    int64_t tokens, batch, shared, source_row;
+    int64_t tokens, batch, source_row;
     uint32_t page_size;
+    int shared;
     int page_log2;  // -1: not a power of two
     int kv_heads, group;
     int table_es, rows_es, len_es, starts_es;
     float scale_log2;  // scale * log2(e)
     // Derived: rows per KV head, prefix row tiles, prefix tiles.
-    int64_t head_rows, prefix_row_tiles, prefix_tiles;
+    int head_rows, prefix_row_tiles, prefix_tiles;
     int blocks;
     // Workspace.
     float* prefix_out;   // [kv_heads][head_rows][dim]: an item's first part
@@ -234,28 +248,30 @@ __device__ __forceinline__ int64_t share_begin(int64_t block, int64_t total, int
 
 // First tile at or behind position x of an item that begins at `start` (its tile t > 0 lies at
 // start + kItemCost + t * kTileCost).
-__device__ __forceinline__ int64_t first_tile(int64_t x, int64_t start, int64_t tiles) {
+__device__ __forceinline__ int first_tile(int64_t x, int64_t start, int tiles) {
     if (x <= start) return 0;
     int64_t t = (x - start - kItemCost + kTileCost - 1) / kTileCost;
     if (t < 1) t = 1;
-    return t < tiles ? t : tiles;
+    return t < tiles ? static_cast<int>(t) : tiles;
 }
 
-struct Item {
-    bool prefix;
-    bool first;          // this block has the item's first tile
+struct __align__(16) Item {
+    int prefix;
+    int first;      // this block has the item's first tile
     int head;
-    int rows;            // rows of the item, up to 256
-    int64_t request;     // own items
-    int64_t row;         // first row: of the head (prefix) or of the request (own)
-    int64_t low, high;   // tiles of this block
-    int64_t begin, end;  // positions of the whole item
+    int rows;       // rows of the item, up to 256; 0 ends the list
+    int row;        // first row: of the head (prefix) or of the request (own)
+    int low, high;  // tiles of this block
+    int begin, end; // positions of the whole item
+    int table_row;  // -1: no row of the table
+    int token;      // query token of row 0 of the head or request
+    int bias;       // own items: token i of the request sees bias + i positions
 };
 
 struct Walk {
     int64_t start, stop;  // this block's share
-    int64_t prefix_cost, prefix_items;
-    int64_t index;        // next prefix item
+    int prefix_cost, prefix_items;
+    int index;            // next prefix item
     uint32_t entry;
     int head;
 };
@@ -264,7 +280,7 @@ __device__ __forceinline__ Walk begin_walk(const AttentionParams& p, const Plan&
     Walk w;
     w.prefix_cost = item_cost(p.prefix_tiles);
     w.prefix_items = p.prefix_tiles ? p.prefix_row_tiles * p.kv_heads : 0;
-    const int64_t prefix_total = w.prefix_cost * w.prefix_items;
+    const int64_t prefix_total = static_cast<int64_t>(w.prefix_cost) * w.prefix_items;
     const int64_t total = prefix_total + static_cast<int64_t>(plan.cost[plan.entries]) * p.kv_heads;
     w.start = share_begin(blockIdx.x, total, p.blocks);
     w.stop = share_begin(blockIdx.x + 1, total, p.blocks);
@@ -272,7 +288,7 @@ __device__ __forceinline__ Walk begin_walk(const AttentionParams& p, const Plan&
     w.entry = 0;
     w.head = 0;
     if (w.start < prefix_total) {
-        w.index = w.start / w.prefix_cost;
+        w.index = static_cast<int>(w.start / w.prefix_cost);
     } else if (plan.entries) {
         // Last entry that begins at or before the share's start.
         const int64_t x = w.start - prefix_total;
@@ -295,23 +311,25 @@ __device__ __forceinline__ Walk begin_walk(const AttentionParams& p, const Plan&
 // The next item of which this block has a tile; false at the end of its share.
 __device__ __forceinline__ bool next_item(const AttentionParams& p, const Plan& plan, Walk& w, Item& item) {
     while (w.index < w.prefix_items) {
-        const int64_t start = w.index * w.prefix_cost;
+        const int64_t start = static_cast<int64_t>(w.index) * w.prefix_cost;
         if (start >= w.stop) return false;
-        const int64_t i = w.index++;
+        const int i = w.index++;
         item.low = first_tile(w.start, start, p.prefix_tiles);
         item.high = first_tile(w.stop, start, p.prefix_tiles);
         if (item.low >= item.high) continue;
-        const int64_t tile = i % p.prefix_row_tiles;
-        item.prefix = true;
+        item.prefix = 1;
         item.first = item.low == 0;
-        item.head = static_cast<int>(i / p.prefix_row_tiles);
-        item.row = tile * 2 * kRows;
-        item.rows = static_cast<int>(p.head_rows - item.row < 2 * kRows ? p.head_rows - item.row : 2 * kRows);
+        item.head = i / p.prefix_row_tiles;
+        item.row = (i - item.head * p.prefix_row_tiles) * 2 * kRows;
+        item.rows = p.head_rows - item.row < 2 * kRows ? p.head_rows - item.row : 2 * kRows;
+        item.table_row = static_cast<int>(p.source_row);
+        item.token = 0;
+        item.bias = 0;
         item.begin = 0;
         item.end = p.shared;
         return true;
     }
-    const int64_t prefix_total = w.prefix_cost * w.prefix_items;
+    const int64_t prefix_total = static_cast<int64_t>(w.prefix_cost) * w.prefix_items;
     while (w.entry < plan.entries) {
         const int64_t cost = plan.cost[w.entry + 1] - plan.cost[w.entry];
         const int64_t start = prefix_total + static_cast<int64_t>(plan.cost[w.entry]) * p.kv_heads + w.head * cost;
@@ -323,43 +341,40 @@ __device__ __forceinline__ bool next_item(const AttentionParams& p, const Plan& 
             w.head = 0;
         }
         if (!cost) continue;
-        const int64_t tiles = (cost - kItemCost) / kTileCost;
+        const int tiles = static_cast<int>((cost - kItemCost) / kTileCost);
         item.low = first_tile(w.start, start, tiles);
         item.high = first_tile(w.stop, start, tiles);
         if (item.low >= item.high) continue;
         const int64_t reach = p.table_width * p.page_size;
-        item.prefix = false;
+        item.prefix = 0;
         item.first = item.low == 0;
         item.head = head;
-        item.request = plan.request[e];
-        item.row = static_cast<int64_t>(plan.row_tile[e]) * 2 * kRows;
-        const int64_t left = (p.starts ? request_at(p, item.request).fresh : 1) * p.group - item.row;
-        item.rows = static_cast<int>(left < 2 * kRows ? left : 2 * kRows);
+        const int64_t b = plan.request[e];
+        const Request request = request_at(p, b);
+        item.row = plan.row_tile[e] * 2 * kRows;
+        const int left = static_cast<int>(request.fresh) * p.group - item.row;
+        item.rows = left < 2 * kRows ? left : 2 * kRows;
+        const int64_t table_row = p.rows ? load_index(p.rows, p.rows_es, b) : b;
+        item.table_row = table_row >= 0 && table_row < p.table_rows ? static_cast<int>(table_row) : -1;
+        item.token = static_cast<int>(request.begin);
+        item.bias = static_cast<int>(request.length - request.fresh + 1);
         item.begin = p.shared;
-        item.end = plan.end[e] < reach ? plan.end[e] : reach;
+        item.end = plan.end[e] < reach ? plan.end[e] : static_cast<int>(reach);
         return true;
     }
     return false;
 }
 
-// The query token and head of an item's row, and the positions it sees (all in [0, 2^31)).
-__device__ __forceinline__ bool row_of(const AttentionParams& p, const Item& item, int r, int64_t& token, int& head,
-                                       int64_t& seen) {
-    seen = 0;
+// Positions that an item's row sees; false for a row of no request.
+__device__ __forceinline__ bool row_sees(const AttentionParams& p, const Item& item, int r, int64_t& seen) {
     if (r >= item.rows) return false;
-    const int64_t local = item.row + r;
-    const int64_t at = local / p.group;
-    head = item.head * p.group + static_cast<int>(local - at * p.group);
+    const int at = (item.row + r) / p.group;
+    seen = item.bias + at;
+    if (!item.prefix) return true;
+    int64_t b;
     Request request;
-    if (item.prefix) {
-        token = at;
-        int64_t b;
-        if (!request_of(p, token, b, request)) return false;
-    } else {
-        request = request_at(p, item.request);
-        token = request.begin + at;
-    }
-    seen = request.length - request.fresh + (token - request.begin) + 1;
+    if (!request_of(p, at, b, request)) return false;
+    seen = request.length - request.fresh + (at - request.begin) + 1;
     return true;
 }
 
@@ -374,10 +389,11 @@ struct Layout {
     static constexpr uint32_t kKeys = 2 * kOperand;
     static constexpr uint32_t kValues = kKeys + kStages * kOperand;
     static constexpr uint32_t kPlan = kValues + kStages * kOperand;
-    static constexpr uint32_t kMasks = kPlan + ((sizeof(Plan) + 15) / 16) * 16;
+    static constexpr uint32_t kItems = kPlan + ((sizeof(Plan) + 15) / 16) * 16;
+    static constexpr uint32_t kMasks = kItems + kItemRing * sizeof(Item);
     static constexpr uint32_t kBarriers = kMasks + kMaskRing * 16;
-    // k_full, k_empty, v_full, v_empty (stages each); q_full, q_empty, s_full, p_full, o_full (slots each); drain.
-    static constexpr int kBarrierCount = 4 * kStages + 5 * 2 + 1;
+    // Six of each stage, seven of each slot, two of each place in the item ring.
+    static constexpr int kBarrierCount = 6 * kStages + 7 * 2 + 2 * kItemRing;
     static constexpr uint32_t kTail = kBarriers + kBarrierCount * 8;
     static constexpr uint32_t kBytes = kTail + 16;  // tensor-memory address, failed flag
 };
@@ -406,64 +422,93 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     using L = Layout<kDim>;
     extern __shared__ __align__(1024) uint8_t shared[];
     Plan& plan = *reinterpret_cast<Plan*>(shared + L::kPlan);
-    volatile uint32_t* masks = reinterpret_cast<uint32_t*>(shared + L::kMasks);
+    uint4* masks = reinterpret_cast<uint4*>(shared + L::kMasks);
     volatile uint32_t* failed = reinterpret_cast<uint32_t*>(shared + L::kTail + 4);
     const uint32_t base = shared_address(shared);
+    constexpr int kIssueWarp = 8 + kGatherWarps;
     const int warp = threadIdx.x >> 5;
     const unsigned lane = lane_id();
 
+    // K and V stages: landed (written), full (and visible to the tensor cores), empty (read).
     const uint32_t barriers = base + L::kBarriers;
-    const auto k_full = [&](int s) { return barriers + 8 * s; };
-    const auto k_empty = [&](int s) { return barriers + 8 * (L::kStages + s); };
-    const auto v_full = [&](int s) { return barriers + 8 * (2 * L::kStages + s); };
-    const auto v_empty = [&](int s) { return barriers + 8 * (3 * L::kStages + s); };
-    const auto slot_barrier = [&](int which, int s) { return barriers + 8 * (4 * L::kStages + 2 * which + s); };
-    const auto q_full = [&](int s) { return slot_barrier(0, s); };
-    const auto q_empty = [&](int s) { return slot_barrier(1, s); };
-    const auto s_full = [&](int s) { return slot_barrier(2, s); };
-    const auto p_full = [&](int s) { return slot_barrier(3, s); };
-    const auto o_full = [&](int s) { return slot_barrier(4, s); };
-    const uint32_t drain = barriers + 8 * (L::kBarrierCount - 1);
+    const auto stage_barrier = [&](int which, int s) { return barriers + 8 * (which * L::kStages + s); };
+    const auto k_landed = [&](int s) { return stage_barrier(0, s); };
+    const auto k_full = [&](int s) { return stage_barrier(1, s); };
+    const auto k_empty = [&](int s) { return stage_barrier(2, s); };
+    const auto v_landed = [&](int s) { return stage_barrier(3, s); };
+    const auto v_full = [&](int s) { return stage_barrier(4, s); };
+    const auto v_empty = [&](int s) { return stage_barrier(5, s); };
+    const auto slot_barrier = [&](int which, int s) { return barriers + 8 * (6 * L::kStages + 2 * which + s); };
+    const auto q_landed = [&](int s) { return slot_barrier(0, s); };
+    const auto q_full = [&](int s) { return slot_barrier(1, s); };
+    const auto q_empty = [&](int s) { return slot_barrier(2, s); };
+    const auto s_full = [&](int s) { return slot_barrier(3, s); };
+    const auto p_full = [&](int s) { return slot_barrier(4, s); };
+    const auto o_full = [&](int s) { return slot_barrier(5, s); };
+    const auto item_full = [&](int i) { return barriers + 8 * (6 * L::kStages + 12 + i); };
+    const auto item_empty = [&](int i) { return barriers + 8 * (6 * L::kStages + 12 + kItemRing + i); };
+    const auto drain = [&](int s) { return barriers + 8 * (L::kBarrierCount - 2 + s); };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < L::kStages; ++s) {
-            barrier_init(k_full(s), 4);
-            barrier_init(k_empty(s), 1);
-            barrier_init(v_full(s), 4);
-            barrier_init(v_empty(s), 1);
+            barrier_init(k_landed(s), 32 * kGatherWarps);
+            barrier_init(k_full(s), 1);
+            barrier_init(k_empty(s), 2);  // both slots, whether they use the tile or not
+            barrier_init(v_landed(s), 32 * kGatherWarps);
+            barrier_init(v_full(s), 1);
+            barrier_init(v_empty(s), 2);
         }
         for (int s = 0; s < 2; ++s) {
-            barrier_init(q_full(s), 4);
+            barrier_init(q_landed(s), 32 * kGatherWarps);
+            barrier_init(q_full(s), 1);
             barrier_init(q_empty(s), 1);
             barrier_init(s_full(s), 1);
             barrier_init(p_full(s), 4);
             barrier_init(o_full(s), 1);
+            barrier_init(drain(s), 1);
         }
-        barrier_init(drain, 1);
+        for (int i = 0; i < kItemRing; ++i) {
+            barrier_init(item_full(i), 1);
+            barrier_init(item_empty(i), 8 + kGatherWarps + 3);  // every warp but the one that walks
+        }
         *failed = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_shared();
     }
-    if (warp == 12) tensor_alloc(base + L::kTail, 512);
+    if (warp == kIssueWarp) tensor_alloc(base + L::kTail, 512);
     grid_dependency_wait();
     tensor_fence_before();
     build_plan(p, plan);  // ends with __syncthreads
     tensor_fence_after();
     const uint32_t tensor = *reinterpret_cast<volatile uint32_t*>(shared + L::kTail);
 
-    Walk walk = begin_walk(p, plan);
+    Item* items = reinterpret_cast<Item*>(shared + L::kItems);
     Item item;
+    uint32_t item_uses = 0;
     int turn = 0;  // slot of the next item of up to 128 rows
+    // The next item, for a whole warp or one thread of it; false at the list's end (or a failed wait).
+    const auto next = [&](bool alone) {
+        const int place = item_uses % kItemRing;
+        bool there = barrier_wait(item_full(place), (item_uses / kItemRing) & 1, failed);
+        if (!alone) there = __all_sync(0xffffffffu, there);
+        if (!there) return false;
+        item = items[place];
+        if (!alone) __syncwarp();
+        if (alone || lane == 0) barrier_arrive(item_empty(place));
+        ++item_uses;
+        return item.rows > 0;
+    };
 
     if (warp < 8) {
         // ------------------------------------------------------------ softmax of slot `slot`
+        registers_grow<kSoftmaxRegisters>();
         const int slot = warp >> 2;
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 tensor-memory lanes a warp
         const uint32_t scores = tensor + lanes + slot * kTile;
         const uint32_t output = tensor + lanes + 256 + slot * 128;
         uint32_t uses = 0, ends = 0, tile_count = 0;
         const int r = (warp & 3) * 32 + lane;
-        while (next_item(p, plan, walk, item)) {
+        while (next(false)) {
             const bool both = item.rows > kRows;
             const int mine = both ? slot : turn;
             turn ^= 1;
@@ -472,85 +517,82 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 continue;
             }
             const int item_row = (both ? slot * kRows : 0) + r;
-            int64_t token = 0, seen;
-            int head = 0;
-            const bool present = row_of(p, item, item_row, token, head, seen);
-            if (!present) seen = INT64_MAX;  // computed with the others and dropped
+            int64_t seen;
+            const bool present = row_sees(p, item, item_row, seen);
+            // Positions from the item's first one on; a row of no request is computed with the others and dropped.
+            const int64_t reach = seen - item.begin;
+            const int limit = !present || reach > INT32_MAX ? INT32_MAX : (reach < 0 ? 0 : static_cast<int>(reach));
             const bool idle = (both ? slot * kRows : 0) + (warp & 3) * 32 >= item.rows;  // no row in this warp
-            float top = -INFINITY, total = 0.f;
-            for (int64_t t = item.low; t < item.high; ++t, ++tile_count) {
+            float top = -INFINITY;
+            float2 total = make_float2(0.f, 0.f);
+            for (int t = item.low; t < item.high; ++t, ++tile_count) {
                 if (!__all_sync(0xffffffffu, barrier_wait(s_full(slot), uses & 1, failed))) goto finish;
                 ++uses;
                 tensor_fence_after();
                 if (!idle) {
-                    const int64_t position = item.begin + t * kTile;
+                    uint32_t s[kTile];
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) tensor_load32(scores + 32 * c, s + 32 * c);
                     // Positions this row sees here: those that have a slot, up to its last.
-                    const int64_t left = seen - position;
-                    uint32_t bits[4];
-                    uint32_t all = 0xffffffffu;
+                    const int left = limit - t * kTile;
+                    const uint4 there = masks[tile_count % kMaskRing];
+                    const bool whole = __all_sync(0xffffffffu, left >= kTile) &&
+                                       (there.x & there.y & there.z & there.w) == 0xffffffffu;
+                    tensor_wait_load();
+                    if (!whole) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int64_t mine_left = left - 32 * c;
-                        const uint32_t limit =
-                            mine_left >= 32 ? 0xffffffffu : (mine_left <= 0 ? 0u : (1u << mine_left) - 1u);
-                        bits[c] = masks[(tile_count % kMaskRing) * 4 + c] & limit;
-                        all &= bits[c];
-                    }
-                    const bool whole = __all_sync(0xffffffffu, all == 0xffffffffu);
-                    float high = -INFINITY;
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t s[32];
-                        tensor_load32(scores + 32 * c, s);
-                        tensor_wait_load();
-                        if (whole) {
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) high = fmaxf(high, __uint_as_float(s[j]));
-                        } else {
+                        for (int c = 0; c < 4; ++c) {
+                            const uint32_t bits = c == 0 ? there.x : c == 1 ? there.y : c == 2 ? there.z : there.w;
 #pragma unroll
                             for (int j = 0; j < 32; ++j) {
-                                high = fmaxf(high, bits[c] >> j & 1u ? __uint_as_float(s[j]) : -INFINITY);
+                                if (!(bits >> j & 1u) || 32 * c + j >= left) s[32 * c + j] = 0xff800000u;  // -inf
                             }
                         }
                     }
-                    high *= p.scale_log2;
+                    float highs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                    for (int j = 0; j < kTile; j += 8) {
+#pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            highs[c] = fmaxf(highs[c], fmaxf(__uint_as_float(s[j + 2 * c]), __uint_as_float(s[j + 2 * c + 1])));
+                        }
+                    }
+                    const float high = fmaxf(fmaxf(highs[0], highs[1]), fmaxf(highs[2], highs[3])) * p.scale_log2;
                     const bool raise = present && (high > top + kRaise || (top == -INFINITY && high > -INFINITY));
                     if (__any_sync(0xffffffffu, raise)) {
                         const float before = top;
                         if (raise) top = high;
                         const float factor = raise ? (before == -INFINITY ? 0.f : exp2_approx(before - top)) : 1.f;
-                        total *= factor;
+                        total.x *= factor;
+                        total.y *= factor;
                         if (t > item.low) {
                             // The products of this slot's earlier tiles are complete (s_full).
 #pragma unroll 1
-                            for (int c = 0; c < kDim / 32; ++c) {
-                                uint32_t o[32];
-                                tensor_load32(output + 32 * c, o);
+                            for (int c = 0; c < kDim / 16; ++c) {
+                                uint32_t o[16];
+                                tensor_load16(output + 16 * c, o);
                                 tensor_wait_load();
 #pragma unroll
-                                for (int j = 0; j < 32; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * factor);
-                                tensor_store32(output + 32 * c, o);
+                                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * factor);
+                                tensor_store16(output + 16 * c, o);
                             }
                         }
                     }
-                    const float shift = top == -INFINITY ? 0.f : top;
+                    const float shift = top == -INFINITY ? 0.f : -top;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        uint32_t s[32], weights[16];
-                        tensor_load32(scores + 32 * c, s);
-                        tensor_wait_load();
+                    for (int c = 0; c < 2; ++c) {
+                        uint32_t weights[32];
 #pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            float a = exp2_approx(fmaf(__uint_as_float(s[j]), p.scale_log2, -shift));
-                            float b = exp2_approx(fmaf(__uint_as_float(s[j + 1]), p.scale_log2, -shift));
-                            if (!whole) {
-                                a = bits[c] >> j & 1u ? a : 0.f;
-                                b = bits[c] >> (j + 1) & 1u ? b : 0.f;
-                            }
-                            total += a + b;
-                            weights[j / 2] = Kind<T>::pack(a, b);
+                        for (int j = 0; j < 32; ++j) {
+                            const int at = 64 * c + 2 * j;
+                            float2 x = fma2(make_float2(__uint_as_float(s[at]), __uint_as_float(s[at + 1])),
+                                            make_float2(p.scale_log2, p.scale_log2), make_float2(shift, shift));
+                            x.x = exp2_approx(x.x);
+                            x.y = exp2_approx(x.y);
+                            total = add2(total, x);
+                            weights[j] = Kind<T>::pack(x.x, x.y);
                         }
-                        tensor_store16(scores + 16 * c, weights);
+                        tensor_store32(scores + 32 * c, weights);
                     }
                     tensor_wait_store();
                 }
@@ -565,10 +607,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 float* partial;
                 float2* stat;
                 if (item.first) {
-                    // Rows of a head in token order: for an own item behind those of its request's first token.
-                    const int64_t row = item.head * p.head_rows +
-                                        (item.prefix ? item.row + item_row
-                                                     : token * p.group + (head - item.head * p.group));
+                    // Rows of a head in token order: an own item's lie behind its request's first token.
+                    const int64_t row = static_cast<int64_t>(item.head) * p.head_rows +
+                                        static_cast<int64_t>(item.token) * p.group + item.row + item_row;
                     partial = (item.prefix ? p.prefix_out : p.own_out) + row * kDim;
                     stat = (item.prefix ? p.prefix_stat : p.own_stat) + row;
                 } else {
@@ -588,204 +629,192 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                         }
                     }
                 }
-                if (present) *stat = make_float2(top, total);
+                if (present) *stat = make_float2(top, total.x + total.y);
                 tensor_fence_before();
             }
         }
-    } else if (warp < 12) {
+    } else if (warp < kIssueWarp) {
         // ------------------------------------------------------------ gather
-        const int part = warp - 8;  // rows 32 * part .. of every operand
+        registers_shrink<kGatherRegisters>();
+        const int first_row = (warp - 8) * kGatherRows;  // of every operand
         constexpr int kLanes = kDim / 8;        // lanes a row (16 bytes each)
         constexpr int kAtOnce = 32 / kLanes;    // rows a step
         const int chunk = lane % kLanes, sub = lane / kLanes;
-        const char* k_plane = static_cast<const char*>(p.k_plane);
-        const char* v_plane = static_cast<const char*>(p.v_plane);
-        constexpr int kGroups = 2 * L::kStages;  // most copy groups in flight
-        uint32_t signals[kGroups] = {};          // barriers of the groups in flight, oldest first
-        int pending = 0;
-        uint32_t k_uses = 0, q_uses[2] = {0, 0};
-        // Complete the oldest group and tell its barrier.
-        const auto signal_oldest = [&]() {
-            switch (pending) {
-                case 1: copies_wait<0>(); break;
-                case 2: copies_wait<1>(); break;
-                case 3: copies_wait<2>(); break;
-                case 4: copies_wait<3>(); break;
-                case 5: copies_wait<4>(); break;
-                case 6: copies_wait<5>(); break;
-                case 7: copies_wait<6>(); break;
-                default: copies_wait<7>(); break;
-            }
-            fence_async_shared();
-            __syncwarp();
-            if (lane == 0) barrier_arrive(signals[0]);
-#pragma unroll
-            for (int i = 0; i + 1 < kGroups; ++i) signals[i] = signals[i + 1];
-            --pending;
-        };
-        // Wait for room, telling what has arrived meanwhile (the room may depend on it).
-        const auto acquire = [&](uint32_t barrier, uint32_t parity) {
-            if (pending == kGroups) signal_oldest();
-            while (!__all_sync(0xffffffffu, barrier_try(barrier, parity))) {
-                if (pending) {
-                    signal_oldest();
-                } else if (!__all_sync(0xffffffffu, barrier_wait(barrier, parity, failed))) {
-                    return false;
-                }
-            }
-            return true;
-        };
-        const auto launched = [&](uint32_t barrier) {
-            copies_commit();
-#pragma unroll
-            for (int i = 0; i < kGroups; ++i) {
-                if (i == pending) signals[i] = barrier;
-            }
-            ++pending;
-        };
+        const char* query = static_cast<const char*>(p.query) + 16 * chunk;
+        uint32_t uses = 0, q_uses[2] = {0, 0};
+        // A row's 16-byte chunks are swizzled within its 128 bytes by the row's place in its eight.
         const auto target = [&](uint32_t operand, int row) {
             return operand + (chunk >> 3) * L::kBlock + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
         };
-        while (next_item(p, plan, walk, item)) {
+        // Plane slot of this lane's row in tile t of the item.
+        const auto find = [&](int t) {
+            const int position = item.begin + t * kTile + first_row + static_cast<int>(lane);
+            return position < item.end ? static_cast<int>(slot_of(p, item.table_row, static_cast<uint32_t>(position))) : -1;
+        };
+        bool more = next(false);
+        int found = more ? find(item.low) : -1;
+        while (more) {
             const bool both = item.rows > kRows;
-            const int64_t first_token = item.prefix ? 0 : request_at(p, item.request).begin;
             // Queries of the slots the item uses.
             for (int half = 0; half < (both ? 2 : 1); ++half) {
                 const int slot = both ? half : turn;
-                if (!acquire(q_empty(slot), (q_uses[slot] & 1) ^ 1)) goto finish;
+                if (!__all_sync(0xffffffffu, barrier_wait(q_empty(slot), (q_uses[slot] & 1) ^ 1, failed))) goto finish;
                 ++q_uses[slot];
                 const uint32_t operand = base + L::kQuery + slot * L::kOperand;
-                for (int i = 0; i < 32; i += kAtOnce) {
-                    const int row = part * 32 + i + sub;
-                    if (half * kRows + part * 32 + i >= item.rows) break;
-                    const int64_t local = item.row + half * kRows + row;
-                    if (half * kRows + row < item.rows) {
-                        const int64_t at = local / p.group;
-                        const int head = item.head * p.group + static_cast<int>(local - at * p.group);
-                        const int64_t token = first_token + at;
-                        const char* source = static_cast<const char*>(p.query) +
-                                             2 * (token * p.q_token + head * p.q_head) + 16 * chunk;
-                        copy16_async(target(operand, row), source, 16);
+#pragma unroll 1
+                for (int i = 0; i < kGatherRows; i += kAtOnce) {
+                    const int r = first_row + i + sub;
+                    if (half * kRows + r < item.rows) {
+                        const int local = item.row + half * kRows + r;
+                        const int at = local / p.group;
+                        const int head = item.head * p.group + local - at * p.group;
+                        copy16_async(target(operand, r), query + 2 * ((item.token + at) * p.q_token + head * p.q_head), 16);
                     }
                 }
-                launched(q_full(slot));
+                copies_arrive(q_landed(slot));
             }
             turn ^= 1;
-            const int64_t table_row =
-                item.prefix ? p.source_row : (p.rows ? load_index(p.rows, p.rows_es, item.request) : item.request);
-            const char* keys = k_plane + 2 * item.head * p.k_head + 16 * chunk;
-            const char* values = v_plane + 2 * item.head * p.v_head + 16 * chunk;
-            for (int64_t t = item.low; t < item.high; ++t, ++k_uses) {
-                const int64_t position = item.begin + t * kTile + part * 32 + lane;
-                const int64_t own = position < item.end ? slot_of(p, table_row, static_cast<uint32_t>(position)) : -1;
-                const uint32_t there = __ballot_sync(0xffffffffu, own >= 0);
-                const int stage = k_uses % L::kStages;
-                const uint32_t parity = ((k_uses / L::kStages) & 1) ^ 1;
-                if (!acquire(k_empty(stage), parity)) goto finish;
-                if (lane == 0) masks[(k_uses % kMaskRing) * 4 + part] = there;
-                const int found = static_cast<int>(own);
+            const char* keys = static_cast<const char*>(p.k_plane) + 2 * item.head * p.k_head + 16 * chunk;
+            const char* values = static_cast<const char*>(p.v_plane) + 2 * item.head * p.v_head + 16 * chunk;
+            const int high = item.high;
+            for (int t = item.low; t < high; ++t, ++uses) {
+                const int stage = uses % L::kStages;
+                const uint32_t parity = ((uses / L::kStages) & 1) ^ 1;
+                const int now = found;
+                // The next tile's slots are looked up while this one's rows are copied.
+                if (t + 1 < high) {
+                    found = find(t + 1);
+                } else {
+                    more = next(false);
+                    if (more) found = find(item.low);
+                }
+                const uint32_t there = __ballot_sync(0xffffffffu, now >= 0);
+                if (!__all_sync(0xffffffffu, barrier_wait(k_empty(stage), parity, failed))) goto finish;
+                // The mask's place was tile n - kMaskRing's.  The stage is empty when the first
+                // products of tile n - kStages are complete, which follow the softmax of every earlier tile.
+                if (lane == 0) reinterpret_cast<uint32_t*>(&masks[uses % kMaskRing])[warp - 8] = there;
                 uint32_t operand = base + L::kKeys + stage * L::kOperand;
 #pragma unroll 8
-                for (int i = 0; i < 32; i += kAtOnce) {
-                    const int row = i + sub;
-                    const int slot = __shfl_sync(0xffffffffu, found, row);
-                    const char* source = slot >= 0 ? keys + 2 * (slot * p.k_slot) : static_cast<const char*>(p.query);
-                    copy16_async(target(operand, part * 32 + row), source, slot >= 0 ? 16 : 0);
+                for (int i = 0; i < kGatherRows; i += kAtOnce) {
+                    const int slot = __shfl_sync(0xffffffffu, now, i + sub);
+                    copy16_async(target(operand, first_row + i + sub), slot >= 0 ? keys + 2 * (slot * p.k_slot) : query,
+                                 slot >= 0 ? 16 : 0);
                 }
-                launched(k_full(stage));
-                if (!acquire(v_empty(stage), parity)) goto finish;
+                copies_arrive(k_landed(stage));
+                if (!__all_sync(0xffffffffu, barrier_wait(v_empty(stage), parity, failed))) goto finish;
                 operand = base + L::kValues + stage * L::kOperand;
 #pragma unroll 8
-                for (int i = 0; i < 32; i += kAtOnce) {
-                    const int row = i + sub;
-                    const int slot = __shfl_sync(0xffffffffu, found, row);
-                    const char* source = slot >= 0 ? values + 2 * (slot * p.v_slot) : static_cast<const char*>(p.query);
-                    copy16_async(target(operand, part * 32 + row), source, slot >= 0 ? 16 : 0);
+                for (int i = 0; i < kGatherRows; i += kAtOnce) {
+                    const int slot = __shfl_sync(0xffffffffu, now, i + sub);
+                    copy16_async(target(operand, first_row + i + sub), slot >= 0 ? values + 2 * (slot * p.v_slot) : query,
+                                 slot >= 0 ? 16 : 0);
                 }
-                launched(v_full(stage));
+                copies_arrive(v_landed(stage));
             }
         }
-        while (pending) signal_oldest();
-    } else if (warp == 12 && lane == 0) {
-        // ------------------------------------------------------------ products
-        constexpr uint32_t kScoreProduct = mma_descriptor(Kind<T>::kBf16, kRows, kTile, false);
-        constexpr uint32_t kOutputProduct = mma_descriptor(Kind<T>::kBf16, kRows, kDim, true);
-        uint32_t k_uses = 0, q_uses[2] = {0, 0}, p_uses[2] = {0, 0};
-        // The second product of a tile is issued after the first one of the next, unless both
-        // use the same slot (whose scores it reads).
-        struct {
-            bool waiting;
-            int slot;
-            uint32_t uses;  // of the K and V stages
-            bool begins, ends, opens, closes;  // first / last tile of the item; first / last slot of the tile
-        } later{};
-        const auto second = [&]() {
-            later.waiting = false;
-            const int slot = later.slot, stage = later.uses % L::kStages;
-            if (!barrier_wait(p_full(slot), p_uses[slot] & 1, failed)) return false;
-            ++p_uses[slot];
-            if (later.opens && !barrier_wait(v_full(stage), (later.uses / L::kStages) & 1, failed)) return false;
-            tensor_fence_after();
-            const uint64_t values = shared_operand(base + L::kValues + stage * L::kOperand, L::kBlock);
-            const uint32_t d = tensor + 256 + slot * 128, weights = tensor + slot * kTile;
-#pragma unroll
-            for (int k = 0; k < kTile / 16; ++k) {
-                mma_tensor(d, weights + 8 * k, values + k * (16 * 128 >> 4), kOutputProduct, !later.begins || k > 0);
-            }
-            if (later.closes) mma_commit(v_empty(stage));
-            if (later.ends) mma_commit(o_full(slot));
-            return true;
-        };
-        bool fine = true;
-        while (fine && next_item(p, plan, walk, item)) {
-            const bool both = item.rows > kRows;
-            const int only = turn;
-            turn ^= 1;
-            for (int64_t t = item.low; fine && t < item.high; ++t, ++k_uses) {
-                const int stage = k_uses % L::kStages;
-                for (int half = 0; half < (both ? 2 : 1); ++half) {
-                    const int slot = both ? half : only;
-                    if (later.waiting && later.slot == slot && !(fine = second())) break;
-                    if (half == 0 && !(fine = barrier_wait(k_full(stage), (k_uses / L::kStages) & 1, failed))) break;
-                    if (t == item.low) {
-                        if (!(fine = barrier_wait(q_full(slot), q_uses[slot] & 1, failed))) break;
-                        ++q_uses[slot];
+    } else {
+        registers_shrink<kIssueRegisters>();
+        if (warp < kIssueWarp + 2 && lane == 0) {
+            // -------------------------------------------------------- products of slot `slot`
+            constexpr uint32_t kScoreProduct = mma_descriptor(Kind<T>::kBf16, kRows, kTile, false);
+            constexpr uint32_t kOutputProduct = mma_descriptor(Kind<T>::kBf16, kRows, kDim, true);
+            const int slot = warp - kIssueWarp;
+            const uint32_t scores = tensor + slot * kTile, output = tensor + 256 + slot * 128;
+            const uint64_t queries = shared_operand(base + L::kQuery + slot * L::kOperand, 16);
+            const uint64_t all_keys = shared_operand(base + L::kKeys, 16);
+            const uint64_t all_values = shared_operand(base + L::kValues, L::kBlock);
+            uint32_t uses = 0, q_uses = 0, p_uses = 0;
+            bool fine = true;
+            while (fine && next(true)) {
+                const bool mine = item.rows > kRows || turn == slot;
+                turn ^= 1;
+                const int low = item.low, high = item.high;
+                if (mine) {
+                    fine = barrier_wait(q_full(slot), q_uses & 1, failed);
+                    ++q_uses;
+                }
+                for (int t = low; fine && t < high; ++t, ++uses) {
+                    const int stage = uses % L::kStages;
+                    const uint32_t parity = (uses / L::kStages) & 1;
+                    if (!(fine = barrier_wait(k_full(stage), parity, failed))) break;
+                    if (!mine) {
+                        barrier_arrive(k_empty(stage));
+                        if (!(fine = barrier_wait(v_full(stage), parity, failed))) break;
+                        barrier_arrive(v_empty(stage));
+                        continue;
                     }
                     tensor_fence_after();
-                    const uint64_t queries = shared_operand(base + L::kQuery + slot * L::kOperand, 16);
-                    const uint64_t keys = shared_operand(base + L::kKeys + stage * L::kOperand, 16);
+                    const uint64_t keys = all_keys + stage * (L::kOperand >> 4);
 #pragma unroll
                     for (int k = 0; k < kDim / 16; ++k) {
                         const uint32_t step = (k / 4) * (L::kBlock >> 4) + (k % 4) * 2;
-                        mma_shared(tensor + slot * kTile, queries + step, keys + step, kScoreProduct, k > 0);
+                        mma_shared(scores, queries + step, keys + step, kScoreProduct, k > 0);
                     }
                     mma_commit(s_full(slot));
-                    const bool last = !both || half == 1;
-                    if (last) mma_commit(k_empty(stage));
-                    if (t + 1 == item.high) mma_commit(q_empty(slot));
-                    if (later.waiting && !(fine = second())) break;
-                    later.waiting = true;
-                    later.slot = slot;
-                    later.uses = k_uses;
-                    later.begins = t == item.low;
-                    later.ends = t + 1 == item.high;
-                    later.opens = half == 0;
-                    later.closes = last;
+                    mma_commit(k_empty(stage));
+                    if (t + 1 == high) mma_commit(q_empty(slot));
+                    if (!(fine = barrier_wait(v_full(stage), parity, failed))) break;
+                    if (!(fine = barrier_wait(p_full(slot), p_uses & 1, failed))) break;
+                    ++p_uses;
+                    tensor_fence_after();
+                    const uint64_t values = all_values + stage * (L::kOperand >> 4);
+#pragma unroll
+                    for (int k = 0; k < kTile / 16; ++k) {
+                        mma_tensor(output, scores + 8 * k, values + k * (16 * 128 >> 4), kOutputProduct, t > low || k > 0);
+                    }
+                    mma_commit(v_empty(stage));
+                    if (t + 1 == high) mma_commit(o_full(slot));
+                }
+            }
+            // Nothing may still use tensor memory when it is freed, whatever happened above.
+            mma_commit(drain(slot));
+            volatile uint32_t ran_out = 0;
+            barrier_wait(drain(slot), 0, &ran_out);
+        } else if (warp == kIssueWarp + 2 && lane == 0) {
+            // -------------------------------------------------------- the block's items
+            Walk walk = begin_walk(p, plan);
+            bool more = true;
+            while (more) {
+                more = next_item(p, plan, walk, item);
+                if (!more) item.rows = 0;
+                const int place = item_uses % kItemRing;
+                if (!barrier_wait(item_empty(place), ((item_uses / kItemRing) & 1) ^ 1, failed)) break;
+                items[place] = item;
+                barrier_arrive(item_full(place));
+                ++item_uses;
+            }
+        } else if (warp == kIssueWarp + 3 && lane == 0) {
+            // -------------------------------------------------------- what the gather has written
+            uint32_t uses = 0, q_uses[2] = {0, 0};
+            bool fine = true;
+            const auto pass_on = [&](uint32_t landed, uint32_t full, uint32_t parity) {
+                if (!barrier_wait(landed, parity, failed)) return false;
+                fence_async_shared();
+                barrier_arrive(full);
+                return true;
+            };
+            while (fine && next(true)) {
+                const bool both = item.rows > kRows;
+                for (int half = 0; fine && half < (both ? 2 : 1); ++half) {
+                    const int slot = both ? half : turn;
+                    fine = pass_on(q_landed(slot), q_full(slot), q_uses[slot] & 1);
+                    ++q_uses[slot];
+                }
+                turn ^= 1;
+                for (int t = item.low; fine && t < item.high; ++t, ++uses) {
+                    const int stage = uses % L::kStages;
+                    const uint32_t parity = (uses / L::kStages) & 1;
+                    fine = pass_on(k_landed(stage), k_full(stage), parity) && pass_on(v_landed(stage), v_full(stage), parity);
                 }
             }
         }
-        if (fine && later.waiting) fine = second();
-        // Nothing may still use tensor memory when it is freed, whatever happened above.
-        mma_commit(drain);
-        volatile uint32_t ran_out = 0;
-        barrier_wait(drain, 0, &ran_out);
     }
 finish:
-    copies_wait<0>();
+    copies_wait_all();
     __syncthreads();
     allow_dependents();
     if (threadIdx.x == 0) p.failed[blockIdx.x] = *failed;
-    if (warp == 12) {
+    if (warp == kIssueWarp) {
         __syncwarp();
         tensor_free(tensor, 512);
     }
@@ -832,14 +861,14 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ At
     const int64_t entry = first_entry + local / (2 * kRows);
     const int64_t entries_end = p.plan_first[p.batch];
     const int64_t total_cost = prefix_total + static_cast<int64_t>(p.plan_cost[entries_end]) * p.kv_heads;
-    const auto join_item = [&](int64_t start, int64_t tiles, const float* out, const float2* stat, int64_t row, int r) {
+    const auto join_item = [&](int64_t start, int tiles, const float* out, const float2* stat, int64_t row, int r) {
         if (tiles <= 0) return;
         int64_t block = ((start + 1) * p.blocks - 1) / total_cost;  // the share that holds `start`
         join(block, out, stat, row);
-        int64_t done = first_tile(share_begin(block + 1, total_cost, p.blocks), start, tiles);
+        int done = first_tile(share_begin(block + 1, total_cost, p.blocks), start, tiles);
         while (done < tiles) {
             ++block;
-            const int64_t high = first_tile(share_begin(block + 1, total_cost, p.blocks), start, tiles);
+            const int high = first_tile(share_begin(block + 1, total_cost, p.blocks), start, tiles);
             if (high > done) join(block, p.next_out, p.next_stat, block * 2 * kRows + r);
             done = high;
         }
@@ -850,7 +879,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ At
     if (entry < entries_end) {
         const int64_t cost = p.plan_cost[entry + 1] - p.plan_cost[entry];
         join_item(prefix_total + static_cast<int64_t>(p.plan_cost[entry]) * p.kv_heads + kv_head * cost,
-                  cost ? (cost - kItemCost) / kTileCost : 0, p.own_out, p.own_stat, kv_head * p.head_rows + head_row,
+                  cost ? static_cast<int>((cost - kItemCost) / kTileCost) : 0, p.own_out, p.own_stat, kv_head * p.head_rows + head_row,
                   static_cast<int>(local % (2 * kRows)));
     }
     const float scale = bad ? NAN : (total == 0.f ? 0.f : 1.f / total);
@@ -1011,7 +1040,7 @@ extern "C" int ekv_shared_prefix_attention(
         }
         p.tokens = tokens;
         p.batch = batch;
-        p.shared = shared_tokens;
+        p.shared = static_cast<int>(shared_tokens);
         p.source_row = source_row;
         p.kv_heads = kv_heads;
         p.group = group;
@@ -1020,9 +1049,9 @@ extern "C" int ekv_shared_prefix_attention(
         p.len_es = lengths_esize;
         p.starts_es = starts_esize;
         p.scale_log2 = scale * 1.4426950408889634f;
-        p.head_rows = head_rows;
-        p.prefix_row_tiles = (head_rows + 2 * kRows - 1) / (2 * kRows);
-        p.prefix_tiles = (shared_tokens + kTile - 1) / kTile;
+        p.head_rows = static_cast<int>(head_rows);
+        p.prefix_row_tiles = static_cast<int>((head_rows + 2 * kRows - 1) / (2 * kRows));
+        p.prefix_tiles = static_cast<int>((shared_tokens + kTile - 1) / kTile);
         p.blocks = blocks;
         char* at = static_cast<char*>(workspace);
         p.prefix_out = reinterpret_cast<float*>(at + w.prefix_out);

@@ -39,22 +39,21 @@ __device__ __forceinline__ uint64_t device_nanoseconds() {
 constexpr uint64_t kWaitLimit = 4000000000ull;
 
 // Wait for the phase of `parity` to complete.  False (and *failed set) when kWaitLimit passes or
-// another thread of the block has given up.
+// another thread of the block has given up.  Kept short: a kernel has many waits.
 __device__ __forceinline__ bool barrier_wait(uint32_t barrier, uint32_t parity, volatile uint32_t* failed) {
-    for (int i = 0; i < 64; ++i) {
-        if (barrier_try(barrier, parity)) return true;
-    }
-    const uint64_t begin = device_nanoseconds();
-    while (true) {
-        for (int i = 0; i < 256; ++i) {
-            if (barrier_try(barrier, parity)) return true;
-        }
-        if (*failed) return false;
-        if (device_nanoseconds() - begin > kWaitLimit) {
+    uint32_t tries = 0;
+    uint64_t begin = 0;
+#pragma unroll 1
+    while (!barrier_try(barrier, parity)) {
+        if (++tries & 255) continue;
+        const uint64_t now = device_nanoseconds();
+        if (!begin) begin = now;
+        if (*failed || now - begin > kWaitLimit) {
             *failed = 1;
             return false;
         }
     }
+    return true;
 }
 
 // ---------------------------------------------------------------- proxies and asynchronous copies
@@ -65,10 +64,20 @@ __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy
 __device__ __forceinline__ void copy16_async(uint32_t target, const void* source, uint32_t bytes) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(target), "l"(source), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int kPending>
-__device__ __forceinline__ void copies_wait() {
-    asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+// One arrival at `barrier` (counted in advance) when this thread's copies so far have landed.
+__device__ __forceinline__ void copies_arrive(uint32_t barrier) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(barrier) : "memory");
+}
+__device__ __forceinline__ void copies_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Registers a thread may use from here on (all warps of the warpgroup together).
+template <int kRegisters>
+__device__ __forceinline__ void registers_grow() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegisters));
+}
+template <int kRegisters>
+__device__ __forceinline__ void registers_shrink() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegisters));
 }
 
 // ---------------------------------------------------------------- tensor memory
@@ -90,21 +99,27 @@ __device__ __forceinline__ void tensor_wait_store() { asm volatile("tcgen05.wait
 #define EKV_I8(r, i) "r"(r[i]), "r"(r[i + 1]), "r"(r[i + 2]), "r"(r[i + 3]), "r"(r[i + 4]), "r"(r[i + 5]), "r"(r[i + 6]), "r"(r[i + 7])
 
 // This lane's 32 consecutive columns (the warp's 32 lanes are tensor-memory lanes).
-__device__ __forceinline__ void tensor_load32(uint32_t address, uint32_t (&r)[32]) {
+__device__ __forceinline__ void tensor_load32(uint32_t address, uint32_t* r) {
     asm volatile(
         "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
         "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
         : EKV_R8(r, 0), EKV_R8(r, 8), EKV_R8(r, 16), EKV_R8(r, 24)
         : "r"(address));
 }
-__device__ __forceinline__ void tensor_store32(uint32_t address, const uint32_t (&r)[32]) {
+__device__ __forceinline__ void tensor_store32(uint32_t address, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
         "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::EKV_I8(r, 0),
         EKV_I8(r, 8), EKV_I8(r, 16), EKV_I8(r, 24), "r"(address)
         : "memory");
 }
-__device__ __forceinline__ void tensor_store16(uint32_t address, const uint32_t (&r)[16]) {
+__device__ __forceinline__ void tensor_load16(uint32_t address, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : EKV_R8(r, 0), EKV_R8(r, 8)
+        : "r"(address));
+}
+__device__ __forceinline__ void tensor_store16(uint32_t address, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::EKV_I8(
             r, 0),
@@ -152,6 +167,24 @@ __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Two 32-bit operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, z, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n mov.b64 z, {%6, %7};\n"
+        " fma.rn.f32x2 w, x, y, z;\n mov.b64 {%0, %1}, w;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n .reg .b64 x, y, w;\n mov.b64 x, {%2, %3};\n mov.b64 y, {%4, %5};\n add.rn.f32x2 w, x, y;\n"
+        " mov.b64 {%0, %1}, w;\n}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
 }
 
 }  // namespace ekv
