@@ -19,15 +19,16 @@
 //
 // attention_kernel, one tile: S = Q K^T and O += P V on the tensor cores (tcgen05, 128 rows x
 // 128 positions, 32-bit sums in tensor memory), a softmax thread per row between them.
-// Roles by warp: 0-3 and 4-7 softmax of row tile halves ("slots") 0 and 1; 8-11 gather the K and V rows
+// Roles by warp: 0-3 and 4-7 softmax of row tile halves ("slots") 0 and 1; 8-15 gather the K and V rows
 // into swizzled shared memory (cp.async, 16 bytes a lane, whole rows; slots resolved through
-// the table, zeros for positions without one); 12 and 13 issue the products of slots 0 and 1 (one
-// thread each, so that the waits and commits of one fall beside the other's products); 14 walks the
-// block's items and hands them to the others through a small ring; 15 passes on what the gather
+// the table, zeros for positions without one); 16 and 17 issue the products of slots 0 and 1 (one
+// thread each, so that the waits and commits of one fall beside the other's products); 18 walks the
+// block's items and hands them to the others through a small ring; 19 passes on what the gather
 // has written, with the fence between ordinary writes and the tensor cores' reads.
-// A 256-row item uses both slots
-// on the same K and V; smaller items alternate between them, so one's softmax runs beside
-// the other's products.  The maximum a row's weights refer to is raised only when the tile's
+// An item of more than 128 rows uses both
+// slots on the same K and V; a smaller one with many tiles gives its even tiles to one slot and
+// its odd ones to the other (kPair; the two join before they are written); with few tiles, items
+// alternate between the slots.  In each case one slot's softmax runs beside the other's products.  The maximum a row's weights refer to is raised only when the tile's
 // maximum passes it by 2^8 (kRaise), which makes rescaling O rare; sums stay exact to 32 bits since the
 // weights are bounded by 2^8.  Weights are rounded to the 16-bit type for the second product
 // (its operand type), the row sum is taken of the unrounded ones.
@@ -41,18 +42,22 @@ namespace {
 
 constexpr int kRows = 128;           // rows of a slot (tensor-memory lanes)
 constexpr int kTile = 128;           // positions of a tile
-constexpr int kGatherWarps = 4;
-constexpr int kGatherRows = kTile / kGatherWarps;  // rows of a tile one gather warp copies, one a lane to look up
-static_assert(kGatherRows == 32, "a lane resolves one row");
+// Eight warps gather: the copies one warp has in flight are few (four warps reached 12 bytes a cycle and
+// SM from HBM where eight reach 21).
+constexpr int kGatherWarps = 8;
+constexpr int kGatherRows = kTile / kGatherWarps;  // rows of a tile one gather warp copies
 constexpr int kThreads = 256 + 32 * kGatherWarps + 128;
-// Registers a thread: 512 threads start with 128; the softmax warps take what the others give
-// up, for the row of scores each of their threads holds.
-constexpr int kStartRegisters = 128, kSoftmaxRegisters = 184, kGatherRegisters = 72, kIssueRegisters = 72;
-static_assert(256 * kSoftmaxRegisters + 32 * kGatherWarps * kGatherRegisters + 128 * kIssueRegisters <=
+// Registers a thread: 640 threads start with 96; the softmax warps take what the gather gives up.
+constexpr int kStartRegisters = 96, kSoftmaxRegisters = 128, kGatherRegisters = 64, kOtherRegisters = 96;
+static_assert(256 * kSoftmaxRegisters + 32 * kGatherWarps * kGatherRegisters + 128 * kOtherRegisters <=
                   kThreads * kStartRegisters, "more registers than the block starts with");
 constexpr int kMaxEntries = EKV_ATTENTION_MAX_ROW_TILES;
-constexpr int kItemCost = 1;         // an item's start, in units of which ...
-constexpr int kTileCost = 2;         // ... a tile is kTileCost
+// What an item costs, in a common unit: a start (queries, first keys, writing the result) and
+// each tile; kBoth items of more than 128 rows, others below.  A share of equal cost per block.
+constexpr int kBothStart = 24, kBothTile = 6;
+constexpr int kSmallStart = 3, kSmallTile = 4;
+constexpr int kPairTiles = 4;        // tiles from which a small item uses both slots
+enum Mode { kSingle = 0, kBoth = 1, kPair = 2 };
 constexpr int kMaskRing = 8;         // more than the stages of any layout
 constexpr int kItemRing = 4;
 constexpr float kRaise = 8.f;
@@ -86,9 +91,10 @@ struct AttentionParams {
     float2* own_stat;
     float* next_out;     // [blocks][256][dim]: the part a block continues
     float2* next_stat;
-    uint32_t* plan_cost; // [kMaxEntries + 1]
-    uint32_t* plan_first;  // [batch + 1]: each request's first entry
-    uint32_t* failed;    // [blocks]
+    uint32_t* item_span;   // of each item the first block with a tile of it, and the last << 16
+    uint32_t* first_entry; // [batch]: each request's first entry
+    int* next_item;      // [blocks]: the item of the part a block continues, or -1
+    uint32_t* failed;    // [blocks]: a wait ran out
 };
 
 // ---------------------------------------------------------------- requests
@@ -154,12 +160,22 @@ struct Plan {
     int32_t end[kMaxEntries];        // positions the tile's last row sees
     uint16_t request[kMaxEntries];
     uint16_t row_tile[kMaxEntries];
+    uint8_t small[kMaxEntries];      // up to 128 rows
     int64_t scratch[kThreads / 32];
     uint32_t entries;
 };
 
-__device__ __forceinline__ uint32_t item_cost(int64_t tiles) {
-    return tiles > 0 ? static_cast<uint32_t>(kItemCost + kTileCost * tiles) : 0u;
+struct Cost {
+    int start, tile;
+};
+__host__ __device__ __forceinline__ Cost cost_of(int64_t rows) {
+    return rows > kRows ? Cost{kBothStart, kBothTile} : Cost{kSmallStart, kSmallTile};
+}
+__device__ __forceinline__ uint32_t item_cost(Cost c, int64_t tiles) {
+    return tiles > 0 ? static_cast<uint32_t>(c.start + c.tile * tiles) : 0u;
+}
+__device__ __forceinline__ int item_tiles(Cost c, uint32_t cost) {
+    return cost ? static_cast<int>((cost - c.start) / c.tile) : 0;
 }
 
 // Index (in the request) of the last token of a row tile.
@@ -200,12 +216,13 @@ __device__ __forceinline__ void build_plan(const AttentionParams& p, Plan& plan)
         int64_t total;
         const int64_t at = entries + block_scan(tiles, total, plan.scratch);
         if (b < p.batch) {
-            if (blockIdx.x == 0) p.plan_first[b] = static_cast<uint32_t>(at < kMaxEntries ? at : kMaxEntries);
+            if (blockIdx.x == 0) p.first_entry[b] = static_cast<uint32_t>(at < kMaxEntries ? at : kMaxEntries);
             for (int64_t t = 0; t < tiles && at + t < kMaxEntries; ++t) {
                 const int64_t seen = r.length - r.fresh + last_token(t, r.fresh, p.group) + 1;
                 plan.request[at + t] = static_cast<uint16_t>(b);
                 plan.row_tile[at + t] = static_cast<uint16_t>(t);
                 plan.end[at + t] = static_cast<int32_t>(seen);
+                plan.small[at + t] = r.fresh * p.group - t * 2 * kRows <= kRows;
             }
         }
         entries += total;
@@ -219,43 +236,79 @@ __device__ __forceinline__ void build_plan(const AttentionParams& p, Plan& plan)
         uint32_t cost = 0;
         if (e < entries) {
             const int64_t end = plan.end[e] < reach ? plan.end[e] : reach;
-            cost = item_cost((end - p.shared + kTile - 1) / kTile);
+            cost = item_cost(cost_of(plan.small[e] ? 1 : 2 * kRows), (end - p.shared + kTile - 1) / kTile);
             if (end <= p.shared) cost = 0;
         }
         int64_t total;
         const uint32_t at = running + static_cast<uint32_t>(block_scan(cost, total, plan.scratch));
-        if (e < entries) {
-            plan.cost[e] = at;
-            if (blockIdx.x == 0) p.plan_cost[e] = at;
-        }
+        if (e < entries) plan.cost[e] = at;
         running += static_cast<uint32_t>(total);
     }
     if (threadIdx.x == 0) {
         plan.cost[entries] = running;
         plan.entries = static_cast<uint32_t>(entries);
-        if (blockIdx.x == 0) {
-            p.plan_cost[entries] = running;
-            p.plan_first[p.batch] = static_cast<uint32_t>(entries);
-        }
     }
     __syncthreads();
 }
 
 // Block `block`'s share of [0, total) begins here.
 __device__ __forceinline__ int64_t share_begin(int64_t block, int64_t total, int blocks) {
-    return total * block / blocks;  // below 2^63: the total is below 2^49
+    const int64_t product = total * block;  // below 2^63: the total is below 2^49
+    if (product <= UINT32_MAX) return static_cast<uint32_t>(product) / static_cast<uint32_t>(blocks);
+    return product / blocks;
+}
+
+// The block whose share holds `at`.
+__device__ __forceinline__ int owner(int64_t at, int64_t total, int blocks) {
+    const int64_t product = (at + 1) * blocks - 1;
+    if (product <= UINT32_MAX && total <= UINT32_MAX) {
+        return static_cast<int>(static_cast<uint32_t>(product) / static_cast<uint32_t>(total));
+    }
+    return static_cast<int>(product / total);
 }
 
 // First tile at or behind position x of an item that begins at `start` (its tile t > 0 lies at
-// start + kItemCost + t * kTileCost).
-__device__ __forceinline__ int first_tile(int64_t x, int64_t start, int tiles) {
+// start + c.start + t * c.tile).
+__device__ __forceinline__ int first_tile(Cost c, int64_t x, int64_t start, int tiles) {
     if (x <= start) return 0;
-    int64_t t = (x - start - kItemCost + kTileCost - 1) / kTileCost;
+    const int64_t behind = x - start - c.start + c.tile - 1;
+    int64_t t = behind >= 0 && behind <= UINT32_MAX ? static_cast<uint32_t>(behind) / static_cast<uint32_t>(c.tile)
+                                                    : behind / c.tile;
     if (t < 1) t = 1;
     return t < tiles ? static_cast<int>(t) : tiles;
 }
 
+// The blocks that each item spans, for combine_kernel; every block of the grid writes some.
+__device__ __forceinline__ void write_spans(const AttentionParams& p, const Plan& plan) {
+    const Cost prefix = cost_of(p.head_rows);
+    const uint32_t prefix_cost = item_cost(prefix, p.prefix_tiles);
+    const int prefix_items = p.prefix_tiles ? p.prefix_row_tiles * p.kv_heads : 0;
+    const int64_t prefix_total = static_cast<int64_t>(prefix_cost) * prefix_items;
+    const int64_t total = prefix_total + static_cast<int64_t>(plan.cost[plan.entries]) * p.kv_heads;
+    const int items = prefix_items + static_cast<int>(plan.entries) * p.kv_heads;
+    for (int i = blockIdx.x * kThreads + threadIdx.x; i < items; i += gridDim.x * kThreads) {
+        Cost c = prefix;
+        uint32_t cost = prefix_cost;
+        int64_t start = static_cast<int64_t>(i) * prefix_cost;
+        if (i >= prefix_items) {
+            const int e = (i - prefix_items) / p.kv_heads, head = i - prefix_items - e * p.kv_heads;
+            c = cost_of(plan.small[e] ? 1 : 2 * kRows);
+            cost = plan.cost[e + 1] - plan.cost[e];
+            start = prefix_total + static_cast<int64_t>(plan.cost[e]) * p.kv_heads + static_cast<int64_t>(head) * cost;
+        }
+        uint32_t span = 1;  // first 1, last 0: nothing
+        if (cost) {
+            const int tiles = item_tiles(c, cost);
+            const int64_t last = start + (tiles > 1 ? c.start + static_cast<int64_t>(tiles - 1) * c.tile : 0);
+            span = static_cast<uint32_t>(owner(start, total, p.blocks)) |
+                   static_cast<uint32_t>(owner(last, total, p.blocks)) << 16;
+        }
+        p.item_span[i] = span;
+    }
+}
+
 struct __align__(16) Item {
+    int mode;       // Mode: how the slots share it
     int prefix;
     int first;      // this block has the item's first tile
     int head;
@@ -264,6 +317,7 @@ struct __align__(16) Item {
     int low, high;  // tiles of this block
     int begin, end; // positions of the whole item
     int table_row;  // -1: no row of the table
+    int id;         // prefix items first, then the own ones, entry by entry
     int token;      // query token of row 0 of the head or request
     int bias;       // own items: token i of the request sees bias + i positions
 };
@@ -278,7 +332,7 @@ struct Walk {
 
 __device__ __forceinline__ Walk begin_walk(const AttentionParams& p, const Plan& plan) {
     Walk w;
-    w.prefix_cost = item_cost(p.prefix_tiles);
+    w.prefix_cost = item_cost(cost_of(p.head_rows), p.prefix_tiles);
     w.prefix_items = p.prefix_tiles ? p.prefix_row_tiles * p.kv_heads : 0;
     const int64_t prefix_total = static_cast<int64_t>(w.prefix_cost) * w.prefix_items;
     const int64_t total = prefix_total + static_cast<int64_t>(plan.cost[plan.entries]) * p.kv_heads;
@@ -314,10 +368,12 @@ __device__ __forceinline__ bool next_item(const AttentionParams& p, const Plan& 
         const int64_t start = static_cast<int64_t>(w.index) * w.prefix_cost;
         if (start >= w.stop) return false;
         const int i = w.index++;
-        item.low = first_tile(w.start, start, p.prefix_tiles);
-        item.high = first_tile(w.stop, start, p.prefix_tiles);
+        const Cost c = cost_of(p.head_rows);
+        item.low = first_tile(c, w.start, start, p.prefix_tiles);
+        item.high = first_tile(c, w.stop, start, p.prefix_tiles);
         if (item.low >= item.high) continue;
         item.prefix = 1;
+        item.id = i;
         item.first = item.low == 0;
         item.head = i / p.prefix_row_tiles;
         item.row = (i - item.head * p.prefix_row_tiles) * 2 * kRows;
@@ -341,12 +397,14 @@ __device__ __forceinline__ bool next_item(const AttentionParams& p, const Plan& 
             w.head = 0;
         }
         if (!cost) continue;
-        const int tiles = static_cast<int>((cost - kItemCost) / kTileCost);
-        item.low = first_tile(w.start, start, tiles);
-        item.high = first_tile(w.stop, start, tiles);
+        const Cost c = cost_of(plan.small[e] ? 1 : 2 * kRows);
+        const int tiles = item_tiles(c, static_cast<uint32_t>(cost));
+        item.low = first_tile(c, w.start, start, tiles);
+        item.high = first_tile(c, w.stop, start, tiles);
         if (item.low >= item.high) continue;
         const int64_t reach = p.table_width * p.page_size;
         item.prefix = 0;
+        item.id = w.prefix_items + static_cast<int>(e) * p.kv_heads + head;
         item.first = item.low == 0;
         item.head = head;
         const int64_t b = plan.request[e];
@@ -363,6 +421,10 @@ __device__ __forceinline__ bool next_item(const AttentionParams& p, const Plan& 
         return true;
     }
     return false;
+}
+
+__device__ __forceinline__ int mode_of(const Item& item) {
+    return item.rows > kRows ? kBoth : (item.high - item.low >= kPairTiles ? kPair : kSingle);
 }
 
 // Positions that an item's row sees; false for a row of no request.
@@ -391,9 +453,11 @@ struct Layout {
     static constexpr uint32_t kPlan = kValues + kStages * kOperand;
     static constexpr uint32_t kItems = kPlan + ((sizeof(Plan) + 15) / 16) * 16;
     static constexpr uint32_t kMasks = kItems + kItemRing * sizeof(Item);
-    static constexpr uint32_t kBarriers = kMasks + kMaskRing * 16;
-    // Six of each stage, seven of each slot, two of each place in the item ring.
-    static constexpr int kBarrierCount = 6 * kStages + 7 * 2 + 2 * kItemRing;
+    static constexpr uint32_t kStats = kMasks + kMaskRing * 16;  // maximum and sum of each row, of both slots
+    static constexpr uint32_t kBarriers = kStats + 2 * kRows * 8;
+    // Six of each stage, eight of each slot, two of each place in the item ring, eight for the
+    // turns, one where the slots of a pair meet.
+    static constexpr int kBarrierCount = 6 * kStages + 8 * 2 + 2 * kItemRing + 8 + 1;
     static constexpr uint32_t kTail = kBarriers + kBarrierCount * 8;
     static constexpr uint32_t kBytes = kTail + 16;  // tensor-memory address, failed flag
 };
@@ -445,15 +509,18 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     const auto s_full = [&](int s) { return slot_barrier(3, s); };
     const auto p_full = [&](int s) { return slot_barrier(4, s); };
     const auto o_full = [&](int s) { return slot_barrier(5, s); };
-    const auto item_full = [&](int i) { return barriers + 8 * (6 * L::kStages + 12 + i); };
-    const auto item_empty = [&](int i) { return barriers + 8 * (6 * L::kStages + 12 + kItemRing + i); };
+    const auto p_half = [&](int s) { return slot_barrier(6, s); };
+    const auto item_full = [&](int i) { return barriers + 8 * (6 * L::kStages + 14 + i); };
+    const auto item_empty = [&](int i) { return barriers + 8 * (6 * L::kStages + 14 + kItemRing + i); };
+    const auto go = [&](int s, int w) { return barriers + 8 * (L::kBarrierCount - 11 + 4 * s + w); };
+    const uint32_t meet = barriers + 8 * (L::kBarrierCount - 3);
     const auto drain = [&](int s) { return barriers + 8 * (L::kBarrierCount - 2 + s); };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < L::kStages; ++s) {
             barrier_init(k_landed(s), 32 * kGatherWarps);
             barrier_init(k_full(s), 1);
-            barrier_init(k_empty(s), 2);  // both slots, whether they use the tile or not
+            barrier_init(k_empty(s), 2);  // both slots, or one of them and the warp that passes on
             barrier_init(v_landed(s), 32 * kGatherWarps);
             barrier_init(v_full(s), 1);
             barrier_init(v_empty(s), 2);
@@ -463,10 +530,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             barrier_init(q_full(s), 1);
             barrier_init(q_empty(s), 1);
             barrier_init(s_full(s), 1);
+            barrier_init(p_half(s), 4);
             barrier_init(p_full(s), 4);
             barrier_init(o_full(s), 1);
             barrier_init(drain(s), 1);
+            for (int w = 0; w < 4; ++w) barrier_init(go(s, w), 1);
         }
+        barrier_init(meet, 8);
         for (int i = 0; i < kItemRing; ++i) {
             barrier_init(item_full(i), 1);
             barrier_init(item_empty(i), 8 + kGatherWarps + 3);  // every warp but the one that walks
@@ -479,6 +549,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     grid_dependency_wait();
     tensor_fence_before();
     build_plan(p, plan);  // ends with __syncthreads
+    write_spans(p, plan);
     tensor_fence_after();
     const uint32_t tensor = *reinterpret_cast<volatile uint32_t*>(shared + L::kTail);
 
@@ -506,15 +577,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 tensor-memory lanes a warp
         const uint32_t scores = tensor + lanes + slot * kTile;
         const uint32_t output = tensor + lanes + 256 + slot * 128;
-        uint32_t uses = 0, ends = 0, tile_count = 0;
+        uint32_t uses = 0, ends = 0, tiles_before = 0, turns = 0, meetings = 0;
         const int r = (warp & 3) * 32 + lane;
+        float2* stats = reinterpret_cast<float2*>(shared + L::kStats);
         while (next(false)) {
-            const bool both = item.rows > kRows;
-            const int mine = both ? slot : turn;
-            turn ^= 1;
-            if (mine != slot) {
-                tile_count += static_cast<uint32_t>(item.high - item.low);
-                continue;
+            const bool both = item.mode == kBoth, pair = item.mode == kPair;
+            const uint32_t tiles = tiles_before;
+            tiles_before += static_cast<uint32_t>(item.high - item.low);
+            if (item.mode == kSingle) {
+                const int owner = turn;
+                turn ^= 1;
+                if (owner != slot) continue;
             }
             const int item_row = (both ? slot * kRows : 0) + r;
             int64_t seen;
@@ -525,37 +598,59 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             const bool idle = (both ? slot * kRows : 0) + (warp & 3) * 32 >= item.rows;  // no row in this warp
             float top = -INFINITY;
             float2 total = make_float2(0.f, 0.f);
-            for (int t = item.low; t < item.high; ++t, ++tile_count) {
+            const int low = item.low + (pair ? slot : 0), step = pair ? 2 : 1;
+            for (int t = low; t < item.high; t += step) {
                 if (!__all_sync(0xffffffffu, barrier_wait(s_full(slot), uses & 1, failed))) goto finish;
                 ++uses;
                 tensor_fence_after();
                 if (!idle) {
-                    uint32_t s[kTile];
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) tensor_load32(scores + 32 * c, s + 32 * c);
                     // Positions this row sees here: those that have a slot, up to its last.
                     const int left = limit - t * kTile;
-                    const uint4 there = masks[tile_count % kMaskRing];
+                    const uint4 there = masks[(tiles + (t - item.low)) % kMaskRing];
                     const bool whole = __all_sync(0xffffffffu, left >= kTile) &&
                                        (there.x & there.y & there.z & there.w) == 0xffffffffu;
-                    tensor_wait_load();
                     if (!whole) {
-#pragma unroll
+#pragma unroll 1
                         for (int c = 0; c < 4; ++c) {
                             const uint32_t bits = c == 0 ? there.x : c == 1 ? there.y : c == 2 ? there.z : there.w;
+                            const int limit32 = left - 32 * c;
+                            const uint32_t seen32 =
+                                bits & (limit32 >= 32 ? 0xffffffffu : (limit32 <= 0 ? 0u : (1u << limit32) - 1u));
+                            if (__all_sync(0xffffffffu, seen32 == 0xffffffffu)) continue;
+                            uint32_t masked[32];
+                            tensor_load32(scores + 32 * c, masked);
+                            tensor_wait_load();
 #pragma unroll
                             for (int j = 0; j < 32; ++j) {
-                                if (!(bits >> j & 1u) || 32 * c + j >= left) s[32 * c + j] = 0xff800000u;  // -inf
+                                if (!(seen32 >> j & 1u)) masked[j] = 0xff800000u;  // -inf
+                            }
+                            tensor_store32(scores + 32 * c, masked);
+                        }
+                        tensor_wait_store();
+                    }
+                    // Largest score: 32 columns are compared while the next 32 are on their way.  The loops over a
+                    // tile are kept rolled: with 128 columns unrolled the kernel ran 1.6 times slower, its roles'
+                    // code exceeding the instruction cache.
+                    uint32_t a[32], b[32];
+                    float highs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    const auto raise_to = [&](const uint32_t* s) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 8) {
+#pragma unroll
+                            for (int c = 0; c < 4; ++c) {
+                                highs[c] = max3(highs[c], __uint_as_float(s[j + 2 * c]), __uint_as_float(s[j + 2 * c + 1]));
                             }
                         }
-                    }
-                    float highs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                    for (int j = 0; j < kTile; j += 8) {
-#pragma unroll
-                        for (int c = 0; c < 4; ++c) {
-                            highs[c] = fmaxf(highs[c], fmaxf(__uint_as_float(s[j + 2 * c]), __uint_as_float(s[j + 2 * c + 1])));
-                        }
+                    };
+                    tensor_load32(scores, a);
+#pragma unroll 1
+                    for (int c = 0; c < kTile; c += 64) {
+                        tensor_wait_load();
+                        tensor_load32(scores + c + 32, b);
+                        raise_to(a);
+                        tensor_wait_load();
+                        tensor_load32(scores + (c ? 0 : 64), a);  // the second time the first columns again, for below
+                        raise_to(b);
                     }
                     const float high = fmaxf(fmaxf(highs[0], highs[1]), fmaxf(highs[2], highs[3])) * p.scale_log2;
                     const bool raise = present && (high > top + kRaise || (top == -INFINITY && high > -INFINITY));
@@ -565,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                         const float factor = raise ? (before == -INFINITY ? 0.f : exp2_approx(before - top)) : 1.f;
                         total.x *= factor;
                         total.y *= factor;
-                        if (t > item.low) {
+                        if (t > low) {
                             // The products of this slot's earlier tiles are complete (s_full).
 #pragma unroll 1
                             for (int c = 0; c < kDim / 16; ++c) {
@@ -579,22 +674,54 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                         }
                     }
                     const float shift = top == -INFINITY ? 0.f : -top;
+                    // The exponentials of the two slots take turns (a warp of each shares a quarter of
+                    // the SM): together they would leave the tensor cores idle, and then wait for them together.
+                    if (both && !__all_sync(0xffffffffu, barrier_wait(go(slot, warp & 3), (turns & 1) ^ (slot ^ 1), failed))) {
+                        goto finish;
+                    }
+                    const auto weigh = [&](const uint32_t* s, uint32_t target) {
+                        uint32_t weights[16];
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {
-                        uint32_t weights[32];
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const int at = 64 * c + 2 * j;
-                            float2 x = fma2(make_float2(__uint_as_float(s[at]), __uint_as_float(s[at + 1])),
+                        for (int j = 0; j < 32; j += 2) {
+                            float2 x = fma2(make_float2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])),
                                             make_float2(p.scale_log2, p.scale_log2), make_float2(shift, shift));
                             x.x = exp2_approx(x.x);
                             x.y = exp2_approx(x.y);
                             total = add2(total, x);
-                            weights[j] = Kind<T>::pack(x.x, x.y);
+                            weights[j / 2] = Kind<T>::pack(x.x, x.y);
                         }
-                        tensor_store32(scores + 32 * c, weights);
+                        tensor_store16(target, weights);
+                    };
+#pragma unroll 1
+                    for (int c = 0; c < kTile; c += 64) {
+                        tensor_wait_load();
+                        tensor_load32(scores + c + 32, b);
+                        weigh(a, scores + c / 2);
+                        if (c) {  // the second product may begin on the first half, whose stores have had time to land
+                            tensor_wait_store();
+                            tensor_fence_before();
+                            __syncwarp();
+                            if (lane == 0) barrier_arrive(p_half(slot));
+                        }
+                        tensor_wait_load();
+                        if (c == 0) tensor_load32(scores + 64, a);
+                        weigh(b, scores + c / 2 + 16);
                     }
                     tensor_wait_store();
+                    if (both) {
+                        __syncwarp();
+                        if (lane == 0) barrier_arrive(go(slot ^ 1, warp & 3));
+                        ++turns;
+                    }
+                } else {
+                    if (lane == 0) barrier_arrive(p_half(slot));
+                    if (both) {
+                        if (!__all_sync(0xffffffffu, barrier_wait(go(slot, warp & 3), (turns & 1) ^ (slot ^ 1), failed))) {
+                            goto finish;
+                        }
+                        if (lane == 0) barrier_arrive(go(slot ^ 1, warp & 3));
+                        ++turns;
+                    }
                 }
                 tensor_fence_before();
                 __syncwarp();
@@ -603,6 +730,23 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             if (!__all_sync(0xffffffffu, barrier_wait(o_full(slot), ends & 1, failed))) goto finish;
             ++ends;
             tensor_fence_after();
+            float sum = total.x + total.y, factor = 1.f, other = 0.f;
+            if (pair) {
+                // The slots exchange their maxima and sums; each then joins half of the columns.
+                stats[slot * kRows + r] = make_float2(top, sum);
+                __syncwarp();
+                if (lane == 0) barrier_arrive(meet);
+                if (!__all_sync(0xffffffffu, barrier_wait(meet, meetings & 1, failed))) goto finish;
+                ++meetings;
+                const float2 its = stats[(slot ^ 1) * kRows + r];
+                const float higher = fmaxf(top, its.x);
+                if (higher > -INFINITY) {
+                    factor = exp2_approx(top - higher);
+                    other = exp2_approx(its.x - higher);
+                }
+                top = higher;
+                sum = sum * factor + its.y * other;
+            }
             if (!idle) {
                 float* partial;
                 float2* stat;
@@ -617,20 +761,34 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                     partial = p.next_out + row * kDim;
                     stat = p.next_stat + row;
                 }
+                const int first = pair ? slot * (kDim / 2) : 0, last = pair ? first + kDim / 2 : kDim;
+                const uint32_t peer = tensor + lanes + 256 + (slot ^ 1) * 128;
 #pragma unroll 1
-                for (int c = 0; c < kDim / 32; ++c) {
-                    uint32_t o[32];
-                    tensor_load32(output + 32 * c, o);
+                for (int c = first; c < last; c += 32) {
+                    uint32_t o[32], q[32];
+                    tensor_load32(output + c, o);
+                    if (pair) tensor_load32(peer + c, q);
                     tensor_wait_load();
-                    if (present) {
+                    if (pair) {
 #pragma unroll
-                        for (int j = 0; j < 32; j += 4) {
-                            *reinterpret_cast<uint4*>(partial + 32 * c + j) = make_uint4(o[j], o[j + 1], o[j + 2], o[j + 3]);
+                        for (int j = 0; j < 32; ++j) {
+                            o[j] = __float_as_uint(__uint_as_float(o[j]) * factor + __uint_as_float(q[j]) * other);
                         }
                     }
+                    if (present) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 8) store_sector(partial + c + j, o + j);
+                    }
                 }
-                if (present) *stat = make_float2(top, total.x + total.y);
+                if (present && (!pair || slot == 0)) *stat = make_float2(top, sum);
                 tensor_fence_before();
+            }
+            if (pair) {  // neither slot goes on before the other has read its columns
+                __syncwarp();
+                if (lane == 0) barrier_arrive(meet);
+                if (!__all_sync(0xffffffffu, barrier_wait(meet, meetings & 1, failed))) goto finish;
+                ++meetings;
+                tensor_fence_after();
             }
         }
     } else if (warp < kIssueWarp) {
@@ -646,18 +804,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         const auto target = [&](uint32_t operand, int row) {
             return operand + (chunk >> 3) * L::kBlock + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
         };
-        // Plane slot of this lane's row in tile t of the item.
+        // Plane slot of this lane's row (lanes 16-31 repeat 0-15) in tile t of the item.
         const auto find = [&](int t) {
-            const int position = item.begin + t * kTile + first_row + static_cast<int>(lane);
+            const int position = item.begin + t * kTile + first_row + static_cast<int>(lane % kGatherRows);
             return position < item.end ? static_cast<int>(slot_of(p, item.table_row, static_cast<uint32_t>(position))) : -1;
         };
         bool more = next(false);
         int found = more ? find(item.low) : -1;
         while (more) {
-            const bool both = item.rows > kRows;
-            // Queries of the slots the item uses.
-            for (int half = 0; half < (both ? 2 : 1); ++half) {
-                const int slot = both ? half : turn;
+            // Queries of the slots the item uses: other rows for each, or the same ones.
+            for (int use = 0; use < (item.mode == kSingle ? 1 : 2); ++use) {
+                const int slot = item.mode == kSingle ? turn : use, half = item.mode == kBoth ? use : 0;
                 if (!__all_sync(0xffffffffu, barrier_wait(q_empty(slot), (q_uses[slot] & 1) ^ 1, failed))) goto finish;
                 ++q_uses[slot];
                 const uint32_t operand = base + L::kQuery + slot * L::kOperand;
@@ -673,7 +830,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 }
                 copies_arrive(q_landed(slot));
             }
-            turn ^= 1;
+            if (item.mode == kSingle) turn ^= 1;
             const char* keys = static_cast<const char*>(p.k_plane) + 2 * item.head * p.k_head + 16 * chunk;
             const char* values = static_cast<const char*>(p.v_plane) + 2 * item.head * p.v_head + 16 * chunk;
             const int high = item.high;
@@ -690,31 +847,32 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 }
                 const uint32_t there = __ballot_sync(0xffffffffu, now >= 0);
                 if (!__all_sync(0xffffffffu, barrier_wait(k_empty(stage), parity, failed))) goto finish;
-                // The mask's place was tile n - kMaskRing's.  The stage is empty when the first
-                // products of tile n - kStages are complete, which follow the softmax of every earlier tile.
-                if (lane == 0) reinterpret_cast<uint32_t*>(&masks[uses % kMaskRing])[warp - 8] = there;
+                // The mask's place was tile n - kMaskRing's.  This warp has copied V of tile n - 1, so the second
+                // products, and with them the softmax, of all tiles up to n - 1 - kStages are complete.
+                if (lane == 0) reinterpret_cast<uint16_t*>(&masks[uses % kMaskRing])[warp - 8] = static_cast<uint16_t>(there);
                 uint32_t operand = base + L::kKeys + stage * L::kOperand;
-#pragma unroll 8
-                for (int i = 0; i < kGatherRows; i += kAtOnce) {
-                    const int slot = __shfl_sync(0xffffffffu, now, i + sub);
-                    copy16_async(target(operand, first_row + i + sub), slot >= 0 ? keys + 2 * (slot * p.k_slot) : query,
-                                 slot >= 0 ? 16 : 0);
-                }
-                copies_arrive(k_landed(stage));
-                if (!__all_sync(0xffffffffu, barrier_wait(v_empty(stage), parity, failed))) goto finish;
-                operand = base + L::kValues + stage * L::kOperand;
-#pragma unroll 8
-                for (int i = 0; i < kGatherRows; i += kAtOnce) {
-                    const int slot = __shfl_sync(0xffffffffu, now, i + sub);
-                    copy16_async(target(operand, first_row + i + sub), slot >= 0 ? values + 2 * (slot * p.v_slot) : query,
-                                 slot >= 0 ? 16 : 0);
+                const char* plane = keys;
+                int64_t stride = 2 * p.k_slot;
+#pragma unroll 1
+                for (int which = 0; which < 2; ++which) {
+#pragma unroll 4
+                    for (int i = 0; i < kGatherRows; i += kAtOnce) {
+                        const int slot = __shfl_sync(0xffffffffu, now, i + sub);
+                        copy16_async(target(operand, first_row + i + sub), slot >= 0 ? plane + slot * stride : query,
+                                     slot >= 0 ? 16 : 0);
+                    }
+                    if (which) break;
+                    copies_arrive(k_landed(stage));
+                    if (!__all_sync(0xffffffffu, barrier_wait(v_empty(stage), parity, failed))) goto finish;
+                    operand = base + L::kValues + stage * L::kOperand;
+                    plane = values;
+                    stride = 2 * p.v_slot;
                 }
                 copies_arrive(v_landed(stage));
             }
         }
-    } else {
-        registers_shrink<kIssueRegisters>();
-        if (warp < kIssueWarp + 2 && lane == 0) {
+    } else if (lane == 0) {
+        if (warp < kIssueWarp + 2) {
             // -------------------------------------------------------- products of slot `slot`
             constexpr uint32_t kScoreProduct = mma_descriptor(Kind<T>::kBf16, kRows, kTile, false);
             constexpr uint32_t kOutputProduct = mma_descriptor(Kind<T>::kBf16, kRows, kDim, true);
@@ -726,64 +884,89 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             uint32_t uses = 0, q_uses = 0, p_uses = 0;
             bool fine = true;
             while (fine && next(true)) {
-                const bool mine = item.rows > kRows || turn == slot;
-                turn ^= 1;
-                const int low = item.low, high = item.high;
-                if (mine) {
-                    fine = barrier_wait(q_full(slot), q_uses & 1, failed);
-                    ++q_uses;
+                const bool pair = item.mode == kPair;
+                const uint32_t before = uses - item.low;  // tile t of the item is the block's tile before + t
+                uses += item.high - item.low;
+                if (item.mode == kSingle) {
+                    const int owner = turn;
+                    turn ^= 1;
+                    if (owner != slot) continue;
                 }
-                for (int t = low; fine && t < high; ++t, ++uses) {
-                    const int stage = uses % L::kStages;
-                    const uint32_t parity = (uses / L::kStages) & 1;
-                    if (!(fine = barrier_wait(k_full(stage), parity, failed))) break;
-                    if (!mine) {
-                        barrier_arrive(k_empty(stage));
-                        if (!(fine = barrier_wait(v_full(stage), parity, failed))) break;
-                        barrier_arrive(v_empty(stage));
-                        continue;
-                    }
-                    tensor_fence_after();
-                    const uint64_t keys = all_keys + stage * (L::kOperand >> 4);
+                const int low = item.low + (pair ? slot : 0), high = item.high, step = pair ? 2 : 1;
+                if (!(fine = barrier_wait(q_full(slot), q_uses & 1, failed))) break;
+                ++q_uses;
+                // The first product of the first tile; then the second product of tile t with the first one
+                // of tile t + 1 right behind it, so that the next scores are on their way at once.
+                const auto first = [&](uint32_t use) {
+                    const uint64_t keys = all_keys + (use % L::kStages) * (L::kOperand >> 4);
 #pragma unroll
                     for (int k = 0; k < kDim / 16; ++k) {
                         const uint32_t step = (k / 4) * (L::kBlock >> 4) + (k % 4) * 2;
                         mma_shared(scores, queries + step, keys + step, kScoreProduct, k > 0);
                     }
                     mma_commit(s_full(slot));
-                    mma_commit(k_empty(stage));
-                    if (t + 1 == high) mma_commit(q_empty(slot));
-                    if (!(fine = barrier_wait(v_full(stage), parity, failed))) break;
+                    mma_commit(k_empty(use % L::kStages));
+                };
+                const auto parity = [&](uint32_t use) { return (use / L::kStages) & 1; };
+                uint32_t use = before + low;
+                if (!(fine = barrier_wait(k_full(use % L::kStages), parity(use), failed))) break;
+                tensor_fence_after();
+                first(use);
+                if (low + step >= high) mma_commit(q_empty(slot));
+                for (int t = low; t < high; t += step, use += step) {
+                    const int stage = use % L::kStages;
+                    const uint32_t next_use = use + step;
+                    if (!(fine = barrier_wait(v_full(stage), parity(use), failed))) break;
+                    const uint64_t values = all_values + stage * (L::kOperand >> 4);
+                    if (!(fine = barrier_wait(p_half(slot), p_uses & 1, failed))) break;
+                    tensor_fence_after();
+#pragma unroll
+                    for (int k = 0; k < kTile / 32; ++k) {
+                        mma_tensor(output, scores + 8 * k, values + k * (16 * 128 >> 4), kOutputProduct, t > low || k > 0);
+                    }
+                    const bool more = t + step < high;
+                    const bool ready = more && barrier_test(k_full(next_use % L::kStages), parity(next_use));
                     if (!(fine = barrier_wait(p_full(slot), p_uses & 1, failed))) break;
                     ++p_uses;
                     tensor_fence_after();
-                    const uint64_t values = all_values + stage * (L::kOperand >> 4);
 #pragma unroll
-                    for (int k = 0; k < kTile / 16; ++k) {
-                        mma_tensor(output, scores + 8 * k, values + k * (16 * 128 >> 4), kOutputProduct, t > low || k > 0);
+                    for (int k = kTile / 32; k < kTile / 16; ++k) {
+                        mma_tensor(output, scores + 8 * k, values + k * (16 * 128 >> 4), kOutputProduct, true);
                     }
-                    mma_commit(v_empty(stage));
-                    if (t + 1 == high) mma_commit(o_full(slot));
+                    if (!ready) mma_commit(v_empty(stage));
+                    if (more) {
+                        if (!ready) {
+                            if (!(fine = barrier_wait(k_full(next_use % L::kStages), parity(next_use), failed))) break;
+                            tensor_fence_after();
+                        }
+                        first(next_use);
+                        if (t + 2 * step >= high) mma_commit(q_empty(slot));
+                    }
+                    if (ready) mma_commit(v_empty(stage));
                 }
+                if (!fine) break;
+                mma_commit(o_full(slot));
             }
             // Nothing may still use tensor memory when it is freed, whatever happened above.
             mma_commit(drain(slot));
             volatile uint32_t ran_out = 0;
             barrier_wait(drain(slot), 0, &ran_out);
-        } else if (warp == kIssueWarp + 2 && lane == 0) {
+        } else if (warp == kIssueWarp + 2) {
             // -------------------------------------------------------- the block's items
             Walk walk = begin_walk(p, plan);
             bool more = true;
             while (more) {
                 more = next_item(p, plan, walk, item);
+                if (!item_uses) p.next_item[blockIdx.x] = more && !item.first ? item.id : -1;
                 if (!more) item.rows = 0;
+                item.mode = mode_of(item);
                 const int place = item_uses % kItemRing;
                 if (!barrier_wait(item_empty(place), ((item_uses / kItemRing) & 1) ^ 1, failed)) break;
                 items[place] = item;
                 barrier_arrive(item_full(place));
                 ++item_uses;
             }
-        } else if (warp == kIssueWarp + 3 && lane == 0) {
+        } else {
             // -------------------------------------------------------- what the gather has written
             uint32_t uses = 0, q_uses[2] = {0, 0};
             bool fine = true;
@@ -794,17 +977,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 return true;
             };
             while (fine && next(true)) {
-                const bool both = item.rows > kRows;
-                for (int half = 0; fine && half < (both ? 2 : 1); ++half) {
-                    const int slot = both ? half : turn;
+                for (int use = 0; fine && use < (item.mode == kSingle ? 1 : 2); ++use) {
+                    const int slot = item.mode == kSingle ? turn : use;
                     fine = pass_on(q_landed(slot), q_full(slot), q_uses[slot] & 1);
                     ++q_uses[slot];
                 }
-                turn ^= 1;
+                if (item.mode == kSingle) turn ^= 1;
                 for (int t = item.low; fine && t < item.high; ++t, ++uses) {
                     const int stage = uses % L::kStages;
                     const uint32_t parity = (uses / L::kStages) & 1;
-                    fine = pass_on(k_landed(stage), k_full(stage), parity) && pass_on(v_landed(stage), v_full(stage), parity);
+                    fine = pass_on(k_landed(stage), k_full(stage), parity);
+                    if (fine && item.mode != kBoth) barrier_arrive(k_empty(stage));  // for the slot that has no use for it
+                    fine = fine && pass_on(v_landed(stage), v_full(stage), parity);
+                    if (fine && item.mode != kBoth) barrier_arrive(v_empty(stage));
                 }
             }
         }
@@ -822,85 +1007,120 @@ finish:
 
 // ---------------------------------------------------------------- joining the parts
 
-// A warp per token and query head: the parts (m_i, l_i, O_i) of a row join as
-// sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i with m = max m_i.
+constexpr int kJoinWarps = 4;
+
+// A warp per token and `per_warp` query heads: the parts (m_i, l_i, O_i) of a row join as
+// sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i with m = max m_i.  The blocks that may hold a part of an
+// item lie next to each other: a lane looks at each, first those of the row's prefix item, then
+// those of its own, so that the loads of one row are all on their way together.
 template <typename T, int kDim>
-__global__ void __launch_bounds__(256) combine_kernel(const __grid_constant__ AttentionParams p) {
+__global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_constant__ AttentionParams p, int per_warp) {
     constexpr int kPer = kDim / 32;
     grid_dependency_wait();
     allow_dependents();
-    const int64_t query_heads = static_cast<int64_t>(p.kv_heads) * p.group;
-    const int64_t index = static_cast<int64_t>(blockIdx.x) * 8 + (threadIdx.x >> 5);
-    const int64_t n = index / query_heads;
-    const int head = static_cast<int>(index - n * query_heads);
-    const unsigned lane = lane_id();
+    const int query_heads = p.kv_heads * p.group;
+    const int turns = (query_heads + per_warp - 1) / per_warp;
+    const int index = blockIdx.x * kJoinWarps + static_cast<int>(threadIdx.x >> 5);
+    const int n = index / turns;
+    const int first_head = (index - n * turns) * per_warp;
+    const int last_head = first_head + per_warp < query_heads ? first_head + per_warp : query_heads;
+    const int lane = static_cast<int>(lane_id());
     int64_t b;
     Request request;
     if (!request_of(p, n, b, request)) return;
-    const int kv_head = head / p.group, g = head - kv_head * p.group;
-    float top = -INFINITY, total = 0.f;
-    float acc[kPer] = {};
-    uint32_t bad = 0;  // a wait ran out in a block whose part is needed
-    const auto join = [&](int64_t block, const float* out, const float2* stat, int64_t row) {
-        const float2 part = stat[row];
-        bad |= p.failed[block];
-        if (part.y == 0.f) return;  // the row sees nothing there
-        const float higher = fmaxf(top, part.x);
-        const float mine = top == -INFINITY ? 0.f : exp2_approx(top - higher), its = exp2_approx(part.x - higher);
-        top = higher;
-        total = total * mine + part.y * its;
-        const float* values = out + row * kDim + lane * kPer;
+    const int prefix_items = p.prefix_tiles ? p.prefix_row_tiles * p.kv_heads : 0;
+    const int first_entry = static_cast<int>(p.first_entry[b]);
+    const int begin = static_cast<int>(request.begin);
+#pragma unroll 1
+    for (int head = first_head; head < last_head; ++head) {
+        const int kv_head = head / p.group, g = head - kv_head * p.group;
+        const int head_row = n * p.group + g, local = head_row - begin * p.group;
+        const int64_t row = static_cast<int64_t>(kv_head) * p.head_rows + head_row;
+        const int prefix_item = kv_head * p.prefix_row_tiles + head_row / (2 * kRows);
+        const int entry = first_entry + local / (2 * kRows);
+        const int own_item = prefix_items + entry * p.kv_heads + kv_head;
+        const uint32_t prefix_span = prefix_items ? p.item_span[prefix_item] : 1;
+        const uint32_t own_span = entry < kMaxEntries ? p.item_span[own_item] : 1;
+        const int prefix_first = prefix_span & 0xffff, prefix_count = static_cast<int>(prefix_span >> 16) - prefix_first + 1;
+        const int own_first = own_span & 0xffff, own_count = static_cast<int>(own_span >> 16) - own_first + 1;
+        float top = -INFINITY, total = 0.f;
+        float acc[kPer] = {};
+        uint32_t bad = 0;  // a wait ran out in a block whose part is needed
+#pragma unroll 1
+        for (int base = 0; base < prefix_count + own_count; base += 32) {
+            int at = base + lane;
+            const bool is_prefix = at < prefix_count;
+            if (!is_prefix) at -= prefix_count;
+            const int block = (is_prefix ? prefix_first : own_first) + at;
+            float2 part = make_float2(-INFINITY, 0.f);
+            const float* values = p.next_out;
+            if (is_prefix || at < own_count) {
+                bad |= p.failed[block];
+                if (at == 0) {
+                    part = (is_prefix ? p.prefix_stat : p.own_stat)[row];
+                    values = (is_prefix ? p.prefix_out : p.own_out) + row * kDim;
+                } else if (p.next_item[block] == (is_prefix ? prefix_item : own_item)) {
+                    const int64_t next = static_cast<int64_t>(block) * 2 * kRows + (is_prefix ? head_row : local) % (2 * kRows);
+                    part = p.next_stat[next];
+                    values = p.next_out + next * kDim;
+                }
+            }
+            uint32_t parts = __ballot_sync(0xffffffffu, part.y != 0.f);  // 0: the row sees nothing there
+            if (!parts) continue;
+            float higher = part.y != 0.f ? part.x : -INFINITY;
 #pragma unroll
-        for (int i = 0; i < kPer; ++i) acc[i] = acc[i] * mine + values[i] * its;
-    };
-    const int64_t prefix_cost = item_cost(p.prefix_tiles);
-    const int64_t prefix_items = p.prefix_tiles ? p.prefix_row_tiles * p.kv_heads : 0;
-    const int64_t prefix_total = prefix_cost * prefix_items;
-    const uint32_t first_entry = p.plan_first[b];
-    const int64_t local = (n - request.begin) * p.group + g;
-    const int64_t entry = first_entry + local / (2 * kRows);
-    const int64_t entries_end = p.plan_first[p.batch];
-    const int64_t total_cost = prefix_total + static_cast<int64_t>(p.plan_cost[entries_end]) * p.kv_heads;
-    const auto join_item = [&](int64_t start, int tiles, const float* out, const float2* stat, int64_t row, int r) {
-        if (tiles <= 0) return;
-        int64_t block = ((start + 1) * p.blocks - 1) / total_cost;  // the share that holds `start`
-        join(block, out, stat, row);
-        int done = first_tile(share_begin(block + 1, total_cost, p.blocks), start, tiles);
-        while (done < tiles) {
-            ++block;
-            const int high = first_tile(share_begin(block + 1, total_cost, p.blocks), start, tiles);
-            if (high > done) join(block, p.next_out, p.next_stat, block * 2 * kRows + r);
-            done = high;
+            for (int d = 16; d; d >>= 1) higher = fmaxf(higher, __shfl_xor_sync(0xffffffffu, higher, d));
+            higher = fmaxf(higher, top);
+            const float before = top == -INFINITY ? 0.f : exp2_approx(top - higher);
+            const float weight = part.y != 0.f ? exp2_approx(part.x - higher) : 0.f;
+            top = higher;
+            float sum = weight * part.y;
+#pragma unroll
+            for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
+            total = total * before + sum;
+#pragma unroll
+            for (int i = 0; i < kPer; ++i) acc[i] *= before;
+            while (parts) {
+                float value[4][kPer], mine[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const int from = parts ? __ffs(parts) - 1 : 0;
+                    const float its = __shfl_sync(0xffffffffu, weight, from);
+                    const float* source = reinterpret_cast<const float*>(
+                        __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(values), from)) + lane * kPer;
+                    mine[u] = parts ? its : 0.f;
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i) value[u][i] = parts ? source[i] : 0.f;
+                    parts &= parts - 1;
+                }
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+#pragma unroll
+                    for (int i = 0; i < kPer; ++i) acc[i] = fmaf(value[u][i], mine[u], acc[i]);
+                }
+            }
         }
-    };
-    const int64_t head_row = n * p.group + g;
-    join_item(prefix_cost * (kv_head * p.prefix_row_tiles + head_row / (2 * kRows)), prefix_items ? p.prefix_tiles : 0,
-              p.prefix_out, p.prefix_stat, kv_head * p.head_rows + head_row, static_cast<int>(head_row % (2 * kRows)));
-    if (entry < entries_end) {
-        const int64_t cost = p.plan_cost[entry + 1] - p.plan_cost[entry];
-        join_item(prefix_total + static_cast<int64_t>(p.plan_cost[entry]) * p.kv_heads + kv_head * cost,
-                  cost ? static_cast<int>((cost - kItemCost) / kTileCost) : 0, p.own_out, p.own_stat, kv_head * p.head_rows + head_row,
-                  static_cast<int>(local % (2 * kRows)));
-    }
-    const float scale = bad ? NAN : (total == 0.f ? 0.f : 1.f / total);
-    T* o = static_cast<T*>(p.out) + n * p.o_token + head * p.o_head + lane * kPer;
+        bad = __any_sync(0xffffffffu, bad);
+        const float scale = bad ? NAN : (total == 0.f ? 0.f : 1.f / total);
+        T* o = static_cast<T*>(p.out) + n * p.o_token + head * p.o_head + lane * kPer;
 #pragma unroll
-    for (int i = 0; i < kPer; i += 2) {
-        *reinterpret_cast<uint32_t*>(o + i) = Kind<T>::pack(acc[i] * scale, acc[i + 1] * scale);
-    }
-    if (p.lse && lane == 0) {
-        p.lse[n * p.lse_token + head * p.lse_head] =
-            bad ? NAN : (total == 0.f ? -INFINITY : (top + log2f(total)) * 0.69314718055994531f);
+        for (int i = 0; i < kPer; i += 2) {
+            *reinterpret_cast<uint32_t*>(o + i) = Kind<T>::pack(acc[i] * scale, acc[i + 1] * scale);
+        }
+        if (p.lse && lane == 0) {
+            p.lse[n * p.lse_token + head * p.lse_head] =
+                bad ? NAN : (total == 0.f ? -INFINITY : (top + log2f(total)) * 0.69314718055994531f);
+        }
     }
 }
 
 // ---------------------------------------------------------------- host side
 
 struct Workspace {
-    int64_t prefix_out, own_out, next_out, prefix_stat, own_stat, next_stat, plan_cost, plan_first, failed, bytes;
+    int64_t prefix_out, own_out, next_out, prefix_stat, own_stat, next_stat, item_span, first_entry, next_item, failed, bytes;
 };
 
-Workspace workspace_of(int64_t tokens, int64_t batch, int64_t query_heads, int64_t dim, int64_t blocks) {
+Workspace workspace_of(int64_t tokens, int64_t batch, int64_t query_heads, int64_t kv_heads, int64_t dim, int64_t blocks) {
     Workspace w{};
     int64_t at = 0;
     const auto take = [&](int64_t bytes) {
@@ -915,25 +1135,31 @@ Workspace workspace_of(int64_t tokens, int64_t batch, int64_t query_heads, int64
     w.prefix_stat = take(rows * 8);
     w.own_stat = take(rows * 8);
     w.next_stat = take(next * 8);
-    w.plan_cost = take((kMaxEntries + 2) * 4);
-    w.plan_first = take((batch + 1) * 4);
+    const int64_t row_tiles = (rows / kv_heads + 2 * kRows - 1) / (2 * kRows);
+    w.item_span = take((row_tiles + kMaxEntries) * kv_heads * 4);
+    w.first_entry = take(batch * 4);
+    w.next_item = take(blocks * 4);
     w.failed = take(blocks * 4);
     w.bytes = at;
     return w;
 }
 
 template <typename T, int kDim>
-void launch(const AttentionParams& p, int device, cudaStream_t stream) {
+void launch(const AttentionParams& p, cudaStream_t stream) {
     using L = Layout<kDim>;
     static_assert(L::kBytes <= 232448, "shared memory of one block");
     cuda_check(cudaFuncSetAttribute(attention_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes),
                "attention shared memory");
     launch_dependent(attention_kernel<T, kDim>, dim3(static_cast<unsigned>(p.blocks)), dim3(kThreads), L::kBytes, stream,
                      "shared_prefix_attention launch", p);
-    const int64_t warps = p.tokens * p.kv_heads * p.group;
-    launch_dependent(combine_kernel<T, kDim>, dim3(static_cast<unsigned>((warps + 7) / 8)), dim3(256), 0, stream,
-                     "shared_prefix_attention join", p);
-    (void)device;
+    // One head a warp while they all fit the GPU at once, more behind that (a warp's start is most of its time).
+    const int64_t heads = static_cast<int64_t>(p.kv_heads) * p.group;
+    const int64_t at_once = static_cast<int64_t>(p.blocks) * 48;
+    int64_t per_warp = (p.tokens * heads + at_once - 1) / at_once;
+    if (per_warp > heads) per_warp = heads;
+    const int64_t warps = p.tokens * ((heads + per_warp - 1) / per_warp);
+    launch_dependent(combine_kernel<T, kDim>, dim3(static_cast<unsigned>((warps + kJoinWarps - 1) / kJoinWarps)),
+                     dim3(32 * kJoinWarps), 0, stream, "shared_prefix_attention join", p, static_cast<int>(per_warp));
 }
 
 void check_shape(int64_t tokens, int64_t batch, int query_heads, int kv_heads, int head_dim) {
@@ -957,7 +1183,7 @@ extern "C" int ekv_shared_prefix_workspace(int64_t tokens, int64_t batch, int qu
     return guarded([&] {
         require(bytes != nullptr, "null pointer argument");
         check_shape(tokens, batch, query_heads, kv_heads, head_dim);
-        *bytes = tokens && batch ? workspace_of(tokens, batch, query_heads, head_dim, sm_count(device)).bytes : 0;
+        *bytes = tokens && batch ? workspace_of(tokens, batch, query_heads, kv_heads, head_dim, sm_count(device)).bytes : 0;
     });
 }
 
@@ -1002,11 +1228,11 @@ extern "C" int ekv_shared_prefix_attention(
         // The plan's running cost of one head is held in 32 bits.
         const int64_t most_tiles = (table_width * page_size + kTile - 1) / kTile;
         const int64_t most_entries = batch + (head_rows + 2 * kRows - 1) / (2 * kRows);
-        require((most_tiles * kTileCost + kItemCost) <= static_cast<int64_t>(UINT32_MAX) / most_entries,
+        require((most_tiles * kBothTile + kBothStart) <= static_cast<int64_t>(UINT32_MAX) / most_entries,
                 "the block table is too wide for this batch");
         bind_device(device);
         const int blocks = sm_count(device);
-        const Workspace w = workspace_of(tokens, batch, query_heads, head_dim, blocks);
+        const Workspace w = workspace_of(tokens, batch, query_heads, kv_heads, head_dim, blocks);
         require(workspace != nullptr && workspace_bytes >= w.bytes, "workspace is too small");
         require(reinterpret_cast<uint64_t>(workspace) % 256 == 0, "workspace must be 256-byte aligned");
         AttentionParams p{};
@@ -1060,15 +1286,16 @@ extern "C" int ekv_shared_prefix_attention(
         p.prefix_stat = reinterpret_cast<float2*>(at + w.prefix_stat);
         p.own_stat = reinterpret_cast<float2*>(at + w.own_stat);
         p.next_stat = reinterpret_cast<float2*>(at + w.next_stat);
-        p.plan_cost = reinterpret_cast<uint32_t*>(at + w.plan_cost);
-        p.plan_first = reinterpret_cast<uint32_t*>(at + w.plan_first);
+        p.item_span = reinterpret_cast<uint32_t*>(at + w.item_span);
+        p.first_entry = reinterpret_cast<uint32_t*>(at + w.first_entry);
+        p.next_item = reinterpret_cast<int*>(at + w.next_item);
         p.failed = reinterpret_cast<uint32_t*>(at + w.failed);
         const auto cstream = static_cast<cudaStream_t>(stream);
         if (dtype == EKV_BF16) {
-            head_dim == 128 ? launch<__nv_bfloat16, 128>(p, device, cstream)
-                            : launch<__nv_bfloat16, 64>(p, device, cstream);
+            head_dim == 128 ? launch<__nv_bfloat16, 128>(p, cstream)
+                            : launch<__nv_bfloat16, 64>(p, cstream);
         } else {
-            head_dim == 128 ? launch<__half, 128>(p, device, cstream) : launch<__half, 64>(p, device, cstream);
+            head_dim == 128 ? launch<__half, 128>(p, cstream) : launch<__half, 64>(p, cstream);
         }
         check_launch("shared_prefix_attention launch");
     });

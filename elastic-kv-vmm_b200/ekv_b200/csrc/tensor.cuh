@@ -29,6 +29,17 @@ __device__ __forceinline__ bool barrier_try(uint32_t barrier, uint32_t parity) {
     return done != 0;
 }
 
+// As barrier_try, which may suspend the thread for a while, but returns at once.
+__device__ __forceinline__ bool barrier_test(uint32_t barrier, uint32_t parity) {
+    uint32_t done;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(done)
+        : "r"(barrier), "r"(parity)
+        : "memory");
+    return done != 0;
+}
+
 __device__ __forceinline__ uint64_t device_nanoseconds() {
     uint64_t t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
@@ -127,6 +138,11 @@ __device__ __forceinline__ void tensor_store16(uint32_t address, const uint32_t*
         : "memory");
 }
 
+// 32 bytes (a whole sector) to a 32-byte aligned address.
+__device__ __forceinline__ void store_sector(float* target, const uint32_t* r) {
+    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(target), EKV_I8(r, 0) : "memory");
+}
+
 // ---------------------------------------------------------------- matrix products
 
 // Instruction descriptor of a 16-bit product with 32-bit accumulation (M x N).
@@ -167,6 +183,13 @@ __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
+}
+
+// Largest of three.
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 // Two 32-bit operations in one instruction.
