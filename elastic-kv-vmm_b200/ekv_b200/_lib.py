@@ -18,7 +18,7 @@ MAX_PLANES = 256  # EKV_MAX_PLANES
 MAX_LAYERS = 128  # EKV_MAX_LAYERS
 SHARED_INLINE_MAX = 512  # EKV_SHARED_INLINE_MAX
 SHADOW_MAX_LAYERS = 128  # EKV_SHADOW_MAX_LAYERS
-ATTENTION_MAX_ROW_TILES = 2048  # EKV_ATTENTION_MAX_ROW_TILES
+ATTENTION_MAX_ROW_TILES = 1536  # EKV_ATTENTION_MAX_ROW_TILES
 
 _p = ct.c_void_p
 _i32 = ct.c_int

@@ -19,12 +19,13 @@
 //
 // attention_kernel, one tile: S = Q K^T and O += P V on the tensor cores (tcgen05, 128 rows x
 // 128 positions, 32-bit sums in tensor memory), a softmax thread per row between them.
-// Roles by warp: 0-3 and 4-7 softmax of row tile halves ("slots") 0 and 1; 8-15 gather the K and V rows
-// into swizzled shared memory (cp.async, 16 bytes a lane, whole rows; slots resolved through
-// the table, zeros for positions without one); 16 and 17 issue the products of slots 0 and 1 (one
-// thread each, so that the waits and commits of one fall beside the other's products); 18 walks the
-// block's items and hands them to the others through a small ring; 19 passes on what the gather
-// has written, with the fence between ordinary writes and the tensor cores' reads.
+// Roles by warp: 0-3 and 4-7 softmax of row tile halves ("slots") 0 and 1; 8-11 gather the K rows,
+// 12-15 the V rows into swizzled shared memory (cp.async, 16 bytes a lane, whole rows; slots
+// resolved through the table, zeros for positions without one; the queries are copied by the softmax
+// warps themselves, as soon as their last product with the ones before is complete); 16 and 17 issue the products of slots 0 and 1 (one
+// thread each, so that the waits and commits of one fall beside the other's products); 18 and 19 pass
+// on the V and K rows that have landed, with the fence between ordinary writes and the tensor cores'
+// reads; 18 also walks the block's items and hands them to the others through a small ring.
 // An item of more than 128 rows uses both
 // slots on the same K and V; a smaller one with many tiles gives its even tiles to one slot and
 // its odd ones to the other (kPair; the two join before they are written); with few tiles, items
@@ -37,6 +38,8 @@
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 namespace ekv {
 namespace {
 
@@ -45,7 +48,8 @@ constexpr int kTile = 128;           // positions of a tile
 // Eight warps gather: the copies one warp has in flight are few (four warps reached 12 bytes a cycle and
 // SM from HBM where eight reach 21).
 constexpr int kGatherWarps = 8;
-constexpr int kGatherRows = kTile / kGatherWarps;  // rows of a tile one gather warp copies
+constexpr int kGatherRows = 2 * kTile / kGatherWarps;  // rows of a K or V tile one gather warp copies
+static_assert(kGatherRows == 32, "a lane resolves one row");
 constexpr int kThreads = 256 + 32 * kGatherWarps + 128;
 // Registers a thread: 640 threads start with 96; the softmax warps take what the gather gives up.
 constexpr int kStartRegisters = 96, kSoftmaxRegisters = 128, kGatherRegisters = 64, kOtherRegisters = 96;
@@ -57,9 +61,14 @@ constexpr int kMaxEntries = EKV_ATTENTION_MAX_ROW_TILES;
 constexpr int kBothStart = 24, kBothTile = 6;
 constexpr int kSmallStart = 3, kSmallTile = 4;
 constexpr int kPairTiles = 4;        // tiles from which a small item uses both slots
+constexpr int kFewRows = 16;         // rows up to which rows_kernel takes a request
+constexpr int kFewTile = 64;         // its unit of work, positions
+constexpr int kFewStart = 2, kFewUnit = 1;
+constexpr int kFewWarps = 8;
+constexpr int kFewPrefix = 4096;     // longest prefix it takes: a part of it to a worker, joined one by one
 enum Mode { kSingle = 0, kBoth = 1, kPair = 2 };
-constexpr int kMaskRing = 8;         // more than the stages of any layout
-constexpr int kItemRing = 4;
+constexpr int kMaskRing = 16;
+constexpr int kItemRing = 8, kItemsAhead = 5;
 constexpr float kRaise = 8.f;
 
 struct AttentionParams {
@@ -93,6 +102,12 @@ struct AttentionParams {
     float2* next_stat;
     uint32_t* item_span;   // of each item the first block with a tile of it, and the last << 16
     uint32_t* first_entry; // [batch]: each request's first entry
+    int few_prefix, few_own, large;  // what rows_kernel does (the prefix; requests), whether attention_kernel runs
+    int few_rows, workers;     // most rows of an item of rows_kernel
+    float* few_out;      // [workers][few_rows][dim]: the part a worker continues
+    float2* few_stat;
+    uint32_t* few_span;  // as item_span, of rows_kernel's items and workers
+    int* few_next;       // [workers]
     int* next_item;      // [blocks]: the item of the part a block continues, or -1
     uint32_t* failed;    // [blocks]: a wait ran out
 };
@@ -140,15 +155,27 @@ __device__ __forceinline__ bool request_of(const AttentionParams& p, int64_t n, 
     return n >= r.begin && n < r.begin + r.fresh;
 }
 
-// Slot of position j of table row `row`, or -1 where there is none inside the planes.
-__device__ __forceinline__ int64_t slot_of(const AttentionParams& p, int64_t row, uint32_t j) {
-    if (row < 0 || row >= p.table_rows) return -1;
+// Where position j of table row `row` is looked up: the page is loaded at once and used later.
+struct Lookup {
+    int64_t page;     // -1: none
+    uint32_t offset;  // in the page
+};
+
+__device__ __forceinline__ Lookup look_up(const AttentionParams& p, int row, uint32_t j) {
+    Lookup found{-1, 0};
     const uint32_t index = p.page_log2 >= 0 ? j >> p.page_log2 : j / p.page_size;
-    if (index >= p.table_width) return -1;
-    const int64_t page = load_index(p.tables, p.table_es, row * p.table_stride + index);
-    if (page < 0 || page >= p.slots) return -1;
-    const int64_t slot = page * p.page_size + (j - index * p.page_size);
-    return slot < p.slots ? slot : -1;
+    if (row >= 0 && index < p.table_width) {
+        found.page = load_index(p.tables, p.table_es, row * p.table_stride + index);
+        found.offset = j - index * p.page_size;
+    }
+    return found;
+}
+
+// The slot, or -1 where there is none inside the planes.
+__device__ __forceinline__ int slot_of(const AttentionParams& p, const Lookup& found) {
+    if (found.page < 0 || found.page >= p.slots) return -1;
+    const int64_t slot = found.page * p.page_size + found.offset;
+    return slot < p.slots ? static_cast<int>(slot) : -1;
 }
 
 // ---------------------------------------------------------------- the list of items
@@ -160,7 +187,8 @@ struct Plan {
     int32_t end[kMaxEntries];        // positions the tile's last row sees
     uint16_t request[kMaxEntries];
     uint16_t row_tile[kMaxEntries];
-    uint8_t small[kMaxEntries];      // up to 128 rows
+    bool small[kMaxEntries];         // up to 128 rows
+    bool few[kMaxEntries];           // up to 16: not attention_kernel's
     int64_t scratch[kThreads / 32];
     uint32_t entries;
 };
@@ -223,6 +251,7 @@ __device__ __forceinline__ void build_plan(const AttentionParams& p, Plan& plan)
                 plan.row_tile[at + t] = static_cast<uint16_t>(t);
                 plan.end[at + t] = static_cast<int32_t>(seen);
                 plan.small[at + t] = r.fresh * p.group - t * 2 * kRows <= kRows;
+                plan.few[at + t] = r.fresh * p.group <= kFewRows;
             }
         }
         entries += total;
@@ -237,7 +266,8 @@ __device__ __forceinline__ void build_plan(const AttentionParams& p, Plan& plan)
         if (e < entries) {
             const int64_t end = plan.end[e] < reach ? plan.end[e] : reach;
             cost = item_cost(cost_of(plan.small[e] ? 1 : 2 * kRows), (end - p.shared + kTile - 1) / kTile);
-            if (end <= p.shared) cost = 0;
+            // rows_kernel takes requests of few rows.
+            if (end <= p.shared || plan.few[e]) cost = 0;
         }
         int64_t total;
         const uint32_t at = running + static_cast<uint32_t>(block_scan(cost, total, plan.scratch));
@@ -307,6 +337,20 @@ __device__ __forceinline__ void write_spans(const AttentionParams& p, const Plan
     }
 }
 
+// Last of `count` entries whose running cost is at most x.
+__device__ __forceinline__ uint32_t entry_at(const uint32_t* cost, uint32_t count, int64_t x) {
+    uint32_t low = 0, high = count;
+    while (high - low > 1) {
+        const uint32_t mid = (low + high) >> 1;
+        if (cost[mid] <= x) {
+            low = mid;
+        } else {
+            high = mid;
+        }
+    }
+    return low;
+}
+
 struct __align__(16) Item {
     int mode;       // Mode: how the slots share it
     int prefix;
@@ -344,20 +388,10 @@ __device__ __forceinline__ Walk begin_walk(const AttentionParams& p, const Plan&
     if (w.start < prefix_total) {
         w.index = static_cast<int>(w.start / w.prefix_cost);
     } else if (plan.entries) {
-        // Last entry that begins at or before the share's start.
         const int64_t x = w.start - prefix_total;
-        uint32_t low = 0, high = plan.entries;
-        while (high - low > 1) {
-            const uint32_t mid = (low + high) >> 1;
-            if (static_cast<int64_t>(plan.cost[mid]) * p.kv_heads <= x) {
-                low = mid;
-            } else {
-                high = mid;
-            }
-        }
-        w.entry = low;
-        const int64_t cost = plan.cost[low + 1] - plan.cost[low];
-        if (cost) w.head = static_cast<int>((x - static_cast<int64_t>(plan.cost[low]) * p.kv_heads) / cost);
+        w.entry = entry_at(plan.cost, plan.entries, x / p.kv_heads);
+        const int64_t cost = plan.cost[w.entry + 1] - plan.cost[w.entry];
+        if (cost) w.head = static_cast<int>((x - static_cast<int64_t>(plan.cost[w.entry]) * p.kv_heads) / cost);
     }
     return w;
 }
@@ -393,7 +427,10 @@ __device__ __forceinline__ bool next_item(const AttentionParams& p, const Plan& 
         const uint32_t e = w.entry;
         const int head = w.head;
         if (!cost || ++w.head >= p.kv_heads) {
-            ++w.entry;
+            // The next entry that costs anything.
+            const uint32_t done = plan.cost[w.entry + 1];
+            const uint32_t found = entry_at(plan.cost, plan.entries, done);
+            w.entry = found > w.entry && done < plan.cost[plan.entries] ? found : plan.entries;
             w.head = 0;
         }
         if (!cost) continue;
@@ -455,9 +492,9 @@ struct Layout {
     static constexpr uint32_t kMasks = kItems + kItemRing * sizeof(Item);
     static constexpr uint32_t kStats = kMasks + kMaskRing * 16;  // maximum and sum of each row, of both slots
     static constexpr uint32_t kBarriers = kStats + 2 * kRows * 8;
-    // Six of each stage, eight of each slot, two of each place in the item ring, eight for the
+    // Six of each stage, seven of each slot, two of each place in the item ring, eight for the
     // turns, one where the slots of a pair meet.
-    static constexpr int kBarrierCount = 6 * kStages + 8 * 2 + 2 * kItemRing + 8 + 1;
+    static constexpr int kBarrierCount = 6 * kStages + 7 * 2 + 2 * kItemRing + 8 + 1;
     static constexpr uint32_t kTail = kBarriers + kBarrierCount * 8;
     static constexpr uint32_t kBytes = kTail + 16;  // tensor-memory address, failed flag
 };
@@ -505,30 +542,28 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     const auto slot_barrier = [&](int which, int s) { return barriers + 8 * (6 * L::kStages + 2 * which + s); };
     const auto q_landed = [&](int s) { return slot_barrier(0, s); };
     const auto q_full = [&](int s) { return slot_barrier(1, s); };
-    const auto q_empty = [&](int s) { return slot_barrier(2, s); };
-    const auto s_full = [&](int s) { return slot_barrier(3, s); };
-    const auto p_full = [&](int s) { return slot_barrier(4, s); };
-    const auto o_full = [&](int s) { return slot_barrier(5, s); };
-    const auto p_half = [&](int s) { return slot_barrier(6, s); };
-    const auto item_full = [&](int i) { return barriers + 8 * (6 * L::kStages + 14 + i); };
-    const auto item_empty = [&](int i) { return barriers + 8 * (6 * L::kStages + 14 + kItemRing + i); };
+    const auto s_full = [&](int s) { return slot_barrier(2, s); };
+    const auto p_full = [&](int s) { return slot_barrier(3, s); };
+    const auto o_full = [&](int s) { return slot_barrier(4, s); };
+    const auto p_half = [&](int s) { return slot_barrier(5, s); };
+    const auto item_full = [&](int i) { return barriers + 8 * (6 * L::kStages + 12 + i); };
+    const auto item_empty = [&](int i) { return barriers + 8 * (6 * L::kStages + 12 + kItemRing + i); };
     const auto go = [&](int s, int w) { return barriers + 8 * (L::kBarrierCount - 11 + 4 * s + w); };
     const uint32_t meet = barriers + 8 * (L::kBarrierCount - 3);
     const auto drain = [&](int s) { return barriers + 8 * (L::kBarrierCount - 2 + s); };
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < L::kStages; ++s) {
-            barrier_init(k_landed(s), 32 * kGatherWarps);
+            barrier_init(k_landed(s), 16 * kGatherWarps);
             barrier_init(k_full(s), 1);
             barrier_init(k_empty(s), 2);  // both slots, or one of them and the warp that passes on
-            barrier_init(v_landed(s), 32 * kGatherWarps);
+            barrier_init(v_landed(s), 16 * kGatherWarps);
             barrier_init(v_full(s), 1);
             barrier_init(v_empty(s), 2);
         }
         for (int s = 0; s < 2; ++s) {
-            barrier_init(q_landed(s), 32 * kGatherWarps);
+            barrier_init(q_landed(s), kRows);
             barrier_init(q_full(s), 1);
-            barrier_init(q_empty(s), 1);
             barrier_init(s_full(s), 1);
             barrier_init(p_half(s), 4);
             barrier_init(p_full(s), 4);
@@ -548,11 +583,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     if (warp == kIssueWarp) tensor_alloc(base + L::kTail, 512);
     grid_dependency_wait();
     tensor_fence_before();
+    allow_dependents();  // rows_kernel needs nothing of this one: its blocks begin where this one's leave room
     build_plan(p, plan);  // ends with __syncthreads
     write_spans(p, plan);
     tensor_fence_after();
     const uint32_t tensor = *reinterpret_cast<volatile uint32_t*>(shared + L::kTail);
 
+    // A row of an operand is copied 16 bytes a lane, kAtOnce rows a step; its chunks are
+    // swizzled within their 128 bytes by the row's place in its eight.
+    constexpr int kLanes = kDim / 8, kAtOnce = 32 / kLanes;
+    const int chunk = lane % kLanes, sub = lane / kLanes;
+    const auto target = [&](uint32_t operand, int row) {
+        return operand + (chunk >> 3) * L::kBlock + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
+    };
     Item* items = reinterpret_cast<Item*>(shared + L::kItems);
     Item item;
     uint32_t item_uses = 0;
@@ -580,15 +623,56 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         uint32_t uses = 0, ends = 0, tiles_before = 0, turns = 0, meetings = 0;
         const int r = (warp & 3) * 32 + lane;
         float2* stats = reinterpret_cast<float2*>(shared + L::kStats);
-        while (next(false)) {
-            const bool both = item.mode == kBoth, pair = item.mode == kPair;
-            const uint32_t tiles = tiles_before;
-            tiles_before += static_cast<uint32_t>(item.high - item.low);
-            if (item.mode == kSingle) {
-                const int owner = turn;
-                turn ^= 1;
-                if (owner != slot) continue;
+        // The items this slot has a part in, one ahead: its queries are copied (each warp its 32 rows)
+        // once the products with the ones before are complete.  An item stays in the ring until it is done.
+        int ahead = -1;        // its place in the ring; -1: none
+        uint32_t ahead_tiles = 0;  // tiles of the block before it
+        const auto release = [&](int place) {
+            __syncwarp();
+            if (lane == 0) barrier_arrive(item_empty(place));
+        };
+        const auto prepare = [&]() {
+            ahead = -1;
+            while (true) {
+                const int place = item_uses % kItemRing;
+                if (!__all_sync(0xffffffffu, barrier_wait(item_full(place), (item_uses / kItemRing) & 1, failed))) return false;
+                ++item_uses;
+                const Item& its = items[place];
+                const int rows = its.rows, mode = its.mode;
+                if (!rows) return true;
+                ahead_tiles = tiles_before;
+                tiles_before += static_cast<uint32_t>(its.high - its.low);
+                if (mode == kSingle) {
+                    const int owner_slot = turn;
+                    turn ^= 1;
+                    if (owner_slot != slot) {
+                        release(place);
+                        continue;
+                    }
+                }
+                ahead = place;
+                const int first = (mode == kBoth ? slot * kRows : 0) + (warp & 3) * 32;
+                const int row = its.row, head = its.head * p.group, token = its.token;
+                const uint32_t operand = base + L::kQuery + slot * L::kOperand;
+#pragma unroll 1
+                for (int i = sub; i < 32 && first + i - sub < rows; i += kAtOnce) {
+                    if (first + i >= rows) break;
+                    const int local = row + first + i;
+                    const int at = local / p.group;
+                    copy16_async(target(operand, (warp & 3) * 32 + i),
+                                 static_cast<const char*>(p.query) + 16 * chunk +
+                                     2 * ((token + at) * p.q_token + (head + local - at * p.group) * p.q_head), 16);
+                }
+                copies_arrive(q_landed(slot));
+                return true;
             }
+        };
+        if (!prepare()) goto finish;
+        while (ahead >= 0) {
+            const int place = ahead;
+            const uint32_t tiles = ahead_tiles;
+            const Item& item = items[place];
+            const bool both = item.mode == kBoth, pair = item.mode == kPair;
             const int item_row = (both ? slot * kRows : 0) + r;
             int64_t seen;
             const bool present = row_sees(p, item, item_row, seen);
@@ -598,15 +682,17 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             const bool idle = (both ? slot * kRows : 0) + (warp & 3) * 32 >= item.rows;  // no row in this warp
             float top = -INFINITY;
             float2 total = make_float2(0.f, 0.f);
-            const int low = item.low + (pair ? slot : 0), step = pair ? 2 : 1;
-            for (int t = low; t < item.high; t += step) {
+            const int low = item.low + (pair ? slot : 0), high = item.high, step = pair ? 2 : 1;
+            const uint32_t mask_base = tiles - item.low;
+            for (int t = low; t < high; t += step) {
                 if (!__all_sync(0xffffffffu, barrier_wait(s_full(slot), uses & 1, failed))) goto finish;
                 ++uses;
                 tensor_fence_after();
+                if (t + step >= high && !prepare()) goto finish;
                 if (!idle) {
                     // Positions this row sees here: those that have a slot, up to its last.
                     const int left = limit - t * kTile;
-                    const uint4 there = masks[(tiles + (t - item.low)) % kMaskRing];
+                    const uint4 there = masks[(mask_base + t) % kMaskRing];
                     const bool whole = __all_sync(0xffffffffu, left >= kTile) &&
                                        (there.x & there.y & there.z & there.w) == 0xffffffffu;
                     if (!whole) {
@@ -652,11 +738,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                         tensor_load32(scores + (c ? 0 : 64), a);  // the second time the first columns again, for below
                         raise_to(b);
                     }
-                    const float high = fmaxf(fmaxf(highs[0], highs[1]), fmaxf(highs[2], highs[3])) * p.scale_log2;
-                    const bool raise = present && (high > top + kRaise || (top == -INFINITY && high > -INFINITY));
+                    const float most = fmaxf(fmaxf(highs[0], highs[1]), fmaxf(highs[2], highs[3])) * p.scale_log2;
+                    const bool raise = present && (most > top + kRaise || (top == -INFINITY && most > -INFINITY));
                     if (__any_sync(0xffffffffu, raise)) {
                         const float before = top;
-                        if (raise) top = high;
+                        if (raise) top = most;
                         const float factor = raise ? (before == -INFINITY ? 0.f : exp2_approx(before - top)) : 1.f;
                         total.x *= factor;
                         total.y *= factor;
@@ -790,55 +876,33 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 ++meetings;
                 tensor_fence_after();
             }
+            release(place);
         }
     } else if (warp < kIssueWarp) {
         // ------------------------------------------------------------ gather
         registers_shrink<kGatherRegisters>();
-        const int first_row = (warp - 8) * kGatherRows;  // of every operand
-        constexpr int kLanes = kDim / 8;        // lanes a row (16 bytes each)
-        constexpr int kAtOnce = 32 / kLanes;    // rows a step
-        const int chunk = lane % kLanes, sub = lane / kLanes;
+        const bool keys = warp < 8 + kGatherWarps / 2;
+        const int first_row = (warp - 8) % (kGatherWarps / 2) * kGatherRows;  // of every operand
         const char* query = static_cast<const char*>(p.query) + 16 * chunk;
-        uint32_t uses = 0, q_uses[2] = {0, 0};
-        // A row's 16-byte chunks are swizzled within its 128 bytes by the row's place in its eight.
-        const auto target = [&](uint32_t operand, int row) {
-            return operand + (chunk >> 3) * L::kBlock + row * 128 + (((chunk & 7) ^ (row & 7)) << 4);
-        };
-        // Plane slot of this lane's row (lanes 16-31 repeat 0-15) in tile t of the item.
+        const int64_t stride = 2 * (keys ? p.k_slot : p.v_slot);
+        uint32_t uses = 0;
+        // This lane's row in tile t of the item.
         const auto find = [&](int t) {
-            const int position = item.begin + t * kTile + first_row + static_cast<int>(lane % kGatherRows);
-            return position < item.end ? static_cast<int>(slot_of(p, item.table_row, static_cast<uint32_t>(position))) : -1;
+            const int position = item.begin + t * kTile + first_row + static_cast<int>(lane);
+            return look_up(p, position < item.end ? item.table_row : -1, static_cast<uint32_t>(position));
         };
         bool more = next(false);
-        int found = more ? find(item.low) : -1;
+        Lookup found{-1, 0};
+        if (more) found = find(item.low);
         while (more) {
-            // Queries of the slots the item uses: other rows for each, or the same ones.
-            for (int use = 0; use < (item.mode == kSingle ? 1 : 2); ++use) {
-                const int slot = item.mode == kSingle ? turn : use, half = item.mode == kBoth ? use : 0;
-                if (!__all_sync(0xffffffffu, barrier_wait(q_empty(slot), (q_uses[slot] & 1) ^ 1, failed))) goto finish;
-                ++q_uses[slot];
-                const uint32_t operand = base + L::kQuery + slot * L::kOperand;
-#pragma unroll 1
-                for (int i = 0; i < kGatherRows; i += kAtOnce) {
-                    const int r = first_row + i + sub;
-                    if (half * kRows + r < item.rows) {
-                        const int local = item.row + half * kRows + r;
-                        const int at = local / p.group;
-                        const int head = item.head * p.group + local - at * p.group;
-                        copy16_async(target(operand, r), query + 2 * ((item.token + at) * p.q_token + head * p.q_head), 16);
-                    }
-                }
-                copies_arrive(q_landed(slot));
-            }
-            if (item.mode == kSingle) turn ^= 1;
-            const char* keys = static_cast<const char*>(p.k_plane) + 2 * item.head * p.k_head + 16 * chunk;
-            const char* values = static_cast<const char*>(p.v_plane) + 2 * item.head * p.v_head + 16 * chunk;
+            const char* plane = (keys ? static_cast<const char*>(p.k_plane) + 2 * item.head * p.k_head
+                                      : static_cast<const char*>(p.v_plane) + 2 * item.head * p.v_head) + 16 * chunk;
             const int high = item.high;
             for (int t = item.low; t < high; ++t, ++uses) {
                 const int stage = uses % L::kStages;
                 const uint32_t parity = ((uses / L::kStages) & 1) ^ 1;
-                const int now = found;
-                // The next tile's slots are looked up while this one's rows are copied.
+                const int now = slot_of(p, found);
+                // The next tile's pages are on their way while this one's rows are copied.
                 if (t + 1 < high) {
                     found = find(t + 1);
                 } else {
@@ -846,29 +910,19 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                     if (more) found = find(item.low);
                 }
                 const uint32_t there = __ballot_sync(0xffffffffu, now >= 0);
-                if (!__all_sync(0xffffffffu, barrier_wait(k_empty(stage), parity, failed))) goto finish;
-                // The mask's place was tile n - kMaskRing's.  This warp has copied V of tile n - 1, so the second
-                // products, and with them the softmax, of all tiles up to n - 1 - kStages are complete.
-                if (lane == 0) reinterpret_cast<uint16_t*>(&masks[uses % kMaskRing])[warp - 8] = static_cast<uint16_t>(there);
-                uint32_t operand = base + L::kKeys + stage * L::kOperand;
-                const char* plane = keys;
-                int64_t stride = 2 * p.k_slot;
-#pragma unroll 1
-                for (int which = 0; which < 2; ++which) {
-#pragma unroll 4
-                    for (int i = 0; i < kGatherRows; i += kAtOnce) {
-                        const int slot = __shfl_sync(0xffffffffu, now, i + sub);
-                        copy16_async(target(operand, first_row + i + sub), slot >= 0 ? plane + slot * stride : query,
-                                     slot >= 0 ? 16 : 0);
-                    }
-                    if (which) break;
-                    copies_arrive(k_landed(stage));
-                    if (!__all_sync(0xffffffffu, barrier_wait(v_empty(stage), parity, failed))) goto finish;
-                    operand = base + L::kValues + stage * L::kOperand;
-                    plane = values;
-                    stride = 2 * p.v_slot;
+                if (!__all_sync(0xffffffffu, barrier_wait(keys ? k_empty(stage) : v_empty(stage), parity, failed))) goto finish;
+                // The first product of tile n - kStages is complete.  A slot's products wait for the softmax of
+                // its tile before, and items that leave the other slot alone have few tiles, so
+                // masks of tiles further back than kStages + kPairTiles are no longer read.
+                if (keys && lane == 0) reinterpret_cast<uint32_t*>(&masks[uses % kMaskRing])[warp - 8] = there;
+                const uint32_t operand = base + (keys ? L::kKeys : L::kValues) + stage * L::kOperand;
+#pragma unroll 8
+                for (int i = 0; i < kGatherRows; i += kAtOnce) {
+                    const int slot = __shfl_sync(0xffffffffu, now, i + sub);
+                    copy16_async(target(operand, first_row + i + sub), slot >= 0 ? plane + slot * stride : query,
+                                 slot >= 0 ? 16 : 0);
                 }
-                copies_arrive(v_landed(stage));
+                copies_arrive(keys ? k_landed(stage) : v_landed(stage));
             }
         }
     } else if (lane == 0) {
@@ -912,7 +966,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 if (!(fine = barrier_wait(k_full(use % L::kStages), parity(use), failed))) break;
                 tensor_fence_after();
                 first(use);
-                if (low + step >= high) mma_commit(q_empty(slot));
                 for (int t = low; t < high; t += step, use += step) {
                     const int stage = use % L::kStages;
                     const uint32_t next_use = use + step;
@@ -940,7 +993,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                             tensor_fence_after();
                         }
                         first(next_use);
-                        if (t + 2 * step >= high) mma_commit(q_empty(slot));
                     }
                     if (ready) mma_commit(v_empty(stage));
                 }
@@ -951,45 +1003,58 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             mma_commit(drain(slot));
             volatile uint32_t ran_out = 0;
             barrier_wait(drain(slot), 0, &ran_out);
-        } else if (warp == kIssueWarp + 2) {
-            // -------------------------------------------------------- the block's items
-            Walk walk = begin_walk(p, plan);
-            bool more = true;
-            while (more) {
-                more = next_item(p, plan, walk, item);
-                if (!item_uses) p.next_item[blockIdx.x] = more && !item.first ? item.id : -1;
-                if (!more) item.rows = 0;
-                item.mode = mode_of(item);
-                const int place = item_uses % kItemRing;
-                if (!barrier_wait(item_empty(place), ((item_uses / kItemRing) & 1) ^ 1, failed)) break;
-                items[place] = item;
-                barrier_arrive(item_full(place));
-                ++item_uses;
-            }
         } else {
-            // -------------------------------------------------------- what the gather has written
+            // -------------------------------------------------------- what the gather has written, and the items
+            const bool keys = warp == kIssueWarp + 3;
             uint32_t uses = 0, q_uses[2] = {0, 0};
-            bool fine = true;
             const auto pass_on = [&](uint32_t landed, uint32_t full, uint32_t parity) {
                 if (!barrier_wait(landed, parity, failed)) return false;
                 fence_async_shared();
                 barrier_arrive(full);
                 return true;
             };
-            while (fine && next(true)) {
-                for (int use = 0; fine && use < (item.mode == kSingle ? 1 : 2); ++use) {
-                    const int slot = item.mode == kSingle ? turn : use;
-                    fine = pass_on(q_landed(slot), q_full(slot), q_uses[slot] & 1);
-                    ++q_uses[slot];
-                }
-                if (item.mode == kSingle) turn ^= 1;
-                for (int t = item.low; fine && t < item.high; ++t, ++uses) {
+            const auto pass_tiles = [&](const Item& its) {
+                bool fine = true;
+                for (int t = its.low; fine && t < its.high; ++t, ++uses) {
                     const int stage = uses % L::kStages;
                     const uint32_t parity = (uses / L::kStages) & 1;
-                    fine = pass_on(k_landed(stage), k_full(stage), parity);
-                    if (fine && item.mode != kBoth) barrier_arrive(k_empty(stage));  // for the slot that has no use for it
-                    fine = fine && pass_on(v_landed(stage), v_full(stage), parity);
-                    if (fine && item.mode != kBoth) barrier_arrive(v_empty(stage));
+                    fine = keys ? pass_on(k_landed(stage), k_full(stage), parity)
+                                : pass_on(v_landed(stage), v_full(stage), parity);
+                    // For the slot that has no use for the tile.
+                    if (fine && its.mode != kBoth) barrier_arrive(keys ? k_empty(stage) : v_empty(stage));
+                }
+                return fine;
+            };
+            bool fine = true;
+            if (keys) {
+                while (fine && next(true)) {
+                    for (int use = 0; fine && use < (item.mode == kSingle ? 1 : 2); ++use) {
+                        const int slot = item.mode == kSingle ? turn : use;
+                        fine = pass_on(q_landed(slot), q_full(slot), q_uses[slot] & 1);
+                        ++q_uses[slot];
+                    }
+                    if (item.mode == kSingle) turn ^= 1;
+                    fine = fine && pass_tiles(item);
+                }
+            } else {
+                Walk walk = begin_walk(p, plan);
+                bool more = true;
+                for (uint32_t i = 0; fine; ++i) {
+                    while (fine && more && item_uses < i + kItemsAhead) {
+                        more = next_item(p, plan, walk, item);
+                        if (!item_uses) p.next_item[blockIdx.x] = more && !item.first ? item.id : -1;
+                        if (!more) item.rows = 0;
+                        item.mode = mode_of(item);
+                        const int place = item_uses % kItemRing;
+                        fine = barrier_wait(item_empty(place), ((item_uses / kItemRing) & 1) ^ 1, failed);
+                        if (!fine) break;
+                        items[place] = item;
+                        barrier_arrive(item_full(place));
+                        ++item_uses;
+                    }
+                    const Item its = items[i % kItemRing];
+                    if (!its.rows) break;
+                    fine = fine && pass_tiles(its);
                 }
             }
         }
@@ -997,7 +1062,6 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
 finish:
     copies_wait_all();
     __syncthreads();
-    allow_dependents();
     if (threadIdx.x == 0) p.failed[blockIdx.x] = *failed;
     if (warp == kIssueWarp) {
         __syncwarp();
@@ -1005,127 +1069,525 @@ finish:
     }
 }
 
+// ---------------------------------------------------------------- few rows
+
+template <int kDim>
+struct FewLayout {
+    static constexpr int kChunk = 2048 / kDim;             // positions a warp has in shared memory
+    static constexpr uint32_t kOperand = kChunk * kDim * 2;  // 4096 bytes of K, as many of V
+    static constexpr uint32_t kWarp = 2 * kOperand + kFewRows * kDim * 2;
+    static constexpr uint32_t kPlan = kFewWarps * kWarp;
+    static constexpr uint32_t kBytes = kPlan + (kMaxEntries + 2) * 4 + (kFewWarps + 1) * 8;
+};
+
+// Requests of up to 16 query rows (a decode step), and a short prefix of a small batch: too few rows to
+// fill a tensor-core tile, so HBM bounds them.  Work is cut as above, into equal shares of 64-position
+// units, but a share belongs to a WARP, which keeps to itself: it copies 16 or 32 positions of K and V at a
+// time into its own shared memory (the next keys while it weighs these, the next values while it
+// scores those) and multiplies them with mma.sync, positions by rows: S^T = K Q^T, O^T += V^T P^T,
+// so that up to 8 rows cost half of what 16 do.  Sixteen such warps an SM have about 128 KB on the way.
+template <typename T, int kDim>
+__global__ void __launch_bounds__(32 * kFewWarps, 2) rows_kernel(const __grid_constant__ AttentionParams p) {
+    using L = FewLayout<kDim>;
+    constexpr int kChunk = L::kChunk, kBlocks = kChunk / 16;  // blocks of 16 positions in a chunk
+    constexpr int kLanes = kDim / 8, kAtOnce = 32 / kLanes;
+    extern __shared__ __align__(1024) uint8_t shared[];
+    uint32_t* running = reinterpret_cast<uint32_t*>(shared + L::kPlan);  // running cost of one head, by group
+    int64_t* scratch = reinterpret_cast<int64_t*>(shared + L::kPlan + (kMaxEntries + 2) * 4);
+    const int warp = threadIdx.x >> 5, lane = static_cast<int>(lane_id());
+    if (!p.large) grid_dependency_wait();  // else attention_kernel, launched before, has waited
+    allow_dependents();
+    // Group 0 is the prefix where rows_kernel takes it, the others are the requests.
+    const int offset = p.few_prefix, groups = static_cast<int>(p.batch) + offset;
+    const int64_t reach = p.table_width * p.page_size;
+    const Cost cost_unit{kFewStart, kFewUnit};
+    uint32_t total32 = 0;
+    for (int first = 0; first < groups; first += 32 * kFewWarps) {
+        const int i = first + static_cast<int>(threadIdx.x);
+        int64_t units = 0;
+        if (i < groups) {
+            if (i < offset) {
+                units = (p.shared + kFewTile - 1) / kFewTile;
+            } else if (p.few_own) {
+                const Request r = request_at(p, i - offset);
+                const int64_t end = r.length < reach ? r.length : reach;
+                if (r.fresh > 0 && r.fresh * p.group <= kFewRows && end > p.shared) {
+                    units = (end - p.shared + kFewTile - 1) / kFewTile;
+                }
+            }
+        }
+        const uint32_t cost = item_cost(cost_unit, units);
+        // Exclusive scan of the costs of 256 groups.
+        int64_t sum = cost;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t up = __shfl_up_sync(0xffffffffu, sum, d);
+            if (lane >= d) sum += up;
+        }
+        __syncthreads();
+        if (lane == 31) scratch[warp] = sum;
+        __syncthreads();
+        int64_t before = 0, all = 0;
+        for (int w = 0; w < kFewWarps; ++w) {
+            if (w == warp) before = all;
+            all += scratch[w];
+        }
+        if (i < groups) running[i] = total32 + static_cast<uint32_t>(before + sum - cost);
+        total32 += static_cast<uint32_t>(all);
+    }
+    if (threadIdx.x == 0) running[groups] = total32;
+    __syncthreads();
+    const int64_t total = static_cast<int64_t>(total32) * p.kv_heads;
+    // Little work goes to as many warps as it has units, an SM after another, so that its parts lie close together.
+    const int workers = total < p.workers ? (total ? static_cast<int>(total) : 1) : p.workers;
+    // What combine_kernel reads of the items.
+    for (int i = blockIdx.x * 32 * kFewWarps + threadIdx.x; i < groups * p.kv_heads; i += gridDim.x * 32 * kFewWarps) {
+        const int group = i / p.kv_heads, head = i - group * p.kv_heads;
+        const uint32_t cost = running[group + 1] - running[group];
+        uint32_t span = 1;
+        if (cost) {
+            const int64_t start = static_cast<int64_t>(running[group]) * p.kv_heads + static_cast<int64_t>(head) * cost;
+            const int units = item_tiles(cost_unit, cost);
+            const int64_t last = start + (units > 1 ? kFewStart + static_cast<int64_t>(units - 1) * kFewUnit : 0);
+            span = static_cast<uint32_t>(owner(start, total, workers)) |
+                   static_cast<uint32_t>(owner(last, total, workers)) << 16;
+        }
+        p.few_span[i] = span;
+    }
+    const int worker = warp * gridDim.x + blockIdx.x;
+    const int64_t share = worker < workers ? share_begin(worker, total, workers) : 0;
+    const int64_t stop = worker < workers ? share_begin(worker + 1, total, workers) : 0;
+    const uint32_t keys = shared_address(shared) + warp * L::kWarp, values = keys + L::kOperand, queries = values + L::kOperand;
+    const int chunk16 = lane % kLanes, sub = lane / kLanes;
+    // Byte of 16-byte chunk c of a row: swizzled as in attention_kernel, rows of the head dimension.
+    const auto place = [](int row, int c) { return static_cast<uint32_t>(row * kDim * 2 + ((c ^ (row & 7)) << 4)); };
+    int continued = -1;
+    int group = 0, head = 0;
+    if (share < stop) {
+        group = static_cast<int>(entry_at(running, groups, share / p.kv_heads));
+        const int64_t cost = running[group + 1] - running[group];
+        if (cost) head = static_cast<int>((share - static_cast<int64_t>(running[group]) * p.kv_heads) / cost);
+    }
+    while (share < stop && group < groups) {
+        const uint32_t cost = running[group + 1] - running[group];
+        const int64_t start = static_cast<int64_t>(running[group]) * p.kv_heads + static_cast<int64_t>(head) * cost;
+        if (cost && start >= stop) break;
+        const int its_group = group, its_head = head;
+        if (!cost || ++head >= p.kv_heads) {
+            ++group;
+            head = 0;
+        }
+        if (!cost) continue;
+        const int units = item_tiles(cost_unit, cost);
+        const int low = first_tile(cost_unit, share, start, units), high = first_tile(cost_unit, stop, start, units);
+        if (low >= high) continue;
+        if (low) continued = its_group * p.kv_heads + its_head;
+        const bool prefix = its_group < offset;
+        const int64_t b = its_group - offset;
+        Request request{0, p.tokens, 0};
+        if (!prefix) request = request_at(p, b);
+        const int rows = static_cast<int>(request.fresh) * p.group;
+        int table_row;
+        if (prefix) {
+            table_row = static_cast<int>(p.source_row);
+        } else {
+            const int64_t at = p.rows ? load_index(p.rows, p.rows_es, b) : b;
+            table_row = at >= 0 && at < p.table_rows ? static_cast<int>(at) : -1;
+        }
+        const int end = prefix ? p.shared : static_cast<int>(request.length < reach ? request.length : reach);
+        const int begin = prefix ? 0 : p.shared;
+        const int from = begin + low * kFewTile, to = begin + high * kFewTile < end ? begin + high * kFewTile : end;
+        const char* k_plane = static_cast<const char*>(p.k_plane) + 2 * its_head * p.k_head + 16 * chunk16;
+        const char* v_plane = static_cast<const char*>(p.v_plane) + 2 * its_head * p.v_head + 16 * chunk16;
+        const auto find = [&](int position) {
+            const int mine = position + lane;
+            return look_up(p, lane < kChunk && mine < to ? table_row : -1, static_cast<uint32_t>(mine));
+        };
+        const auto copy = [&](uint32_t operand, const char* plane, int64_t stride, int slots) {
+#pragma unroll
+            for (int i = 0; i < kChunk; i += kAtOnce) {
+                const int slot = __shfl_sync(0xffffffffu, slots, i + sub);
+                copy16_async(operand + place(i + sub, chunk16), slot >= 0 ? plane + slot * stride : static_cast<const char*>(p.query),
+                             slot >= 0 ? 16 : 0);
+            }
+        };
+        // Queries and the first chunk.
+        for (int i = sub; i < rows; i += kAtOnce) {
+            const int token = i / p.group;
+            copy16_async(queries + place(i, chunk16),
+                         static_cast<const char*>(p.query) + 16 * chunk16 +
+                             2 * ((request.begin + token) * p.q_token + (its_head * p.group + i - token * p.group) * p.q_head), 16);
+        }
+        int slots = slot_of(p, find(from));
+        uint32_t there = __ballot_sync(0xffffffffu, slots >= 0);
+        copy(keys, k_plane, 2 * p.k_slot, slots);
+        copies_commit();
+        copy(values, v_plane, 2 * p.v_slot, slots);
+        copies_commit();
+        // Per row of this lane (two of each block of 8): positions it sees, maximum, sum, output.
+        const auto work = [&](auto row_blocks) {
+            constexpr int kRowBlocks = decltype(row_blocks)::value;
+            int sees[kRowBlocks][2];
+            float top[kRowBlocks][2], sum[kRowBlocks][2], out[kDim / 16][kRowBlocks][4];
+#pragma unroll
+            for (int n = 0; n < kRowBlocks; ++n) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int row = n * 8 + (lane & 3) * 2 + j, token = row / p.group;
+                    int64_t seen = 0;
+                    if (row < rows) {
+                        seen = request.length - request.fresh + token + 1;
+                        if (prefix) {
+                            int64_t its;
+                            Request r;
+                            seen = request_of(p, token, its, r) ? r.length - r.fresh + (token - r.begin) + 1 : 0;
+                        }
+                    }
+                    sees[n][j] = seen < 0 ? 0 : static_cast<int>(seen < INT32_MAX ? seen : INT32_MAX);
+                    top[n][j] = -INFINITY;
+                    sum[n][j] = 0.f;
+                }
+#pragma unroll
+                for (int d = 0; d < kDim / 16; ++d) out[d][n][0] = out[d][n][1] = out[d][n][2] = out[d][n][3] = 0.f;
+            }
+            const int block = lane >> 3, line = lane & 7;  // this lane's address in a load of four 8 x 8 blocks
+#pragma unroll 1
+            for (int position = from; position < to; position += kChunk) {
+                const bool more = position + kChunk < to;
+                Lookup next{-1, 0};
+                if (more) next = find(position + kChunk);
+                copies_wait<1>();  // the keys (and queries)
+                __syncwarp();
+                float score[kBlocks][kRowBlocks][4] = {};
+#pragma unroll
+                for (int k = 0; k < kDim / 16; k += 2) {
+                    uint32_t q[2][4];
+                    if (kRowBlocks == 1) {  // rows 0-7, four chunks of 8 dimensions: two steps
+                        load_blocks<false>(queries + place(line, 2 * k + block), q[0]);
+                    } else {  // rows 0-7 and 8-15, two chunks: a step each
+                        load_blocks<false>(queries + place((block >> 1) * 8 + line, 2 * k + (block & 1)), q[0]);
+                        load_blocks<false>(queries + place((block >> 1) * 8 + line, 2 * k + 2 + (block & 1)), q[1]);
+                    }
+#pragma unroll
+                    for (int step = 0; step < 2; ++step) {
+#pragma unroll
+                        for (int m = 0; m < kBlocks; ++m) {
+                            uint32_t a[4];
+                            load_blocks<false>(keys + place(m * 16 + (block & 1) * 8 + line, 2 * (k + step) + (block >> 1)), a);
+                            if (kRowBlocks == 1) {
+                                mma_warp<Kind<T>::kBf16>(score[m][0], a, q[0][2 * step], q[0][2 * step + 1]);
+                            } else {
+#pragma unroll
+                                for (int n = 0; n < kRowBlocks; ++n) {
+                                    mma_warp<Kind<T>::kBf16>(score[m][n], a, q[step][2 * n], q[step][2 * n + 1]);
+                                }
+                            }
+                        }
+                    }
+                }
+                __syncwarp();
+                const uint32_t seen_now = there;
+                if (more) {
+                    slots = slot_of(p, next);
+                    there = __ballot_sync(0xffffffffu, slots >= 0);
+                    copy(keys, k_plane, 2 * p.k_slot, slots);
+                }
+                copies_commit();
+                // A lane's scores: positions lane / 4 and lane / 4 + 8 of each block, two rows.
+                float most[kRowBlocks][2];
+                bool raise = false;
+#pragma unroll
+                for (int n = 0; n < kRowBlocks; ++n) {
+                    most[n][0] = most[n][1] = -INFINITY;
+#pragma unroll
+                    for (int m = 0; m < kBlocks; ++m) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const int at = m * 16 + (lane >> 2) + (i >> 1) * 8;
+                            const bool visible = (seen_now >> at & 1u) && position + at < sees[n][i & 1];
+                            score[m][n][i] = visible ? score[m][n][i] * p.scale_log2 : -INFINITY;
+                            most[n][i & 1] = fmaxf(most[n][i & 1], score[m][n][i]);
+                        }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+                        for (int d = 4; d < 32; d <<= 1) most[n][j] = fmaxf(most[n][j], __shfl_xor_sync(0xffffffffu, most[n][j], d));
+                        raise |= most[n][j] > top[n][j] + kRaise || (top[n][j] == -INFINITY && most[n][j] > -INFINITY);
+                    }
+                }
+                if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+                    for (int n = 0; n < kRowBlocks; ++n) {
+                        float factor[2];
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            const float higher = fmaxf(top[n][j], most[n][j]);
+                            factor[j] = top[n][j] == -INFINITY ? 0.f : exp2_approx(top[n][j] - higher);
+                            top[n][j] = higher;
+                            sum[n][j] *= factor[j];
+                        }
+#pragma unroll
+                        for (int d = 0; d < kDim / 16; ++d) {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) out[d][n][i] *= factor[i & 1];
+                        }
+                    }
+                }
+                uint32_t weights[kBlocks][kRowBlocks][2];
+#pragma unroll
+                for (int m = 0; m < kBlocks; ++m) {
+#pragma unroll
+                    for (int n = 0; n < kRowBlocks; ++n) {
+                        float w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const float base = top[n][i & 1] == -INFINITY ? 0.f : top[n][i & 1];
+                            w[i] = exp2_approx(score[m][n][i] - base);
+                            sum[n][i & 1] += w[i];
+                        }
+                        weights[m][n][0] = transpose_block(Kind<T>::pack(w[0], w[1]));
+                        weights[m][n][1] = transpose_block(Kind<T>::pack(w[2], w[3]));
+                    }
+                }
+                copies_wait<1>();  // the values
+                __syncwarp();
+#pragma unroll
+                for (int d = 0; d < kDim / 16; ++d) {
+#pragma unroll
+                    for (int m = 0; m < kBlocks; ++m) {
+                        uint32_t a[4];
+                        load_blocks<true>(values + place(m * 16 + (block >> 1) * 8 + line, 2 * d + (block & 1)), a);
+#pragma unroll
+                        for (int n = 0; n < kRowBlocks; ++n) {
+                            mma_warp<Kind<T>::kBf16>(out[d][n], a, weights[m][n][0], weights[m][n][1]);
+                        }
+                    }
+                }
+                __syncwarp();
+                if (more) copy(values, v_plane, 2 * p.v_slot, slots);
+                copies_commit();
+            }
+            float* partial = p.few_out + static_cast<int64_t>(worker) * p.few_rows * kDim;
+            float2* stat = p.few_stat + static_cast<int64_t>(worker) * p.few_rows;
+            if (low == 0) {
+                const int64_t row = static_cast<int64_t>(its_head) * p.head_rows + request.begin * p.group;
+                partial = (prefix ? p.prefix_out : p.own_out) + row * kDim;
+                stat = (prefix ? p.prefix_stat : p.own_stat) + row;
+            }
+#pragma unroll
+            for (int n = 0; n < kRowBlocks; ++n) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int row = n * 8 + (lane & 3) * 2 + j;
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) sum[n][j] += __shfl_xor_sync(0xffffffffu, sum[n][j], d);
+                    if (row >= rows) continue;
+                    float* target = partial + static_cast<int64_t>(row) * kDim + (lane >> 2);
+#pragma unroll
+                    for (int d = 0; d < kDim / 16; ++d) {
+                        target[16 * d] = out[d][n][j];
+                        target[16 * d + 8] = out[d][n][2 + j];
+                    }
+                    if (lane < 4) stat[row] = make_float2(top[n][j], sum[n][j]);
+                }
+            }
+        };
+        if (rows <= 8) {
+            work(std::integral_constant<int, 1>{});
+        } else {
+            work(std::integral_constant<int, 2>{});
+        }
+        copies_wait_all();
+        __syncwarp();
+    }
+    if (lane == 0) p.few_next[worker] = continued;
+    if (p.large) grid_dependency_wait();  // this grid completes after attention_kernel, so what follows it may read both
+}
+
 // ---------------------------------------------------------------- joining the parts
 
 constexpr int kJoinWarps = 4;
+constexpr int kJoinLanes = 8;  // of a row
 
-// A warp per token and `per_warp` query heads: the parts (m_i, l_i, O_i) of a row join as
-// sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i with m = max m_i.  The blocks that may hold a part of an
-// item lie next to each other: a lane looks at each, first those of the row's prefix item, then
-// those of its own, so that the loads of one row are all on their way together.
-template <typename T, int kDim>
-__global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_constant__ AttentionParams p, int per_warp) {
-    constexpr int kPer = kDim / 32;
+// Eight lanes a row: the parts (m_i, l_i, O_i) of a row join as
+// sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i with m = max m_i.  The blocks (or workers) that may hold a part
+// of an item lie next to each other: a lane looks at each, first those of the row's prefix item, then
+// those of its own.  Bound by instructions for many rows (eight lanes a row take a quarter of what a warp
+// a row takes: 8 x 8001 prompts 20 us against 42); by the latency of dependent loads for few, so
+// then the four eights of a warp (kSplit) share one row's parts and join at the end.
+template <typename T, int kDim, int kSplit>
+__global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_constant__ AttentionParams p) {
+    constexpr int kVectors = kDim / (4 * kJoinLanes);  // of four values, of a row, in a lane
+    constexpr int kAtOnce = kSplit == 1 ? 2 : 4;       // parts whose loads are on their way together
+    constexpr uint32_t kAll = 0xffffffffu;
     grid_dependency_wait();
     allow_dependents();
-    const int query_heads = p.kv_heads * p.group;
-    const int turns = (query_heads + per_warp - 1) / per_warp;
-    const int index = blockIdx.x * kJoinWarps + static_cast<int>(threadIdx.x >> 5);
-    const int n = index / turns;
-    const int first_head = (index - n * turns) * per_warp;
-    const int last_head = first_head + per_warp < query_heads ? first_head + per_warp : query_heads;
-    const int lane = static_cast<int>(lane_id());
+    const int lane = static_cast<int>(lane_id()) % kJoinLanes;
+    const int mine_of = static_cast<int>(threadIdx.x) / kJoinLanes % kSplit;
+    const int64_t index = (static_cast<int64_t>(blockIdx.x) * 32 * kJoinWarps + threadIdx.x) / (kJoinLanes * kSplit);
+    const int heads = p.kv_heads * p.group;
+    const int n = static_cast<int>(index / heads), head = static_cast<int>(index - static_cast<int64_t>(n) * heads);
+    const int kv_head = head / p.group, head_row = n * p.group + head - kv_head * p.group;
     int64_t b;
-    Request request;
-    if (!request_of(p, n, b, request)) return;
-    const int prefix_items = p.prefix_tiles ? p.prefix_row_tiles * p.kv_heads : 0;
-    const int first_entry = static_cast<int>(p.first_entry[b]);
-    const int begin = static_cast<int>(request.begin);
+    Request request{0, 0, 0};
+    const bool active = request_of(p, n, b, request);
+    int prefix_item = 0, own_item = 0, local = 0, prefix_first = 0, own_first = 0, prefix_count = 0, count = 0;
+    bool few = false;
+    if (active) {
+        const int prefix_items = p.prefix_tiles ? p.prefix_row_tiles * p.kv_heads : 0;
+        few = p.few_own && request.fresh * p.group <= kFewRows;
+        local = head_row - static_cast<int>(request.begin) * p.group;
+        uint32_t prefix_span = 1, own_span = 1;
+        if (p.few_prefix) {
+            prefix_item = kv_head;
+            prefix_span = p.few_span[prefix_item];
+        } else if (prefix_items) {
+            prefix_item = kv_head * p.prefix_row_tiles + head_row / (2 * kRows);
+            prefix_span = p.item_span[prefix_item];
+        }
+        if (few) {
+            own_item = (static_cast<int>(b) + p.few_prefix) * p.kv_heads + kv_head;
+            own_span = p.few_span[own_item];
+        } else if (p.large) {
+            const int entry = static_cast<int>(p.first_entry[b]) + local / (2 * kRows);
+            own_item = prefix_items + entry * p.kv_heads + kv_head;
+            if (entry < kMaxEntries) own_span = p.item_span[own_item];
+        }
+        prefix_first = static_cast<int>(prefix_span & 0xffff);
+        own_first = static_cast<int>(own_span & 0xffff);
+        prefix_count = static_cast<int>(prefix_span >> 16) - prefix_first + 1;
+        count = prefix_count + static_cast<int>(own_span >> 16) - own_first + 1;
+    }
+    float top = -INFINITY, total = 0.f;
+    float4 acc[kVectors];
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    uint32_t bad = 0;  // a wait ran out in a block whose part is needed
 #pragma unroll 1
-    for (int head = first_head; head < last_head; ++head) {
-        const int kv_head = head / p.group, g = head - kv_head * p.group;
-        const int head_row = n * p.group + g, local = head_row - begin * p.group;
-        const int64_t row = static_cast<int64_t>(kv_head) * p.head_rows + head_row;
-        const int prefix_item = kv_head * p.prefix_row_tiles + head_row / (2 * kRows);
-        const int entry = first_entry + local / (2 * kRows);
-        const int own_item = prefix_items + entry * p.kv_heads + kv_head;
-        const uint32_t prefix_span = prefix_items ? p.item_span[prefix_item] : 1;
-        const uint32_t own_span = entry < kMaxEntries ? p.item_span[own_item] : 1;
-        const int prefix_first = prefix_span & 0xffff, prefix_count = static_cast<int>(prefix_span >> 16) - prefix_first + 1;
-        const int own_first = own_span & 0xffff, own_count = static_cast<int>(own_span >> 16) - own_first + 1;
-        float top = -INFINITY, total = 0.f;
-        float acc[kPer] = {};
-        uint32_t bad = 0;  // a wait ran out in a block whose part is needed
+    for (int base = mine_of * kJoinLanes; __any_sync(kAll, base < count); base += kSplit * kJoinLanes) {
+        const int candidate = base + lane;
+        float2 part = make_float2(-INFINITY, 0.f);
+        uint32_t source = 0;  // all parts lie in one workspace: its row of kDim
+        if (candidate < count) {
+            const bool is_prefix = candidate < prefix_count;
+            const bool worker = is_prefix ? p.few_prefix : few;
+            const int place = is_prefix ? candidate : candidate - prefix_count;
+            const int block = (is_prefix ? prefix_first : own_first) + place;
+            const float2* stat;
+            const float* values;
+            int64_t row;
+            bool here = true;
+            if (place == 0) {
+                row = static_cast<int64_t>(kv_head) * p.head_rows + head_row;
+                stat = is_prefix ? p.prefix_stat : p.own_stat;
+                values = is_prefix ? p.prefix_out : p.own_out;
+            } else {
+                const int its_row = is_prefix ? head_row : local;
+                row = worker ? static_cast<int64_t>(block) * p.few_rows + its_row
+                             : static_cast<int64_t>(block) * 2 * kRows + its_row % (2 * kRows);
+                stat = worker ? p.few_stat : p.next_stat;
+                values = worker ? p.few_out : p.next_out;
+                here = (worker ? p.few_next : p.next_item)[block] == (is_prefix ? prefix_item : own_item);
+            }
+            const float2 its = stat[row];
+            if (here) part = its;
+            if (!worker) bad |= p.failed[block];
+            source = static_cast<uint32_t>((values - p.prefix_out) / kDim + row);
+        }
+        const bool counts = part.y != 0.f;  // a sum of 0: the row sees nothing there
+        float higher = counts ? part.x : -INFINITY;
+#pragma unroll
+        for (int d = 1; d < kJoinLanes; d <<= 1) higher = fmaxf(higher, __shfl_xor_sync(kAll, higher, d));
+        higher = fmaxf(higher, top);
+        const float before = top == -INFINITY ? 0.f : exp2_approx(top - higher);
+        const float weight = counts ? exp2_approx(part.x - higher) : 0.f;
+        float share = weight * part.y;
+#pragma unroll
+        for (int d = 1; d < kJoinLanes; d <<= 1) share += __shfl_xor_sync(kAll, share, d);
+        top = higher;
+        total = total * before + share;
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            acc[v] = make_float4(acc[v].x * before, acc[v].y * before, acc[v].z * before, acc[v].w * before);
+        }
 #pragma unroll 1
-        for (int base = 0; base < prefix_count + own_count; base += 32) {
-            int at = base + lane;
-            const bool is_prefix = at < prefix_count;
-            if (!is_prefix) at -= prefix_count;
-            const int block = (is_prefix ? prefix_first : own_first) + at;
-            float2 part = make_float2(-INFINITY, 0.f);
-            const float* values = p.next_out;
-            if (is_prefix || at < own_count) {
-                bad |= p.failed[block];
-                if (at == 0) {
-                    part = (is_prefix ? p.prefix_stat : p.own_stat)[row];
-                    values = (is_prefix ? p.prefix_out : p.own_out) + row * kDim;
-                } else if (p.next_item[block] == (is_prefix ? prefix_item : own_item)) {
-                    const int64_t next = static_cast<int64_t>(block) * 2 * kRows + (is_prefix ? head_row : local) % (2 * kRows);
-                    part = p.next_stat[next];
-                    values = p.next_out + next * kDim;
+        for (int u = 0; u < kJoinLanes && __any_sync(kAll, base + u < count); u += kAtOnce) {
+            float4 value[kAtOnce][kVectors];
+            float mine[kAtOnce];
+#pragma unroll
+            for (int i = 0; i < kAtOnce; ++i) {
+                mine[i] = __shfl_sync(kAll, weight, u + i, kJoinLanes);
+                const uint32_t its = __shfl_sync(kAll, source, u + i, kJoinLanes);
+                const float4* from = reinterpret_cast<const float4*>(p.prefix_out) + static_cast<int64_t>(its) * (kDim / 4) + lane;
+#pragma unroll
+                for (int v = 0; v < kVectors; ++v) {
+                    value[i][v] = mine[i] != 0.f ? from[v * kJoinLanes] : make_float4(0.f, 0.f, 0.f, 0.f);
                 }
             }
-            uint32_t parts = __ballot_sync(0xffffffffu, part.y != 0.f);  // 0: the row sees nothing there
-            if (!parts) continue;
-            float higher = part.y != 0.f ? part.x : -INFINITY;
 #pragma unroll
-            for (int d = 16; d; d >>= 1) higher = fmaxf(higher, __shfl_xor_sync(0xffffffffu, higher, d));
-            higher = fmaxf(higher, top);
-            const float before = top == -INFINITY ? 0.f : exp2_approx(top - higher);
-            const float weight = part.y != 0.f ? exp2_approx(part.x - higher) : 0.f;
-            top = higher;
-            float sum = weight * part.y;
+            for (int i = 0; i < kAtOnce; ++i) {
 #pragma unroll
-            for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, d);
-            total = total * before + sum;
-#pragma unroll
-            for (int i = 0; i < kPer; ++i) acc[i] *= before;
-            while (parts) {
-                float value[4][kPer], mine[4];
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const int from = parts ? __ffs(parts) - 1 : 0;
-                    const float its = __shfl_sync(0xffffffffu, weight, from);
-                    const float* source = reinterpret_cast<const float*>(
-                        __shfl_sync(0xffffffffu, reinterpret_cast<uint64_t>(values), from)) + lane * kPer;
-                    mine[u] = parts ? its : 0.f;
-#pragma unroll
-                    for (int i = 0; i < kPer; ++i) value[u][i] = parts ? source[i] : 0.f;
-                    parts &= parts - 1;
-                }
-#pragma unroll
-                for (int u = 0; u < 4; ++u) {
-#pragma unroll
-                    for (int i = 0; i < kPer; ++i) acc[i] = fmaf(value[u][i], mine[u], acc[i]);
+                for (int v = 0; v < kVectors; ++v) {
+                    acc[v].x = fmaf(value[i][v].x, mine[i], acc[v].x);
+                    acc[v].y = fmaf(value[i][v].y, mine[i], acc[v].y);
+                    acc[v].z = fmaf(value[i][v].z, mine[i], acc[v].z);
+                    acc[v].w = fmaf(value[i][v].w, mine[i], acc[v].w);
                 }
             }
         }
-        bad = __any_sync(0xffffffffu, bad);
-        const float scale = bad ? NAN : (total == 0.f ? 0.f : 1.f / total);
-        T* o = static_cast<T*>(p.out) + n * p.o_token + head * p.o_head + lane * kPer;
+    }
 #pragma unroll
-        for (int i = 0; i < kPer; i += 2) {
-            *reinterpret_cast<uint32_t*>(o + i) = Kind<T>::pack(acc[i] * scale, acc[i + 1] * scale);
+    for (int d = 1; d < kJoinLanes * kSplit; d <<= 1) bad |= __shfl_xor_sync(kAll, bad, d);
+    if (kSplit > 1) {
+        float higher = top;
+#pragma unroll
+        for (int d = kJoinLanes; d < 32; d <<= 1) higher = fmaxf(higher, __shfl_xor_sync(kAll, higher, d));
+        const float weight = top == -INFINITY ? 0.f : exp2_approx(top - higher);
+        top = higher;
+        total *= weight;
+#pragma unroll
+        for (int d = kJoinLanes; d < 32; d <<= 1) total += __shfl_xor_sync(kAll, total, d);
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            float* a = reinterpret_cast<float*>(&acc[v]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                a[i] *= weight;
+#pragma unroll
+                for (int d = kJoinLanes; d < 32; d <<= 1) a[i] += __shfl_xor_sync(kAll, a[i], d);
+            }
         }
-        if (p.lse && lane == 0) {
-            p.lse[n * p.lse_token + head * p.lse_head] =
-                bad ? NAN : (total == 0.f ? -INFINITY : (top + log2f(total)) * 0.69314718055994531f);
-        }
+    }
+    if (!active || mine_of) return;
+    const float scale = bad ? NAN : (total == 0.f ? 0.f : 1.f / total);
+    T* o = static_cast<T*>(p.out) + n * p.o_token + head * p.o_head + 4 * lane;
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v) {
+        *reinterpret_cast<uint2*>(o + v * 4 * kJoinLanes) = make_uint2(Kind<T>::pack(acc[v].x * scale, acc[v].y * scale),
+                                                                       Kind<T>::pack(acc[v].z * scale, acc[v].w * scale));
+    }
+    if (p.lse && lane == 0) {
+        p.lse[n * p.lse_token + head * p.lse_head] =
+            bad ? NAN : (total == 0.f ? -INFINITY : (top + log2f(total)) * 0.69314718055994531f);
     }
 }
 
 // ---------------------------------------------------------------- host side
 
 struct Workspace {
-    int64_t prefix_out, own_out, next_out, prefix_stat, own_stat, next_stat, item_span, first_entry, next_item, failed, bytes;
+    int64_t prefix_out, own_out, next_out, prefix_stat, own_stat, next_stat, item_span, first_entry, next_item, failed;
+    int64_t few_out, few_stat, few_span, few_next, bytes;
 };
+
+int64_t few_workers(int64_t blocks) { return blocks * 2 * kFewWarps; }
 
 Workspace workspace_of(int64_t tokens, int64_t batch, int64_t query_heads, int64_t kv_heads, int64_t dim, int64_t blocks) {
     Workspace w{};
     int64_t at = 0;
     const auto take = [&](int64_t bytes) {
         const int64_t here = at;
-        at += (bytes + 255) / 256 * 256;
+        at += (bytes + 511) / 512 * 512;  // whole rows of any head dimension
         return here;
     };
     const int64_t rows = tokens * query_heads, next = blocks * 2 * kRows;
@@ -1140,6 +1602,11 @@ Workspace workspace_of(int64_t tokens, int64_t batch, int64_t query_heads, int64
     w.first_entry = take(batch * 4);
     w.next_item = take(blocks * 4);
     w.failed = take(blocks * 4);
+    const int64_t workers = few_workers(blocks);
+    w.few_out = take(workers * kFewRows * dim * 4);
+    w.few_stat = take(workers * kFewRows * 8);
+    w.few_span = take((batch + 1) * kv_heads * 4);
+    w.few_next = take(workers * 4);
     w.bytes = at;
     return w;
 }
@@ -1150,16 +1617,24 @@ void launch(const AttentionParams& p, cudaStream_t stream) {
     static_assert(L::kBytes <= 232448, "shared memory of one block");
     cuda_check(cudaFuncSetAttribute(attention_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kBytes),
                "attention shared memory");
-    launch_dependent(attention_kernel<T, kDim>, dim3(static_cast<unsigned>(p.blocks)), dim3(kThreads), L::kBytes, stream,
-                     "shared_prefix_attention launch", p);
-    // One head a warp while they all fit the GPU at once, more behind that (a warp's start is most of its time).
-    const int64_t heads = static_cast<int64_t>(p.kv_heads) * p.group;
-    const int64_t at_once = static_cast<int64_t>(p.blocks) * 48;
-    int64_t per_warp = (p.tokens * heads + at_once - 1) / at_once;
-    if (per_warp > heads) per_warp = heads;
-    const int64_t warps = p.tokens * ((heads + per_warp - 1) / per_warp);
-    launch_dependent(combine_kernel<T, kDim>, dim3(static_cast<unsigned>((warps + kJoinWarps - 1) / kJoinWarps)),
-                     dim3(32 * kJoinWarps), 0, stream, "shared_prefix_attention join", p, static_cast<int>(per_warp));
+    if (p.large) {
+        launch_dependent(attention_kernel<T, kDim>, dim3(static_cast<unsigned>(p.blocks)), dim3(kThreads), L::kBytes, stream,
+                         "shared_prefix_attention launch", p);
+    }
+    if (p.few_prefix || p.few_own) {
+        constexpr uint32_t kFewBytes = FewLayout<kDim>::kBytes;
+        cuda_check(cudaFuncSetAttribute(rows_kernel<T, kDim>, cudaFuncAttributeMaxDynamicSharedMemorySize, kFewBytes),
+                   "attention shared memory");
+        launch_dependent(rows_kernel<T, kDim>, dim3(static_cast<unsigned>(p.workers / kFewWarps)), dim3(32 * kFewWarps),
+                         kFewBytes, stream, "shared_prefix_attention rows", p);
+    }
+    // A warp a row while all of them fit the GPU at once, a quarter of one behind that.
+    const int64_t rows = p.tokens * p.kv_heads * p.group;
+    const bool split = rows <= static_cast<int64_t>(p.blocks) * 48;
+    const int64_t threads = rows * kJoinLanes * (split ? 4 : 1);
+    launch_dependent(split ? combine_kernel<T, kDim, 4> : combine_kernel<T, kDim, 1>,
+                     dim3(static_cast<unsigned>((threads + 32 * kJoinWarps - 1) / (32 * kJoinWarps))), dim3(32 * kJoinWarps),
+                     0, stream, "shared_prefix_attention join", p);
 }
 
 void check_shape(int64_t tokens, int64_t batch, int query_heads, int kv_heads, int head_dim) {
@@ -1279,6 +1754,14 @@ extern "C" int ekv_shared_prefix_attention(
         p.prefix_row_tiles = static_cast<int>((head_rows + 2 * kRows - 1) / (2 * kRows));
         p.prefix_tiles = static_cast<int>((shared_tokens + kTile - 1) / kTile);
         p.blocks = blocks;
+        p.workers = static_cast<int>(few_workers(blocks));
+        p.few_own = group <= kFewRows;
+        p.few_rows = static_cast<int>(head_rows < kFewRows ? head_rows : kFewRows);
+        if (!query_starts && !(shared_tokens && head_rows <= kFewRows)) p.few_rows = group < kFewRows ? group : kFewRows;
+        p.few_prefix = shared_tokens > 0 && head_rows <= kFewRows && shared_tokens <= kFewPrefix;
+        if (p.few_prefix) p.prefix_tiles = 0;
+        // With one token a request, all of them have `group` rows.
+        p.large = p.prefix_tiles > 0 || (query_starts ? head_rows > kFewRows : !p.few_own);
         char* at = static_cast<char*>(workspace);
         p.prefix_out = reinterpret_cast<float*>(at + w.prefix_out);
         p.own_out = reinterpret_cast<float*>(at + w.own_out);
@@ -1289,6 +1772,10 @@ extern "C" int ekv_shared_prefix_attention(
         p.item_span = reinterpret_cast<uint32_t*>(at + w.item_span);
         p.first_entry = reinterpret_cast<uint32_t*>(at + w.first_entry);
         p.next_item = reinterpret_cast<int*>(at + w.next_item);
+        p.few_out = reinterpret_cast<float*>(at + w.few_out);
+        p.few_stat = reinterpret_cast<float2*>(at + w.few_stat);
+        p.few_span = reinterpret_cast<uint32_t*>(at + w.few_span);
+        p.few_next = reinterpret_cast<int*>(at + w.few_next);
         p.failed = reinterpret_cast<uint32_t*>(at + w.failed);
         const auto cstream = static_cast<cudaStream_t>(stream);
         if (dtype == EKV_BF16) {

@@ -138,7 +138,7 @@ def shared_prefix_attention(query: torch.Tensor, k_plane: torch.Tensor, v_plane:
     slot (a negative page, one outside the planes, past the table) is skipped.  A query token
     that sees no position gets zeros and a log-sum-exp of minus infinity.
 
-    One call takes up to ``ATTENTION_MAX_ROW_TILES`` (2048) row tiles: one per request and 256 query rows of a KV head.
+    One call takes up to ``ATTENTION_MAX_ROW_TILES`` (1536) row tiles: one per request and 256 query rows of a KV head.
     ``scale`` defaults to ``1 / sqrt(dim)``; ``lse`` is float32 [tokens, query_heads], the natural
     logarithm of the sum of the exponentials.  Scores, maxima, sums and outputs are held in 32 bits.
     """

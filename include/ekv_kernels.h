@@ -561,7 +561,7 @@ int ekv_append_rows(
  */
 #define EKV_BF16 0
 #define EKV_FP16 1
-#define EKV_ATTENTION_MAX_ROW_TILES 2048
+#define EKV_ATTENTION_MAX_ROW_TILES 1536
 int ekv_shared_prefix_workspace(
     int64_t tokens, int64_t batch, int query_heads, int kv_heads, int head_dim, int device, int64_t* bytes);
 int ekv_shared_prefix_attention(

@@ -113,7 +113,7 @@ def _attend():
     (dict(query_starts=torch.zeros(3, dtype=torch.int32)), ValueError, "4 entries"),
     (dict(lengths=torch.ones(2, dtype=torch.int32)), ValueError, "one query token"),
     (dict(query=torch.zeros(1 << 18, 4, 1, dtype=torch.bfloat16).expand(-1, -1, 64)), ValueError, "last dimension"),
-    (dict(lengths=torch.ones(2049, dtype=torch.int32), query=torch.zeros(2049, 4, 64, dtype=torch.bfloat16)), ValueError,
+    (dict(lengths=torch.ones(1537, dtype=torch.int32), query=torch.zeros(1537, 4, 64, dtype=torch.bfloat16)), ValueError,
      "one call takes"),
     (dict(scale=0.0), ValueError, "scale"),
     (dict(scale=float("nan")), ValueError, "scale"),
@@ -157,8 +157,8 @@ def _attention_args(**change):
     (dict(source=3), b"source row"), (dict(scale=-1.0), b"scale"), (dict(scale=float("nan")), b"scale"),
     (dict(batch=2), b"one query token"), (dict(query=None), b"null pointer"), (dict(query=4098), b"16-byte"),
     (dict(ks=(127, 64)), b"16-byte"), (dict(table_es=2), b"element size"),
-    (dict(tokens=2049, batch=2049), b"ROW_TILES"), (dict(tokens=1 << 20, starts=4096), b"ROW_TILES"),
-    (dict(width=1 << 30, page=1, tokens=2000, batch=2000), b"too wide"),
+    (dict(tokens=1537, batch=1537), b"ROW_TILES"), (dict(tokens=1 << 20, starts=4096), b"ROW_TILES"),
+    (dict(width=1 << 30, page=1, tokens=1500, batch=1500), b"too wide"),
 ])
 def test_c_entry_refuses_before_touching_a_device(change, message, library_path):
     from ekv_b200 import _lib
