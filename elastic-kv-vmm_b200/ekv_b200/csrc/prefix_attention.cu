@@ -885,6 +885,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         const int first_row = (warp - 8) % (kGatherWarps / 2) * kGatherRows;  // of every operand
         const char* query = static_cast<const char*>(p.query) + 16 * chunk;
         const int64_t stride = 2 * (keys ? p.k_slot : p.v_slot);
+        // Where this lane's copies of a stage go: the swizzle repeats every eight rows.
+        constexpr int kPlaces = 8 / kAtOnce;
+        uint32_t places[kPlaces];
+#pragma unroll
+        for (int i = 0; i < kPlaces; ++i) {
+            places[i] = target(base + (keys ? L::kKeys : L::kValues), first_row + i * kAtOnce + sub);
+        }
         uint32_t uses = 0;
         // This lane's row in tile t of the item.
         const auto find = [&](int t) {
@@ -915,12 +922,20 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 // its tile before, and items that leave the other slot alone have few tiles, so
                 // masks of tiles further back than kStages + kPairTiles are no longer read.
                 if (keys && lane == 0) reinterpret_cast<uint32_t*>(&masks[uses % kMaskRing])[warp - 8] = there;
-                const uint32_t operand = base + (keys ? L::kKeys : L::kValues) + stage * L::kOperand;
-#pragma unroll 8
-                for (int i = 0; i < kGatherRows; i += kAtOnce) {
-                    const int slot = __shfl_sync(0xffffffffu, now, i + sub);
-                    copy16_async(target(operand, first_row + i + sub), slot >= 0 ? plane + slot * stride : query,
-                                 slot >= 0 ? 16 : 0);
+                const uint32_t operand = stage * L::kOperand;
+                if (there == 0xffffffffu) {
+#pragma unroll
+                    for (int i = 0; i < kGatherRows; i += kAtOnce) {
+                        const int slot = __shfl_sync(0xffffffffu, now, i + sub);
+                        copy16_async(places[i / kAtOnce % kPlaces] + operand + (i / 8) * 1024, plane + slot * stride, 16);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int i = 0; i < kGatherRows; i += kAtOnce) {
+                        const int slot = __shfl_sync(0xffffffffu, now, i + sub);
+                        copy16_async(target(base + (keys ? L::kKeys : L::kValues) + operand, first_row + i + sub),
+                                     slot >= 0 ? plane + slot * stride : query, slot >= 0 ? 16 : 0);
+                    }
                 }
                 copies_arrive(keys ? k_landed(stage) : v_landed(stage));
             }

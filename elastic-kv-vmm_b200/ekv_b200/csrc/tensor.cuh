@@ -19,12 +19,15 @@ __device__ __forceinline__ void barrier_arrive(uint32_t barrier) {
     asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(barrier) : "memory");
 }
 
+// May suspend the thread until the phase is complete, for up to kSuspend nanoseconds.
+constexpr uint32_t kSuspend = 1000000;
+
 __device__ __forceinline__ bool barrier_try(uint32_t barrier, uint32_t parity) {
     uint32_t done;
     asm volatile(
-        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n selp.u32 %0, 1, 0, p;\n}"
         : "=r"(done)
-        : "r"(barrier), "r"(parity)
+        : "r"(barrier), "r"(parity), "r"(kSuspend)
         : "memory");
     return done != 0;
 }
@@ -56,7 +59,7 @@ __device__ __forceinline__ bool barrier_wait(uint32_t barrier, uint32_t parity, 
     uint64_t begin = 0;
 #pragma unroll 1
     while (!barrier_try(barrier, parity)) {
-        if (++tries & 255) continue;
+        if (++tries & 15) continue;
         const uint64_t now = device_nanoseconds();
         if (!begin) begin = now;
         if (*failed || now - begin > kWaitLimit) {
