@@ -292,7 +292,11 @@ def torch_binding():
                 ct.cast(lib.ekv_lookup_slots, ct.c_void_p).value,
                 ct.cast(lib.ekv_resolve_shared_blocks, ct.c_void_p).value,
                 ct.cast(lib.ekv_gather_rows, ct.c_void_p).value,
-                ct.cast(lib.ekv_gather_rows_planes, ct.c_void_p).value)
+                ct.cast(lib.ekv_gather_rows_planes, ct.c_void_p).value,
+                ct.cast(lib.ekv_extend_block_tables, ct.c_void_p).value,
+                ct.cast(lib.ekv_append_rows, ct.c_void_p).value,
+                ct.cast(lib.ekv_shared_prefix_workspace, ct.c_void_p).value,
+                ct.cast(lib.ekv_shared_prefix_attention, ct.c_void_p).value)
     return module
 
 

@@ -19,7 +19,7 @@ from typing import NamedTuple
 
 import torch
 
-from ._lib import MAX_PLANES, call, index_esize, require_cuda, stream_handle, u64_array
+from ._lib import MAX_PLANES, call, index_esize, last_error, require_cuda, stream_handle, torch_binding, u64_array
 
 _INT32_MAX = (1 << 31) - 1
 
@@ -74,6 +74,16 @@ def extend_block_tables(block_tables: torch.Tensor, lengths: torch.Tensor, new_t
     distinct rows.  ``out`` takes the tensors of an earlier result again; they must not
     overlap the inputs (copy ``out.lengths`` to the next step's lengths instead).
     """
+    fast = torch_binding() if out is None and type(page_size) is int and type(max_tokens) is int else None
+    if fast is not None:
+        try:
+            rc, *results = fast.extend_block_tables(block_tables, lengths, new_tokens, free_pages, page_size, max_tokens, rows)
+        except TypeError:  # not tensors: the checked path below reports it
+            rc = fast.NOT_HANDLED
+        if rc == 0:
+            return TableExtension(*results)
+        if rc == fast.KERNEL_ERROR:
+            raise last_error("ekv_extend_block_tables")
     if type(page_size) is not int or not 1 <= page_size <= _INT32_MAX:
         raise ValueError("page_size outside the supported range")
     if type(max_tokens) is not int or not 0 <= max_tokens <= _INT32_MAX:
@@ -139,6 +149,16 @@ def append_rows(rows, slot_map: torch.Tensor, planes) -> None:
     copied bit for bit.
     """
     rows, planes = list(rows), list(planes)
+    fast = torch_binding()
+    if fast is not None:
+        try:
+            rc = fast.append_rows(rows, slot_map, planes)
+        except TypeError:  # not tensors: the checked path below reports it
+            rc = fast.NOT_HANDLED
+        if rc == 0:
+            return
+        if rc == fast.KERNEL_ERROR:
+            raise last_error("ekv_append_rows")
     if len(rows) != len(planes):
         raise ValueError("rows and planes differ in length")
     if not planes:

@@ -66,6 +66,7 @@ constexpr int kFewTile = 64;         // its unit of work, positions
 constexpr int kFewStart = 2, kFewUnit = 1;
 constexpr int kFewWarps = 8;
 constexpr int kFewPrefix = 4096;     // longest prefix it takes: a part of it to a worker, joined one by one
+constexpr int kLargeTime = 37, kFewTime = 40, kLeastShare = 24;
 enum Mode { kSingle = 0, kBoth = 1, kPair = 2 };
 constexpr int kMaskRing = 16;
 constexpr int kItemRing = 8, kItemsAhead = 5;
@@ -191,6 +192,7 @@ struct Plan {
     bool few[kMaxEntries];           // up to 16: not attention_kernel's
     int64_t scratch[kThreads / 32];
     uint32_t entries;
+    int blocks;  // of the grid that have work, the first ones
 };
 
 struct Cost {
@@ -204,6 +206,29 @@ __device__ __forceinline__ uint32_t item_cost(Cost c, int64_t tiles) {
 }
 __device__ __forceinline__ int item_tiles(Cost c, uint32_t cost) {
     return cost ? static_cast<int>((cost - c.start) / c.tile) : 0;
+}
+
+// What rows_kernel takes of a request, and its cost of one head.
+__device__ __forceinline__ uint32_t few_cost(const AttentionParams& p, const Request& r) {
+    const int64_t reach = p.table_width * p.page_size, end = r.length < reach ? r.length : reach;
+    if (!p.few_own || r.fresh <= 0 || r.fresh * p.group > kFewRows || end <= p.shared) return 0;
+    return item_cost(Cost{kFewStart, kFewUnit}, (end - p.shared + kFewTile - 1) / kFewTile);
+}
+__device__ __forceinline__ uint32_t few_prefix_cost(const AttentionParams& p) {
+    return p.few_prefix ? item_cost(Cost{kFewStart, kFewUnit}, (p.shared + kFewTile - 1) / kFewTile) : 0;
+}
+
+// Blocks (an SM each) that attention_kernel uses when both kernels have work: the two share the SMs in
+// proportion to their estimated times there (a unit of its cost took 0.37 us, one of rows_kernel's 0.40 us), so
+// that the memory-bound part runs beside the compute-bound one.
+__device__ __forceinline__ int large_blocks(const AttentionParams& p, int64_t large, int64_t few) {
+    if (!few || !large) return p.blocks;
+    const int64_t mine = large * kLargeTime, its = few * kFewTime;
+    int64_t blocks = (mine * p.blocks + mine + its - 1) / (mine + its);
+    const int64_t most = (large + kLeastShare - 1) / kLeastShare;  // a few tiles a block at least
+    if (blocks > most) blocks = most;
+    if (blocks > p.blocks - 1) blocks = p.blocks - 1;
+    return blocks < 1 ? 1 : static_cast<int>(blocks);
 }
 
 // Index (in the request) of the last token of a row tile.
@@ -235,7 +260,7 @@ __device__ __forceinline__ int64_t block_scan(int64_t value, int64_t& total, int
 }
 
 __device__ __forceinline__ void build_plan(const AttentionParams& p, Plan& plan) {
-    int64_t entries = 0;
+    int64_t entries = 0, few = few_prefix_cost(p);
     for (int64_t first = 0; first < p.batch; first += kThreads) {
         const int64_t b = first + threadIdx.x;
         Request r{0, 0, 0};
@@ -243,6 +268,9 @@ __device__ __forceinline__ void build_plan(const AttentionParams& p, Plan& plan)
         const int64_t tiles = (r.fresh * p.group + 2 * kRows - 1) / (2 * kRows);
         int64_t total;
         const int64_t at = entries + block_scan(tiles, total, plan.scratch);
+        int64_t its;
+        block_scan(b < p.batch ? few_cost(p, r) : 0, its, plan.scratch);
+        few += its;
         if (b < p.batch) {
             if (blockIdx.x == 0) p.first_entry[b] = static_cast<uint32_t>(at < kMaxEntries ? at : kMaxEntries);
             for (int64_t t = 0; t < tiles && at + t < kMaxEntries; ++t) {
@@ -277,6 +305,9 @@ __device__ __forceinline__ void build_plan(const AttentionParams& p, Plan& plan)
     if (threadIdx.x == 0) {
         plan.cost[entries] = running;
         plan.entries = static_cast<uint32_t>(entries);
+        const int64_t prefix = p.prefix_tiles ? static_cast<int64_t>(item_cost(cost_of(p.head_rows), p.prefix_tiles)) *
+                                                    p.prefix_row_tiles * p.kv_heads : 0;
+        plan.blocks = large_blocks(p, prefix + static_cast<int64_t>(running) * p.kv_heads, few * p.kv_heads);
     }
     __syncthreads();
 }
@@ -316,7 +347,7 @@ __device__ __forceinline__ void write_spans(const AttentionParams& p, const Plan
     const int64_t prefix_total = static_cast<int64_t>(prefix_cost) * prefix_items;
     const int64_t total = prefix_total + static_cast<int64_t>(plan.cost[plan.entries]) * p.kv_heads;
     const int items = prefix_items + static_cast<int>(plan.entries) * p.kv_heads;
-    for (int i = blockIdx.x * kThreads + threadIdx.x; i < items; i += gridDim.x * kThreads) {
+    for (int i = blockIdx.x * kThreads + threadIdx.x; i < items; i += plan.blocks * kThreads) {
         Cost c = prefix;
         uint32_t cost = prefix_cost;
         int64_t start = static_cast<int64_t>(i) * prefix_cost;
@@ -330,8 +361,8 @@ __device__ __forceinline__ void write_spans(const AttentionParams& p, const Plan
         if (cost) {
             const int tiles = item_tiles(c, cost);
             const int64_t last = start + (tiles > 1 ? c.start + static_cast<int64_t>(tiles - 1) * c.tile : 0);
-            span = static_cast<uint32_t>(owner(start, total, p.blocks)) |
-                   static_cast<uint32_t>(owner(last, total, p.blocks)) << 16;
+            span = static_cast<uint32_t>(owner(start, total, plan.blocks)) |
+                   static_cast<uint32_t>(owner(last, total, plan.blocks)) << 16;
         }
         p.item_span[i] = span;
     }
@@ -380,8 +411,8 @@ __device__ __forceinline__ Walk begin_walk(const AttentionParams& p, const Plan&
     w.prefix_items = p.prefix_tiles ? p.prefix_row_tiles * p.kv_heads : 0;
     const int64_t prefix_total = static_cast<int64_t>(w.prefix_cost) * w.prefix_items;
     const int64_t total = prefix_total + static_cast<int64_t>(plan.cost[plan.entries]) * p.kv_heads;
-    w.start = share_begin(blockIdx.x, total, p.blocks);
-    w.stop = share_begin(blockIdx.x + 1, total, p.blocks);
+    w.start = share_begin(blockIdx.x, total, plan.blocks);
+    w.stop = share_begin(blockIdx.x + 1, total, plan.blocks);
     w.index = w.prefix_items;
     w.entry = 0;
     w.head = 0;
@@ -585,9 +616,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     tensor_fence_before();
     allow_dependents();  // rows_kernel needs nothing of this one: its blocks begin where this one's leave room
     build_plan(p, plan);  // ends with __syncthreads
-    write_spans(p, plan);
     tensor_fence_after();
     const uint32_t tensor = *reinterpret_cast<volatile uint32_t*>(shared + L::kTail);
+    if (static_cast<int>(blockIdx.x) >= plan.blocks) {  // rows_kernel's SM
+        if (warp == kIssueWarp) tensor_free(tensor, 512);
+        return;
+    }
+    write_spans(p, plan);
 
     // A row of an operand is copied 16 bytes a lane, kAtOnce rows a step; its chunks are
     // swizzled within their 128 bytes by the row's place in its eight.
@@ -1117,21 +1152,23 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) rows_kernel(const __grid_co
     const int64_t reach = p.table_width * p.page_size;
     const Cost cost_unit{kFewStart, kFewUnit};
     uint32_t total32 = 0;
+    int64_t large = 0;  // attention_kernel's cost, of one head
     for (int first = 0; first < groups; first += 32 * kFewWarps) {
         const int i = first + static_cast<int>(threadIdx.x);
-        int64_t units = 0;
-        if (i < groups) {
-            if (i < offset) {
-                units = (p.shared + kFewTile - 1) / kFewTile;
-            } else if (p.few_own) {
-                const Request r = request_at(p, i - offset);
-                const int64_t end = r.length < reach ? r.length : reach;
-                if (r.fresh > 0 && r.fresh * p.group <= kFewRows && end > p.shared) {
-                    units = (end - p.shared + kFewTile - 1) / kFewTile;
+        uint32_t cost = 0;
+        if (i < offset) {
+            cost = few_prefix_cost(p);
+        } else if (i < groups) {
+            const Request r = request_at(p, i - offset);
+            cost = few_cost(p, r);
+            if (p.large && r.fresh * p.group > kFewRows) {
+                for (int64_t t = 0; t * 2 * kRows < r.fresh * p.group; ++t) {
+                    const int64_t seen = r.length - r.fresh + last_token(t, r.fresh, p.group) + 1;
+                    const int64_t tiles = ((seen < reach ? seen : reach) - p.shared + kTile - 1) / kTile;
+                    large += item_cost(cost_of(r.fresh * p.group - t * 2 * kRows), tiles);
                 }
             }
         }
-        const uint32_t cost = item_cost(cost_unit, units);
         // Exclusive scan of the costs of 256 groups.
         int64_t sum = cost;
 #pragma unroll
@@ -1151,12 +1188,23 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) rows_kernel(const __grid_co
         total32 += static_cast<uint32_t>(all);
     }
     if (threadIdx.x == 0) running[groups] = total32;
+#pragma unroll
+    for (int d = 16; d; d >>= 1) large += __shfl_xor_sync(0xffffffffu, large, d);
     __syncthreads();
+    if (lane == 0) scratch[warp] = large;
+    __syncthreads();
+    large = 0;
+    for (int w = 0; w < kFewWarps; ++w) large += scratch[w];
+    if (p.prefix_tiles) large += static_cast<int64_t>(item_cost(cost_of(p.head_rows), p.prefix_tiles)) * p.prefix_row_tiles;
     const int64_t total = static_cast<int64_t>(total32) * p.kv_heads;
+    // The SMs that attention_kernel leaves take two blocks each.
+    int blocks = static_cast<int>(gridDim.x);
+    if (p.large && large && total) blocks = 2 * (p.blocks - large_blocks(p, large * p.kv_heads, total));
+    if (static_cast<int>(blockIdx.x) >= blocks) return;
     // Little work goes to as many warps as it has units, an SM after another, so that its parts lie close together.
-    const int workers = total < p.workers ? (total ? static_cast<int>(total) : 1) : p.workers;
+    const int workers = total < blocks * kFewWarps ? (total ? static_cast<int>(total) : 1) : blocks * kFewWarps;
     // What combine_kernel reads of the items.
-    for (int i = blockIdx.x * 32 * kFewWarps + threadIdx.x; i < groups * p.kv_heads; i += gridDim.x * 32 * kFewWarps) {
+    for (int i = blockIdx.x * 32 * kFewWarps + threadIdx.x; i < groups * p.kv_heads; i += blocks * 32 * kFewWarps) {
         const int group = i / p.kv_heads, head = i - group * p.kv_heads;
         const uint32_t cost = running[group + 1] - running[group];
         uint32_t span = 1;
@@ -1169,7 +1217,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) rows_kernel(const __grid_co
         }
         p.few_span[i] = span;
     }
-    const int worker = warp * gridDim.x + blockIdx.x;
+    const int worker = warp * blocks + blockIdx.x;
     const int64_t share = worker < workers ? share_begin(worker, total, workers) : 0;
     const int64_t stop = worker < workers ? share_begin(worker + 1, total, workers) : 0;
     const uint32_t keys = shared_address(shared) + warp * L::kWarp, values = keys + L::kOperand, queries = values + L::kOperand;
@@ -1416,7 +1464,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) rows_kernel(const __grid_co
         copies_wait_all();
         __syncwarp();
     }
-    if (lane == 0) p.few_next[worker] = continued;
+    if (lane == 0 && worker < workers) p.few_next[worker] = continued;
     if (p.large) grid_dependency_wait();  // this grid completes after attention_kernel, so what follows it may read both
 }
 

@@ -1,8 +1,9 @@
 // Compiled Python binding of the per-call residency lookups and gathers (optional).
 //
-// resolve_resident, lookup_slots, the batched shared-prefix resolver and
-// gather_rows / gather_rows_planes are called once per layer per decode step
-// through the reference's Python API.  Through ctypes a call costs ~10 us of
+// resolve_resident, lookup_slots, the batched shared-prefix resolver,
+// gather_rows / gather_rows_planes, append_rows and shared_prefix_attention are
+// called once per layer per decode step (extend_block_tables once per step)
+// through the Python API.  Through ctypes a call costs ~10 us of
 // host time (reading ~30 tensor attributes in Python and marshalling ~28
 // arguments); here the tensors arrive as at::Tensor and their pointers,
 // strides and the current stream are read in C++.  The kernels are reached
@@ -17,6 +18,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <algorithm>
+#include <cmath>
 #include <cstdint>
 #include <limits>
 #include <optional>
@@ -34,13 +36,22 @@ decltype(&ekv_lookup_slots) g_lookup = nullptr;
 decltype(&ekv_resolve_shared_blocks) g_shared = nullptr;
 decltype(&ekv_gather_rows) g_gather = nullptr;
 decltype(&ekv_gather_rows_planes) g_gather_planes = nullptr;
+decltype(&ekv_extend_block_tables) g_extend = nullptr;
+decltype(&ekv_append_rows) g_append = nullptr;
+decltype(&ekv_shared_prefix_workspace) g_workspace = nullptr;
+decltype(&ekv_shared_prefix_attention) g_attention = nullptr;
 
-void bind(int64_t resolve, int64_t lookup, int64_t shared, int64_t gather, int64_t gather_planes) {
+void bind(int64_t resolve, int64_t lookup, int64_t shared, int64_t gather, int64_t gather_planes, int64_t extend,
+          int64_t append, int64_t workspace, int64_t attention) {
     g_resolve = reinterpret_cast<decltype(&ekv_resolve_resident)>(resolve);
     g_lookup = reinterpret_cast<decltype(&ekv_lookup_slots)>(lookup);
     g_shared = reinterpret_cast<decltype(&ekv_resolve_shared_blocks)>(shared);
     g_gather = reinterpret_cast<decltype(&ekv_gather_rows)>(gather);
     g_gather_planes = reinterpret_cast<decltype(&ekv_gather_rows_planes)>(gather_planes);
+    g_extend = reinterpret_cast<decltype(&ekv_extend_block_tables)>(extend);
+    g_append = reinterpret_cast<decltype(&ekv_append_rows)>(append);
+    g_workspace = reinterpret_cast<decltype(&ekv_shared_prefix_workspace)>(workspace);
+    g_attention = reinterpret_cast<decltype(&ekv_shared_prefix_attention)>(attention);
 }
 
 int index_size(const at::Tensor& t) {
@@ -322,6 +333,168 @@ int gather_rows_planes(const std::vector<at::Tensor>& planes, const std::vector<
     return 0;
 }
 
+// ---------------------------------------------------------------- a serving step
+
+const at::Tensor* optional_tensor(const std::optional<at::Tensor>& t) { return t ? &*t : nullptr; }
+
+// Element size of a contiguous one-dimensional index tensor with `count` entries (-1: any), or 0.
+int vector_size(const at::Tensor& t, int64_t count) {
+    if (t.dim() != 1 || (t.numel() > 1 && t.stride(0) != 1) || (count >= 0 && t.size(0) != count)) return 0;
+    return index_size(t);
+}
+
+constexpr int64_t kInt32Max = std::numeric_limits<int32_t>::max();
+
+// (status, query_starts, slot_map, positions, lengths, pages_used): fresh outputs.
+py::tuple extend_block_tables(const at::Tensor& tables, const at::Tensor& lengths, const at::Tensor& fresh,
+                              const at::Tensor& free_pages, int64_t page_size, int64_t max_tokens,
+                              const std::optional<at::Tensor>& rows) {
+    auto status = [](int rc) { return py::make_tuple(rc, py::none(), py::none(), py::none(), py::none(), py::none()); };
+    if (!g_extend || page_size < 1 || page_size > kInt32Max || max_tokens < 0 || max_tokens > kInt32Max) {
+        return status(kNotHandled);
+    }
+    const int device = common_device({&tables, &lengths, &fresh, &free_pages, optional_tensor(rows)});
+    if (device < 0 || tables.scalar_type() != at::kInt || free_pages.scalar_type() != at::kInt || tables.dim() != 2 ||
+        (tables.size(1) > 1 && tables.stride(1) != 1) || (tables.size(0) > 1 && tables.stride(0) < tables.size(1)) ||
+        tables.size(1) > kInt32Max / page_size || lengths.dim() != 1) {
+        return status(kNotHandled);
+    }
+    const int64_t batch = lengths.size(0);
+    const int len_es = vector_size(lengths, batch), fresh_es = vector_size(fresh, batch);
+    const int rows_es = rows ? vector_size(*rows, batch) : 8;
+    if (!len_es || !fresh_es || !rows_es || !vector_size(free_pages, -1)) return status(kNotHandled);
+    const at::Tensor flat = at::empty({2 * batch + 2 * max_tokens + 2}, tables.options());
+    at::Tensor starts = flat.narrow(0, 0, batch + 1), slots = flat.narrow(0, batch + 1, max_tokens);
+    at::Tensor positions = flat.narrow(0, batch + 1 + max_tokens, max_tokens);
+    at::Tensor after = flat.narrow(0, batch + 1 + 2 * max_tokens, batch);
+    at::Tensor used = flat.narrow(0, 2 * batch + 1 + 2 * max_tokens, 1);
+    const int rc = g_extend(
+        tables.data_ptr<int32_t>(), tables.size(0), tables.size(1), tables.stride(0),
+        rows ? rows->data_ptr() : nullptr, rows_es, lengths.data_ptr(), len_es, fresh.data_ptr(), fresh_es, batch,
+        free_pages.data_ptr<int32_t>(), free_pages.size(0), page_size, max_tokens, starts.data_ptr<int32_t>(),
+        slots.data_ptr<int32_t>(), positions.data_ptr<int32_t>(), after.data_ptr<int32_t>(), used.data_ptr<int32_t>(),
+        device, stream_of(device));
+    if (rc != 0) return status(kKernelError);
+    return py::make_tuple(0, starts, slots, positions, after, used);
+}
+
+// Elements between the rows of [count, ...] when each row is contiguous, or -1; `elements` of one row.
+int64_t row_stride(const at::Tensor& t, int64_t& elements) {
+    elements = 1;
+    for (int64_t d = t.dim() - 1; d > 0; --d) {
+        if (t.size(d) != 1 && t.stride(d) != elements) return -1;
+        elements *= t.size(d);
+    }
+    return t.size(0) > 1 ? t.stride(0) : elements;
+}
+
+int append_rows(const std::vector<at::Tensor>& rows, const at::Tensor& slot_map, const std::vector<at::Tensor>& planes) {
+    if (!g_append || rows.size() != planes.size() || planes.size() > EKV_MAX_PLANES || planes.empty()) return kNotHandled;
+    const int map_es = vector_size(slot_map, -1);
+    if (!map_es || !slot_map.is_cuda()) return kNotHandled;
+    const int device = slot_map.get_device();
+    const int64_t tokens = slot_map.size(0);
+    uint64_t src[EKV_MAX_PLANES], dst[EKV_MAX_PLANES];
+    int64_t elements = 0, src_stride = 0, dst_stride = 0;
+    const at::ScalarType dtype = planes[0].scalar_type();
+    for (size_t i = 0; i < planes.size(); ++i) {
+        const at::Tensor& row = rows[i];
+        const at::Tensor& plane = planes[i];
+        if (common_device({&row, &plane}) != device || row.dim() < 2 || row.size(0) != tokens ||
+            row.sizes().slice(1) != plane.sizes().slice(1) || row.scalar_type() != dtype || plane.scalar_type() != dtype ||
+            row.sizes() != rows[0].sizes() || plane.sizes() != planes[0].sizes()) {
+            return kNotHandled;
+        }
+        int64_t of_row, of_plane;
+        const int64_t from = row_stride(row, of_row), to = row_stride(plane, of_plane);
+        if (from < 0 || to < of_plane || (i && (from != src_stride || to != dst_stride))) return kNotHandled;
+        elements = of_row;
+        src_stride = from;
+        dst_stride = to;
+        src[i] = reinterpret_cast<uint64_t>(row.data_ptr());
+        dst[i] = reinterpret_cast<uint64_t>(plane.data_ptr());
+    }
+    if (!tokens || !planes[0].size(0) || !elements) return 0;
+    const int64_t itemsize = planes[0].element_size();
+    const int rc = g_append(src, dst, static_cast<int>(planes.size()), elements * itemsize, src_stride * itemsize,
+                            dst_stride * itemsize, slot_map.data_ptr(), map_es, tokens, planes[0].size(0), device,
+                            stream_of(device));
+    return rc == 0 ? 0 : kKernelError;
+}
+
+// [count, heads, dim] with contiguous, 16-byte aligned rows of 16-bit values; `apart`: that do not overlap.
+bool head_rows_ok(const at::Tensor& t, bool apart) {
+    if (t.stride(2) != 1 || reinterpret_cast<uint64_t>(t.data_ptr()) % 16) return false;
+    for (int d = 0; d < 2; ++d) {
+        if (t.size(d) > 1 && (t.stride(d) % 8 || (apart && t.stride(d) < t.size(2)))) return false;
+    }
+    return true;
+}
+
+int64_t stride_of(const at::Tensor& t, int d) { return t.size(d) > 1 ? t.stride(d) : 0; }
+
+// (status, out, lse or None)
+py::tuple shared_prefix_attention(const at::Tensor& query, const at::Tensor& k_plane, const at::Tensor& v_plane,
+                                  const at::Tensor& tables, const at::Tensor& lengths, int64_t page_size,
+                                  int64_t shared_tokens, int64_t source_row, const std::optional<at::Tensor>& rows,
+                                  const std::optional<at::Tensor>& starts, std::optional<double> scale,
+                                  std::optional<at::Tensor> out, std::optional<at::Tensor> lse, bool want_lse) {
+    auto status = [](int rc) { return py::make_tuple(rc, py::none(), py::none()); };
+    const int device = common_device({&query, &k_plane, &v_plane, &tables, &lengths, optional_tensor(rows),
+                                      optional_tensor(starts), optional_tensor(out), optional_tensor(lse)});
+    if (!g_attention || device < 0 || query.dim() != 3 || k_plane.dim() != 3 || v_plane.sizes() != k_plane.sizes()) {
+        return status(kNotHandled);
+    }
+    const at::ScalarType dtype = query.scalar_type();
+    const int64_t tokens = query.size(0), heads = query.size(1), dim = query.size(2);
+    const int64_t slots = k_plane.size(0), kv_heads = k_plane.size(1);
+    if ((dtype != at::kBFloat16 && dtype != at::kHalf) || k_plane.scalar_type() != dtype || v_plane.scalar_type() != dtype ||
+        (dim != 64 && dim != 128) || k_plane.size(2) != dim || !kv_heads || !heads || heads % kv_heads) {
+        return status(kNotHandled);
+    }
+    if (out && (out->scalar_type() != dtype || out->sizes() != query.sizes())) return status(kNotHandled);
+    if (!head_rows_ok(query, false) || !head_rows_ok(k_plane, true) || !head_rows_ok(v_plane, true) ||
+        (out && !head_rows_ok(*out, true))) {
+        return status(kNotHandled);
+    }
+    if (lse && (lse->scalar_type() != at::kFloat || lse->dim() != 2 || lse->size(0) != tokens || lse->size(1) != heads)) {
+        return status(kNotHandled);
+    }
+    if (page_size < 1 || page_size > kInt32Max || tables.dim() != 2 || (tables.size(1) > 1 && tables.stride(1) != 1) ||
+        !index_size(tables) || tables.size(1) > kInt32Max / page_size || shared_tokens < 0 ||
+        shared_tokens > tables.size(1) * page_size ||
+        (shared_tokens && (source_row < 0 || source_row >= tables.size(0))) || lengths.dim() != 1) {
+        return status(kNotHandled);
+    }
+    const int64_t batch = lengths.size(0);
+    const int len_es = vector_size(lengths, batch), rows_es = rows ? vector_size(*rows, batch) : 8;
+    const int starts_es = starts ? vector_size(*starts, batch + 1) : 8;
+    if (!len_es || !rows_es || !starts_es || (!starts && tokens != batch) || tokens * heads > kInt32Max ||
+        batch + (tokens * heads / kv_heads + 255) / 256 > EKV_ATTENTION_MAX_ROW_TILES) {
+        return status(kNotHandled);
+    }
+    const double factor = scale ? *scale : 1.0 / std::sqrt(static_cast<double>(dim));
+    if (!(factor > 0.0 && factor < 3.0e38)) return status(kNotHandled);
+    if (!out) out = at::empty(query.sizes(), query.options());
+    if (!lse && want_lse) lse = at::empty({tokens, heads}, query.options().dtype(at::kFloat));
+    int64_t bytes = 0;
+    if (g_workspace(tokens, batch, static_cast<int>(heads), static_cast<int>(kv_heads), static_cast<int>(dim), device, &bytes)) {
+        return status(kKernelError);
+    }
+    const at::Tensor workspace = at::empty({bytes}, query.options().dtype(at::kByte));
+    const int rc = g_attention(
+        query.data_ptr(), stride_of(query, 0), stride_of(query, 1), k_plane.data_ptr(), stride_of(k_plane, 0),
+        stride_of(k_plane, 1), v_plane.data_ptr(), stride_of(v_plane, 0), stride_of(v_plane, 1), slots,
+        dtype == at::kBFloat16 ? EKV_BF16 : EKV_FP16, static_cast<int>(dim), static_cast<int>(heads),
+        static_cast<int>(kv_heads), tokens, batch, tables.data_ptr(), index_size(tables), tables.size(0), tables.size(1),
+        tables.stride(0), page_size, rows ? rows->data_ptr() : nullptr, rows_es, lengths.data_ptr(), len_es,
+        starts ? starts->data_ptr() : nullptr, starts_es, shared_tokens, source_row, static_cast<float>(factor),
+        out->data_ptr(), stride_of(*out, 0), stride_of(*out, 1), lse ? lse->data_ptr<float>() : nullptr,
+        lse ? lse->stride(0) : 0, lse ? lse->stride(1) : 0, workspace.data_ptr(), bytes, device, stream_of(device));
+    if (rc != 0) return status(kKernelError);
+    return py::make_tuple(0, *out, lse ? py::cast(*lse) : py::object(py::none()));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -333,6 +506,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("shared_blocks", &shared_blocks);
     m.def("gather_rows", &gather_rows);
     m.def("gather_rows_planes", &gather_rows_planes);
+    m.def("extend_block_tables", &extend_block_tables);
+    m.def("append_rows", &append_rows);
+    m.def("shared_prefix_attention", &shared_prefix_attention);
     m.attr("NOT_HANDLED") = kNotHandled;
     m.attr("KERNEL_ERROR") = kKernelError;
 }

@@ -20,7 +20,7 @@ import math
 
 import torch
 
-from ._lib import ATTENTION_MAX_ROW_TILES, call, index_esize, require_cuda, stream_handle
+from ._lib import ATTENTION_MAX_ROW_TILES, call, index_esize, last_error, require_cuda, stream_handle, torch_binding
 from .block_tables import _vector
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}  # EKV_BF16, EKV_FP16
@@ -39,6 +39,15 @@ def _rows_ok(tensor: torch.Tensor, name: str) -> None:
 def _strides(tensor: torch.Tensor) -> tuple[int, int]:
     """Strides of the first two dimensions; 0 for one of a single entry."""
     return tuple(s if n > 1 else 0 for n, s in zip(tensor.shape[:2], tensor.stride()[:2]))
+
+
+def _outputs(query, out, lse, return_lse):
+    require_cuda(dict(query=query))
+    if out is None:
+        out = torch.empty(query.shape, dtype=query.dtype, device=query.device)
+    if lse is None and return_lse:
+        lse = torch.empty(query.shape[:2], dtype=torch.float32, device=query.device)
+    return out, lse
 
 
 def _bind(query, k_plane, v_plane, block_tables, lengths, page_size, shared_tokens, source_row, rows,
@@ -142,10 +151,19 @@ def shared_prefix_attention(query: torch.Tensor, k_plane: torch.Tensor, v_plane:
     ``scale`` defaults to ``1 / sqrt(dim)``; ``lse`` is float32 [tokens, query_heads], the natural
     logarithm of the sum of the exponentials.  Scores, maxima, sums and outputs are held in 32 bits.
     """
-    if out is None:
-        out = torch.empty_like(query, memory_format=torch.contiguous_format)
-    if lse is None and return_lse:
-        lse = torch.empty(query.shape[:2], dtype=torch.float32, device=query.device)
+    fast = torch_binding() if all(type(x) is int for x in (page_size, shared_tokens, source_row)) else None
+    if fast is not None:
+        try:
+            rc, result, sums = fast.shared_prefix_attention(query, k_plane, v_plane, block_tables, lengths, page_size,
+                                                            shared_tokens, source_row, rows, query_starts, scale, out, lse,
+                                                            return_lse)
+        except TypeError:  # not tensors: the checked path below reports it
+            rc = fast.NOT_HANDLED
+        if rc == 0:
+            return result if sums is None else (result, sums)
+        if rc == fast.KERNEL_ERROR:
+            raise last_error("ekv_shared_prefix_attention")
+    out, lse = _outputs(query, out, lse, return_lse)
     args, device = _bind(query, k_plane, v_plane, block_tables, lengths, page_size, shared_tokens, source_row, rows,
                          query_starts, scale, out, lse)
     need = _workspace_bytes(query, k_plane.shape[1], lengths.shape[0], device)
@@ -165,10 +183,7 @@ class SharedPrefixAttention:
 
     def __init__(self, query, k_plane, v_plane, block_tables, lengths, *, page_size, shared_tokens=0, source_row=0,
                  rows=None, query_starts=None, scale=None, out=None, lse=None, return_lse=False):
-        if out is None:
-            out = torch.empty_like(query, memory_format=torch.contiguous_format)
-        if lse is None and return_lse:
-            lse = torch.empty(query.shape[:2], dtype=torch.float32, device=query.device)
+        out, lse = _outputs(query, out, lse, return_lse)
         args, self.device = _bind(query, k_plane, v_plane, block_tables, lengths, page_size, shared_tokens,
                                   source_row, rows, query_starts, scale, out, lse)
         need = _workspace_bytes(query, k_plane.shape[1], lengths.shape[0], self.device)
