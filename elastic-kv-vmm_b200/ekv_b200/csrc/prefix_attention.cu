@@ -66,7 +66,7 @@ constexpr int kFewTile = 64;         // its unit of work, positions
 constexpr int kFewStart = 2, kFewUnit = 1;
 constexpr int kFewWarps = 8;
 constexpr int kFewPrefix = 4096;     // longest prefix it takes: a part of it to a worker, joined one by one
-constexpr int kLargeTime = 37, kFewTime = 40, kLeastShare = 24;
+constexpr int kLargeTime = 37, kFewTime = 35, kLeastShare = 24;
 enum Mode { kSingle = 0, kBoth = 1, kPair = 2 };
 constexpr int kMaskRing = 16;
 constexpr int kItemRing = 8, kItemsAhead = 5;
@@ -219,7 +219,7 @@ __device__ __forceinline__ uint32_t few_prefix_cost(const AttentionParams& p) {
 }
 
 // Blocks (an SM each) that attention_kernel uses when both kernels have work: the two share the SMs in
-// proportion to their estimated times there (a unit of its cost took 0.37 us, one of rows_kernel's 0.40 us), so
+// proportion to their estimated times there (a unit of its cost took 0.37 us, one of rows_kernel's 0.35 us), so
 // that the memory-bound part runs beside the compute-bound one.
 __device__ __forceinline__ int large_blocks(const AttentionParams& p, int64_t large, int64_t few) {
     if (!few || !large) return p.blocks;
