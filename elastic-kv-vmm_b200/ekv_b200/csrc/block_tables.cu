@@ -8,7 +8,7 @@
 // granted request's pages are free_pages[P(b-1) .. P(b)), and its i-th token (position
 // L + i) has slot  page(position / p) * p + position % p.
 // Bound by latency up to ~10^5 tokens: one launch in which EVERY block scans the
-// whole batch (512 requests a pass; two dependent 4-byte loads and one block scan)
+// whole batch (1024 requests a pass; two dependent 4-byte loads and one block scan)
 // and then places only its own slice of tokens and pages, so no second launch or
 // grid-wide wait separates the scan from the placement.
 //
@@ -20,10 +20,10 @@
 namespace ekv {
 namespace {
 
-constexpr int kTableThreads = 512;
+constexpr int kTableThreads = 1024;
 constexpr int kTableWarps = kTableThreads / 32;
-// Tokens (and pages) one block places per pass over its slice.
-constexpr int kTokensPerBlock = 4 * kTableThreads;
+// Tokens (and pages) one block places.
+constexpr int kTokensPerBlock = 2 * kTableThreads;
 
 struct TableParams {
     int32_t* tables;
@@ -49,6 +49,7 @@ __device__ __forceinline__ uint32_t page_of(const TableParams& p, uint32_t posit
 }
 
 // Inclusive scan of (a, b) over the block; totals of the block in (ta, tb).
+static_assert(kTableWarps == 32, "a lane per warp");
 __device__ __forceinline__ void block_scan(int64_t& a, int64_t& b, int64_t& ta, int64_t& tb, int64_t (*sums)[2]) {
     const unsigned lane = lane_id(), warp = threadIdx.x >> 5;
 #pragma unroll
@@ -58,16 +59,17 @@ __device__ __forceinline__ void block_scan(int64_t& a, int64_t& b, int64_t& ta, 
     }
     if (lane == 31) sums[warp][0] = a, sums[warp][1] = b;
     __syncthreads();
-    int64_t before_a = 0, before_b = 0;
-    ta = tb = 0;
+    // Every warp scans the warps' sums, a lane each.
+    int64_t ra = sums[lane][0], rb = sums[lane][1];
 #pragma unroll
-    for (int w = 0; w < kTableWarps; ++w) {
-        if (w == warp) before_a = ta, before_b = tb;
-        ta += sums[w][0];
-        tb += sums[w][1];
+    for (int d = 1; d < 32; d <<= 1) {
+        const int64_t ua = __shfl_up_sync(0xffffffffu, ra, d), ub = __shfl_up_sync(0xffffffffu, rb, d);
+        if (lane >= d) ra += ua, rb += ub;
     }
-    a += before_a;
-    b += before_b;
+    ta = __shfl_sync(0xffffffffu, ra, 31);
+    tb = __shfl_sync(0xffffffffu, rb, 31);
+    const int64_t before_a = __shfl_sync(0xffffffffu, ra, warp - 1), before_b = __shfl_sync(0xffffffffu, rb, warp - 1);
+    if (warp) a += before_a, b += before_b;
 }
 
 // Largest i in [0, count) with start[i] <= x, for start[0] <= x (start ascending).

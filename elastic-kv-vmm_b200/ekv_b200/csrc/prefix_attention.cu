@@ -1484,8 +1484,6 @@ __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_c
     constexpr int kVectors = kDim / (4 * kJoinLanes);  // of four values, of a row, in a lane
     constexpr int kAtOnce = kSplit == 1 ? 2 : 4;       // parts whose loads are on their way together
     constexpr uint32_t kAll = 0xffffffffu;
-    grid_dependency_wait();
-    allow_dependents();
     const int lane = static_cast<int>(lane_id()) % kJoinLanes;
     const int mine_of = static_cast<int>(threadIdx.x) / kJoinLanes % kSplit;
     const int64_t index = (static_cast<int64_t>(blockIdx.x) * 32 * kJoinWarps + threadIdx.x) / (kJoinLanes * kSplit);
@@ -1494,7 +1492,10 @@ __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_c
     const int kv_head = head / p.group, head_row = n * p.group + head - kv_head * p.group;
     int64_t b;
     Request request{0, 0, 0};
+    // The requests are as the kernels before found them (they have waited for what writes them).
     const bool active = request_of(p, n, b, request);
+    grid_dependency_wait();
+    allow_dependents();
     int prefix_item = 0, own_item = 0, local = 0, prefix_first = 0, own_first = 0, prefix_count = 0, count = 0;
     bool few = false;
     if (active) {

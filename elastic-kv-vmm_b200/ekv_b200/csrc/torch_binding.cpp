@@ -363,11 +363,18 @@ py::tuple extend_block_tables(const at::Tensor& tables, const at::Tensor& length
     const int len_es = vector_size(lengths, batch), fresh_es = vector_size(fresh, batch);
     const int rows_es = rows ? vector_size(*rows, batch) : 8;
     if (!len_es || !fresh_es || !rows_es || !vector_size(free_pages, -1)) return status(kNotHandled);
+    // Five outputs in one allocation; the views are made without the dispatcher, which took most of the call.
     const at::Tensor flat = at::empty({2 * batch + 2 * max_tokens + 2}, tables.options());
-    at::Tensor starts = flat.narrow(0, 0, batch + 1), slots = flat.narrow(0, batch + 1, max_tokens);
-    at::Tensor positions = flat.narrow(0, batch + 1 + max_tokens, max_tokens);
-    at::Tensor after = flat.narrow(0, batch + 1 + 2 * max_tokens, batch);
-    at::Tensor used = flat.narrow(0, 2 * batch + 1 + 2 * max_tokens, 1);
+    int64_t offset = 0;
+    const auto part = [&](int64_t count) {
+        at::Tensor view = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(flat.storage()), flat.key_set(), flat.dtype());
+        view.unsafeGetTensorImpl()->set_storage_offset(offset);
+        view.unsafeGetTensorImpl()->set_sizes_contiguous({count});
+        offset += count;
+        return view;
+    };
+    at::Tensor starts = part(batch + 1), slots = part(max_tokens), positions = part(max_tokens);
+    at::Tensor after = part(batch), used = part(1);
     const int rc = g_extend(
         tables.data_ptr<int32_t>(), tables.size(0), tables.size(1), tables.stride(0),
         rows ? rows->data_ptr() : nullptr, rows_es, lengths.data_ptr(), len_es, fresh.data_ptr(), fresh_es, batch,
