@@ -52,7 +52,7 @@ constexpr int kGatherRows = 2 * kTile / kGatherWarps;  // rows of a K or V tile 
 static_assert(kGatherRows == 32, "a lane resolves one row");
 constexpr int kThreads = 256 + 32 * kGatherWarps + 128;
 // Registers a thread: 640 threads start with 96; the softmax warps take what the gather gives up.
-constexpr int kStartRegisters = 96, kSoftmaxRegisters = 128, kGatherRegisters = 64, kOtherRegisters = 96;
+constexpr int kStartRegisters = 96, kSoftmaxRegisters = 144, kGatherRegisters = 48, kOtherRegisters = 96;
 static_assert(256 * kSoftmaxRegisters + 32 * kGatherWarps * kGatherRegisters + 128 * kOtherRegisters <=
                   kThreads * kStartRegisters, "more registers than the block starts with");
 constexpr int kMaxEntries = EKV_ATTENTION_MAX_ROW_TILES;
@@ -158,7 +158,7 @@ __device__ __forceinline__ bool request_of(const AttentionParams& p, int64_t n, 
 
 // Where position j of table row `row` is looked up: the page is loaded at once and used later.
 struct Lookup {
-    int64_t page;     // -1: none
+    int page;         // -1: none
     uint32_t offset;  // in the page
 };
 
@@ -166,7 +166,13 @@ __device__ __forceinline__ Lookup look_up(const AttentionParams& p, int row, uin
     Lookup found{-1, 0};
     const uint32_t index = p.page_log2 >= 0 ? j >> p.page_log2 : j / p.page_size;
     if (row >= 0 && index < p.table_width) {
-        found.page = load_index(p.tables, p.table_es, row * p.table_stride + index);
+        const int64_t at = row * p.table_stride + index;
+        if (p.table_es == 8) {
+            const int64_t page = static_cast<const int64_t*>(p.tables)[at];
+            found.page = page >= 0 && page < p.slots ? static_cast<int>(page) : -1;
+        } else {
+            found.page = static_cast<const int32_t*>(p.tables)[at];
+        }
         found.offset = j - index * p.page_size;
     }
     return found;
@@ -175,7 +181,7 @@ __device__ __forceinline__ Lookup look_up(const AttentionParams& p, int row, uin
 // The slot, or -1 where there is none inside the planes.
 __device__ __forceinline__ int slot_of(const AttentionParams& p, const Lookup& found) {
     if (found.page < 0 || found.page >= p.slots) return -1;
-    const int64_t slot = found.page * p.page_size + found.offset;
+    const int64_t slot = static_cast<int64_t>(found.page) * p.page_size + found.offset;
     return slot < p.slots ? static_cast<int>(slot) : -1;
 }
 
@@ -523,9 +529,8 @@ struct Layout {
     static constexpr uint32_t kMasks = kItems + kItemRing * sizeof(Item);
     static constexpr uint32_t kStats = kMasks + kMaskRing * 16;  // maximum and sum of each row, of both slots
     static constexpr uint32_t kBarriers = kStats + 2 * kRows * 8;
-    // Six of each stage, seven of each slot, two of each place in the item ring, eight for the
-    // turns, one where the slots of a pair meet.
-    static constexpr int kBarrierCount = 6 * kStages + 7 * 2 + 2 * kItemRing + 8 + 1;
+    // Six of each stage, nine of each slot, two of each place in the item ring, one where the slots of a pair meet.
+    static constexpr int kBarrierCount = 6 * kStages + 9 * 2 + 2 * kItemRing + 1;
     static constexpr uint32_t kTail = kBarriers + kBarrierCount * 8;
     static constexpr uint32_t kBytes = kTail + 16;  // tensor-memory address, failed flag
 };
@@ -573,15 +578,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     const auto slot_barrier = [&](int which, int s) { return barriers + 8 * (6 * L::kStages + 2 * which + s); };
     const auto q_landed = [&](int s) { return slot_barrier(0, s); };
     const auto q_full = [&](int s) { return slot_barrier(1, s); };
-    const auto s_full = [&](int s) { return slot_barrier(2, s); };
-    const auto p_full = [&](int s) { return slot_barrier(3, s); };
-    const auto o_full = [&](int s) { return slot_barrier(4, s); };
-    const auto p_half = [&](int s) { return slot_barrier(5, s); };
-    const auto item_full = [&](int i) { return barriers + 8 * (6 * L::kStages + 12 + i); };
-    const auto item_empty = [&](int i) { return barriers + 8 * (6 * L::kStages + 12 + kItemRing + i); };
-    const auto go = [&](int s, int w) { return barriers + 8 * (L::kBarrierCount - 11 + 4 * s + w); };
-    const uint32_t meet = barriers + 8 * (L::kBarrierCount - 3);
-    const auto drain = [&](int s) { return barriers + 8 * (L::kBarrierCount - 2 + s); };
+    const auto s_full = [&](int s, int half) { return slot_barrier(2 + half, s); };  // scores of half a tile
+    const auto p_full = [&](int s, int half) { return slot_barrier(4 + half, s); };  // its weights
+    const auto o_half = [&](int s) { return slot_barrier(6, s); };                   // added to the output
+    const auto o_full = [&](int s) { return slot_barrier(7, s); };                   // the item's last one too
+    const auto drain = [&](int s) { return slot_barrier(8, s); };
+    const auto item_full = [&](int i) { return barriers + 8 * (6 * L::kStages + 18 + i); };
+    const auto item_empty = [&](int i) { return barriers + 8 * (6 * L::kStages + 18 + kItemRing + i); };
+    const uint32_t meet = barriers + 8 * (L::kBarrierCount - 1);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < L::kStages; ++s) {
@@ -595,12 +599,13 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         for (int s = 0; s < 2; ++s) {
             barrier_init(q_landed(s), kRows);
             barrier_init(q_full(s), 1);
-            barrier_init(s_full(s), 1);
-            barrier_init(p_half(s), 4);
-            barrier_init(p_full(s), 4);
+            for (int half = 0; half < 2; ++half) {
+                barrier_init(s_full(s, half), 1);
+                barrier_init(p_full(s, half), 4);
+            }
+            barrier_init(o_half(s), 1);
             barrier_init(o_full(s), 1);
             barrier_init(drain(s), 1);
-            for (int w = 0; w < 4; ++w) barrier_init(go(s, w), 1);
         }
         barrier_init(meet, 8);
         for (int i = 0; i < kItemRing; ++i) {
@@ -655,7 +660,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         const uint32_t lanes = static_cast<uint32_t>(warp & 3) << 21;  // 32 tensor-memory lanes a warp
         const uint32_t scores = tensor + lanes + slot * kTile;
         const uint32_t output = tensor + lanes + 256 + slot * 128;
-        uint32_t uses = 0, ends = 0, tiles_before = 0, turns = 0, meetings = 0;
+        uint32_t uses = 0, halves = 0, ends = 0, tiles_before = 0, meetings = 0;
         const int r = (warp & 3) * 32 + lane;
         float2* stats = reinterpret_cast<float2*>(shared + L::kStats);
         // The items this slot has a part in, one ahead: its queries are copied (each warp its 32 rows)
@@ -719,134 +724,85 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             float2 total = make_float2(0.f, 0.f);
             const int low = item.low + (pair ? slot : 0), high = item.high, step = pair ? 2 : 1;
             const uint32_t mask_base = tiles - item.low;
-            for (int t = low; t < high; t += step) {
-                if (!__all_sync(0xffffffffu, barrier_wait(s_full(slot), uses & 1, failed))) goto finish;
-                ++uses;
-                tensor_fence_after();
-                if (t + step >= high && !prepare()) goto finish;
-                if (!idle) {
-                    // Positions this row sees here: those that have a slot, up to its last.
-                    const int left = limit - t * kTile;
-                    const uint4 there = masks[(mask_base + t) % kMaskRing];
-                    const bool whole = __all_sync(0xffffffffu, left >= kTile) &&
-                                       (there.x & there.y & there.z & there.w) == 0xffffffffu;
-                    if (!whole) {
+            for (int t = low; t < high; t += step, ++uses) {
 #pragma unroll 1
-                        for (int c = 0; c < 4; ++c) {
-                            const uint32_t bits = c == 0 ? there.x : c == 1 ? there.y : c == 2 ? there.z : there.w;
-                            const int limit32 = left - 32 * c;
-                            const uint32_t seen32 =
-                                bits & (limit32 >= 32 ? 0xffffffffu : (limit32 <= 0 ? 0u : (1u << limit32) - 1u));
-                            if (__all_sync(0xffffffffu, seen32 == 0xffffffffu)) continue;
-                            uint32_t masked[32];
-                            tensor_load32(scores + 32 * c, masked);
-                            tensor_wait_load();
+                for (int half = 0; half < 2; ++half, ++halves) {
+                    if (!__all_sync(0xffffffffu, barrier_wait(s_full(slot, half), uses & 1, failed))) goto finish;
+                    tensor_fence_after();
+                    if (half && t + step >= high && !prepare()) goto finish;
+                    if (!idle) {
+                        const uint32_t mine = scores + 64 * half;
+                        uint32_t s[64];
+                        tensor_load32(mine, s);
+                        tensor_load32(mine + 32, s + 32);
+                        // Positions this row sees here: those that have a slot, up to its last.
+                        const int left = limit - t * kTile - 64 * half;
+                        const uint2 there = reinterpret_cast<const uint2*>(&masks[(mask_base + t) % kMaskRing])[half];
+                        const bool whole = __all_sync(0xffffffffu, left >= 64) && (there.x & there.y) == 0xffffffffu;
+                        tensor_wait_load();
+                        if (!whole) {
+                            const auto until = [](int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); };
+                            const uint32_t first = there.x & until(left), second = there.y & until(left - 32);
 #pragma unroll
                             for (int j = 0; j < 32; ++j) {
-                                if (!(seen32 >> j & 1u)) masked[j] = 0xff800000u;  // -inf
+                                if (!(first >> j & 1u)) s[j] = 0xff800000u;  // -inf
+                                if (!(second >> j & 1u)) s[32 + j] = 0xff800000u;
                             }
-                            tensor_store32(scores + 32 * c, masked);
                         }
-                        tensor_wait_store();
-                    }
-                    // Largest score: 32 columns are compared while the next 32 are on their way.  The loops over a
-                    // tile are kept rolled: with 128 columns unrolled the kernel ran 1.6 times slower, its roles'
-                    // code exceeding the instruction cache.
-                    uint32_t a[32], b[32];
-                    float highs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                    const auto raise_to = [&](const uint32_t* s) {
+                        float highs[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-                        for (int j = 0; j < 32; j += 8) {
+                        for (int j = 0; j < 64; j += 8) {
 #pragma unroll
                             for (int c = 0; c < 4; ++c) {
                                 highs[c] = max3(highs[c], __uint_as_float(s[j + 2 * c]), __uint_as_float(s[j + 2 * c + 1]));
                             }
                         }
-                    };
-                    tensor_load32(scores, a);
+                        const float most = fmaxf(fmaxf(highs[0], highs[1]), fmaxf(highs[2], highs[3])) * p.scale_log2;
+                        const bool raise = present && (most > top + kRaise || (top == -INFINITY && most > -INFINITY));
+                        if (__any_sync(0xffffffffu, raise)) {
+                            const float before = top;
+                            if (raise) top = most;
+                            const float factor = raise ? (before == -INFINITY ? 0.f : exp2_approx(before - top)) : 1.f;
+                            total.x *= factor;
+                            total.y *= factor;
+                            if (t > low || half) {
+                                // The weights so far are all in the output before it is scaled (those before the last
+                                // half's are: the product behind them gave these scores).
+                                if (!__all_sync(0xffffffffu, barrier_wait(o_half(slot), (halves - 1) & 1, failed))) goto finish;
+                                tensor_fence_after();
 #pragma unroll 1
-                    for (int c = 0; c < kTile; c += 64) {
-                        tensor_wait_load();
-                        tensor_load32(scores + c + 32, b);
-                        raise_to(a);
-                        tensor_wait_load();
-                        tensor_load32(scores + (c ? 0 : 64), a);  // the second time the first columns again, for below
-                        raise_to(b);
-                    }
-                    const float most = fmaxf(fmaxf(highs[0], highs[1]), fmaxf(highs[2], highs[3])) * p.scale_log2;
-                    const bool raise = present && (most > top + kRaise || (top == -INFINITY && most > -INFINITY));
-                    if (__any_sync(0xffffffffu, raise)) {
-                        const float before = top;
-                        if (raise) top = most;
-                        const float factor = raise ? (before == -INFINITY ? 0.f : exp2_approx(before - top)) : 1.f;
-                        total.x *= factor;
-                        total.y *= factor;
-                        if (t > low) {
-                            // The products of this slot's earlier tiles are complete (s_full).
-#pragma unroll 1
-                            for (int c = 0; c < kDim / 16; ++c) {
-                                uint32_t o[16];
-                                tensor_load16(output + 16 * c, o);
-                                tensor_wait_load();
+                                for (int c = 0; c < kDim / 16; ++c) {
+                                    uint32_t o[16];
+                                    tensor_load16(output + 16 * c, o);
+                                    tensor_wait_load();
 #pragma unroll
-                                for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * factor);
-                                tensor_store16(output + 16 * c, o);
+                                    for (int j = 0; j < 16; ++j) o[j] = __float_as_uint(__uint_as_float(o[j]) * factor);
+                                    tensor_store16(output + 16 * c, o);
+                                }
                             }
                         }
-                    }
-                    const float shift = top == -INFINITY ? 0.f : -top;
-                    // The exponentials of the two slots take turns (a warp of each shares a quarter of
-                    // the SM): together they would leave the tensor cores idle, and then wait for them together.
-                    if (both && !__all_sync(0xffffffffu, barrier_wait(go(slot, warp & 3), (turns & 1) ^ (slot ^ 1), failed))) {
-                        goto finish;
-                    }
-                    const auto weigh = [&](const uint32_t* s, uint32_t target) {
-                        uint32_t weights[16];
+                        const float shift = top == -INFINITY ? 0.f : -top;
 #pragma unroll
-                        for (int j = 0; j < 32; j += 2) {
-                            float2 x = fma2(make_float2(__uint_as_float(s[j]), __uint_as_float(s[j + 1])),
-                                            make_float2(p.scale_log2, p.scale_log2), make_float2(shift, shift));
-                            x.x = exp2_approx(x.x);
-                            x.y = exp2_approx(x.y);
-                            total = add2(total, x);
-                            weights[j / 2] = Kind<T>::pack(x.x, x.y);
+                        for (int c = 0; c < 2; ++c) {
+                            uint32_t weights[16];
+#pragma unroll
+                            for (int j = 0; j < 32; j += 2) {
+                                const int at = 32 * c + j;
+                                float2 x = fma2(make_float2(__uint_as_float(s[at]), __uint_as_float(s[at + 1])),
+                                                make_float2(p.scale_log2, p.scale_log2), make_float2(shift, shift));
+                                x.x = exp2_approx(x.x);
+                                x.y = exp2_approx(x.y);
+                                total = add2(total, x);
+                                weights[j / 2] = Kind<T>::pack(x.x, x.y);
+                            }
+                            tensor_store16(mine + 16 * c, weights);
                         }
-                        tensor_store16(target, weights);
-                    };
-#pragma unroll 1
-                    for (int c = 0; c < kTile; c += 64) {
-                        tensor_wait_load();
-                        tensor_load32(scores + c + 32, b);
-                        weigh(a, scores + c / 2);
-                        if (c) {  // the second product may begin on the first half, whose stores have had time to land
-                            tensor_wait_store();
-                            tensor_fence_before();
-                            __syncwarp();
-                            if (lane == 0) barrier_arrive(p_half(slot));
-                        }
-                        tensor_wait_load();
-                        if (c == 0) tensor_load32(scores + 64, a);
-                        weigh(b, scores + c / 2 + 16);
+                        tensor_wait_store();
                     }
-                    tensor_wait_store();
-                    if (both) {
-                        __syncwarp();
-                        if (lane == 0) barrier_arrive(go(slot ^ 1, warp & 3));
-                        ++turns;
-                    }
-                } else {
-                    if (lane == 0) barrier_arrive(p_half(slot));
-                    if (both) {
-                        if (!__all_sync(0xffffffffu, barrier_wait(go(slot, warp & 3), (turns & 1) ^ (slot ^ 1), failed))) {
-                            goto finish;
-                        }
-                        if (lane == 0) barrier_arrive(go(slot ^ 1, warp & 3));
-                        ++turns;
-                    }
+                    tensor_fence_before();
+                    __syncwarp();
+                    if (lane == 0) barrier_arrive(p_full(slot, half));
                 }
-                tensor_fence_before();
-                __syncwarp();
-                if (lane == 0) barrier_arrive(p_full(slot));
             }
             if (!__all_sync(0xffffffffu, barrier_wait(o_full(slot), ends & 1, failed))) goto finish;
             ++ends;
@@ -978,7 +934,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     } else if (lane == 0) {
         if (warp < kIssueWarp + 2) {
             // -------------------------------------------------------- products of slot `slot`
-            constexpr uint32_t kScoreProduct = mma_descriptor(Kind<T>::kBf16, kRows, kTile, false);
+            constexpr uint32_t kScoreProduct = mma_descriptor(Kind<T>::kBf16, kRows, kTile / 2, false);
             constexpr uint32_t kOutputProduct = mma_descriptor(Kind<T>::kBf16, kRows, kDim, true);
             const int slot = warp - kIssueWarp;
             const uint32_t scores = tensor + slot * kTile, output = tensor + 256 + slot * 128;
@@ -999,55 +955,53 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                 const int low = item.low + (pair ? slot : 0), high = item.high, step = pair ? 2 : 1;
                 if (!(fine = barrier_wait(q_full(slot), q_uses & 1, failed))) break;
                 ++q_uses;
-                // The first product of the first tile; then the second product of tile t with the first one
-                // of tile t + 1 right behind it, so that the next scores are on their way at once.
-                const auto first = [&](uint32_t use) {
-                    const uint64_t keys = all_keys + (use % L::kStages) * (L::kOperand >> 4);
+                const auto parity = [&](uint32_t use) { return (use / L::kStages) & 1; };
+                // Scores of half a tile; then, as soon as the weights of a half are there, their product
+                // with V, and right behind it the scores of that half of the next tile, so that
+                // the softmax of one half runs beside the products of the other.
+                const auto score = [&](uint32_t use, int half) {
+                    const uint64_t keys = all_keys + (use % L::kStages) * (L::kOperand >> 4) + half * (64 * 128 >> 4);
 #pragma unroll
                     for (int k = 0; k < kDim / 16; ++k) {
                         const uint32_t step = (k / 4) * (L::kBlock >> 4) + (k % 4) * 2;
-                        mma_shared(scores, queries + step, keys + step, kScoreProduct, k > 0);
+                        mma_shared(scores + 64 * half, queries + step, keys + step, kScoreProduct, k > 0);
                     }
-                    mma_commit(s_full(slot));
-                    mma_commit(k_empty(use % L::kStages));
+                    mma_commit(s_full(slot, half));
                 };
-                const auto parity = [&](uint32_t use) { return (use / L::kStages) & 1; };
                 uint32_t use = before + low;
                 if (!(fine = barrier_wait(k_full(use % L::kStages), parity(use), failed))) break;
                 tensor_fence_after();
-                first(use);
-                for (int t = low; t < high; t += step, use += step) {
+                score(use, 0);
+                score(use, 1);
+                mma_commit(k_empty(use % L::kStages));
+                for (int t = low; t < high; t += step, use += step, ++p_uses) {
                     const int stage = use % L::kStages;
                     const uint32_t next_use = use + step;
-                    if (!(fine = barrier_wait(v_full(stage), parity(use), failed))) break;
-                    const uint64_t values = all_values + stage * (L::kOperand >> 4);
-                    if (!(fine = barrier_wait(p_half(slot), p_uses & 1, failed))) break;
-                    tensor_fence_after();
-#pragma unroll
-                    for (int k = 0; k < kTile / 32; ++k) {
-                        mma_tensor(output, scores + 8 * k, values + k * (16 * 128 >> 4), kOutputProduct, t > low || k > 0);
-                    }
                     const bool more = t + step < high;
-                    const bool ready = more && barrier_test(k_full(next_use % L::kStages), parity(next_use));
-                    if (!(fine = barrier_wait(p_full(slot), p_uses & 1, failed))) break;
-                    ++p_uses;
-                    tensor_fence_after();
+                    if (!(fine = barrier_wait(v_full(stage), parity(use), failed))) break;
+#pragma unroll 1
+                    for (int half = 0; half < 2; ++half) {
+                        const uint64_t values = all_values + stage * (L::kOperand >> 4) + half * (64 * 128 >> 4);
+                        if (!(fine = barrier_wait(p_full(slot, half), p_uses & 1, failed))) break;
+                        tensor_fence_after();
 #pragma unroll
-                    for (int k = kTile / 32; k < kTile / 16; ++k) {
-                        mma_tensor(output, scores + 8 * k, values + k * (16 * 128 >> 4), kOutputProduct, true);
-                    }
-                    if (!ready) mma_commit(v_empty(stage));
-                    if (more) {
-                        if (!ready) {
+                        for (int k = 0; k < kTile / 32; ++k) {
+                            mma_tensor(output, scores + 64 * half + 8 * k, values + k * (16 * 128 >> 4), kOutputProduct,
+                                       t > low || half > 0 || k > 0);
+                        }
+                        mma_commit(o_half(slot));
+                        if (half) mma_commit(v_empty(stage));
+                        if (!more) continue;
+                        if (!half) {
                             if (!(fine = barrier_wait(k_full(next_use % L::kStages), parity(next_use), failed))) break;
                             tensor_fence_after();
                         }
-                        first(next_use);
+                        score(next_use, half);
+                        if (half) mma_commit(k_empty(next_use % L::kStages));
                     }
-                    if (ready) mma_commit(v_empty(stage));
+                    if (!fine) break;
                 }
-                if (!fine) break;
-                mma_commit(o_full(slot));
+                if (fine) mma_commit(o_full(slot));
             }
             // Nothing may still use tensor memory when it is freed, whatever happened above.
             mma_commit(drain(slot));
