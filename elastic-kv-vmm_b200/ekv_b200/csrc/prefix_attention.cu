@@ -5,34 +5,43 @@
 // source request's table row, every other through the request's own:
 //     o = sum_j exp(scale q.k_j) v_j / sum_j exp(scale q.k_j),   lse = log sum_j exp(scale q.k_j).
 //
-// The work is a list of ITEMS, one per KV head and row tile (up to 256 query rows that read
-// the same keys, a row being a token and one of the head's query heads):
-//   * prefix items: row tiles over ALL tokens of the batch against the P shared positions;
-//   * own items: row tiles of one request against its positions from P on.
-// An item is a run of 128-position tiles.  Its cost is kItemCost + kTileCost per tile; the
-// total is cut into one equal share per SM (attention_kernel runs one block per SM), so an
-// item may be spread over several blocks, each of which leaves a partial result (running
-// maximum, sum and unscaled output in 32 bits).  Every block derives its share from the
-// lengths by itself (one scan over the requests), so lengths may change under a captured
-// graph, and memory-bound own items run beside the compute-bound prefix items.
-// combine_kernel joins the partial results of each row.
+// Three kernels.  rows_kernel takes the requests of up to 16 query rows a KV head (a decode step), each
+// against its own positions from P on, and a short prefix of a small batch: too few rows for a
+// tensor-core tile, so HBM bounds it.  attention_kernel takes the rest: all rows of the batch against the
+// shared positions, a matrix product that grows with the batch, and the own positions of requests
+// with more rows (prompts).  combine_kernel joins what they leave.  The first two run side by side, each on
+// SMs of its own: blocks of attention_kernel that the plan has no work for leave at once.
 //
-// attention_kernel, one tile: S = Q K^T and O += P V on the tensor cores (tcgen05, 128 rows x
-// 128 positions, 32-bit sums in tensor memory), a softmax thread per row between them.
-// Roles by warp: 0-3 and 4-7 softmax of row tile halves ("slots") 0 and 1; 8-11 gather the K rows,
-// 12-15 the V rows into swizzled shared memory (cp.async, 16 bytes a lane, whole rows; slots
-// resolved through the table, zeros for positions without one; the queries are copied by the softmax
-// warps themselves, as soon as their last product with the ones before is complete); 16 and 17 issue the products of slots 0 and 1 (one
-// thread each, so that the waits and commits of one fall beside the other's products); 18 and 19 pass
-// on the V and K rows that have landed, with the fence between ordinary writes and the tensor cores'
-// reads; 18 also walks the block's items and hands them to the others through a small ring.
-// An item of more than 128 rows uses both
-// slots on the same K and V; a smaller one with many tiles gives its even tiles to one slot and
-// its odd ones to the other (kPair; the two join before they are written); with few tiles, items
-// alternate between the slots.  In each case one slot's softmax runs beside the other's products.  The maximum a row's weights refer to is raised only when the tile's
-// maximum passes it by 2^8 (kRaise), which makes rescaling O rare; sums stay exact to 32 bits since the
-// weights are bounded by 2^8.  Weights are rounded to the 16-bit type for the second product
-// (its operand type), the row sum is taken of the unrounded ones.
+// Work is a list of ITEMS, one per KV head and row tile (up to 256 query rows that read the same
+// keys, a row being a token and one of the head's query heads), each a run of 128-position
+// tiles.  An item costs a start and so much a tile; the total is cut into one equal share per block,
+// so an item may be spread over several, each of which leaves a part (maximum, sum and unscaled output
+// in 32 bits).  Every block derives its share from the lengths by itself (one scan over the
+// requests), so lengths may change under a captured graph and nothing is read back.
+//
+// attention_kernel, one tile: S = Q K^T and O += P V on the tensor cores (tcgen05, 128 rows, 32-bit sums
+// in tensor memory), a softmax thread per row between them.  The two halves of a tile follow one
+// another: the softmax of one runs beside the second product of the other and, right behind it, the first
+// product of that half of the next tile, whose scores take the place of its weights.  (A first product of 64
+// columns runs at half the tensor cores' rate, since its 128 rows come from shared memory each time; waiting
+// for products of whole tiles cost more: 8 prompts of 8001 tokens 372 us against 343.)
+// Roles by warp: 0-3 and 4-7 softmax of the halves ("slots") 0 and 1 of a row tile; 8-11 copy the K rows,
+// 12-15 the V rows into swizzled shared memory (cp.async, 16 bytes a lane, whole rows; slots resolved
+// through the table, zeros for positions without one); 16 and 17 issue the products of slots 0 and 1
+// (a thread each, so that the waits and commits of one fall beside the other's products); 18 and 19
+// pass on the V and K rows that have landed, with the fence between ordinary writes and the tensor cores'
+// reads; 18 also walks the block's items and hands them to the others through a small ring.  The queries
+// are copied by the softmax warps, as soon as their last product with the ones before is complete.
+// An item of more than 128 rows uses both slots on the same K and V (kBoth); a smaller one with many
+// tiles gives its even tiles to one slot and its odd ones to the other (kPair; the two join before
+// they are written); with few tiles, items alternate between the slots (kSingle).
+// What bounds it: the instructions of the softmax warps (128 x 256 exponentials a tile), beside which
+// eight copying warps run; the tensor cores are busy 40 % of the time.  256 requests of 64 heads over 32768
+// shared tokens and 1 to 256 own ones: 375 us for 279 GFLOP, 0.44 of the measured matrix peak.
+//
+// The maximum a row's weights refer to is raised only when the scores' maximum passes it by 2^8
+// (kRaise), which makes rescaling O rare; weights are then at most 2^8.  They are rounded to the 16-bit type
+// for the second product (its operand type); the row sum is taken of the unrounded ones.
 #include "tensor.cuh"
 
 #include <cuda_bf16.h>
@@ -225,8 +234,9 @@ __device__ __forceinline__ uint32_t few_prefix_cost(const AttentionParams& p) {
 }
 
 // Blocks (an SM each) that attention_kernel uses when both kernels have work: the two share the SMs in
-// proportion to their estimated times there (a unit of its cost took 0.37 us, one of rows_kernel's 0.35 us), so
-// that the memory-bound part runs beside the compute-bound one.
+// proportion to their estimated times there (a unit of its cost takes about 0.37 us of an SM, one of
+// rows_kernel's 0.35 us), so that the memory-bound part runs beside the compute-bound one: 128 requests over
+// 16384 shared tokens 181 us against 217 one behind the other.
 __device__ __forceinline__ int large_blocks(const AttentionParams& p, int64_t large, int64_t few) {
     if (!few || !large) return p.blocks;
     const int64_t mine = large * kLargeTime, its = few * kFewTime;
@@ -544,6 +554,9 @@ struct Kind<__nv_bfloat16> {
         const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&v);
     }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) {
+        return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&v));
+    }
 };
 template <>
 struct Kind<__half> {
@@ -551,6 +564,9 @@ struct Kind<__half> {
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __half2 v = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    static __device__ __forceinline__ float2 unpack(uint32_t v) {
+        return __half22float2(*reinterpret_cast<const __half2*>(&v));
     }
 };
 
@@ -1085,7 +1101,8 @@ struct FewLayout {
 };
 
 // Requests of up to 16 query rows (a decode step), and a short prefix of a small batch: too few rows to
-// fill a tensor-core tile, so HBM bounds them.  Work is cut as above, into equal shares of 64-position
+// fill a tensor-core tile, so HBM bounds them (the own positions of 128 requests, 0.5 GB: 92 us alone on the
+// GPU, 5.6 TB/s).  Work is cut as above, into equal shares of 64-position
 // units, but a share belongs to a WARP, which keeps to itself: it copies 16 or 32 positions of K and V at a
 // time into its own shared memory (the next keys while it weighs these, the next values while it
 // scores those) and multiplies them with mma.sync, positions by rows: S^T = K Q^T, O^T += V^T P^T,
@@ -1427,6 +1444,93 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) rows_kernel(const __grid_co
 constexpr int kJoinWarps = 4;
 constexpr int kJoinLanes = 8;  // of a row
 
+__device__ __forceinline__ bool finite(const float4& v) {
+    return isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w);
+}
+
+template <typename T, int kDim>
+__device__ __forceinline__ void write_row(const AttentionParams& p, int n, int head, int lane, const float4* acc, float scale) {
+    T* o = static_cast<T*>(p.out) + n * p.o_token + head * p.o_head + 4 * lane;
+#pragma unroll
+    for (int v = 0; v < kDim / (4 * kJoinLanes); ++v) {
+        *reinterpret_cast<uint2*>(o + v * 4 * kJoinLanes) = make_uint2(Kind<T>::pack(acc[v].x * scale, acc[v].y * scale),
+                                                                       Kind<T>::pack(acc[v].z * scale, acc[v].w * scale));
+    }
+}
+
+// A weight of 0 does not keep an infinity or NaN out of a product: a V row that a query row does not see
+// but another of its tile does (a later token of its request, a shared position behind a short request) may
+// leave one in its sum.  Such a row is summed again over the positions it sees, by the eight lanes that join it;
+// its maximum and sum stand, they come from the scores alone.  If what it does not see is finite, nothing is done.
+template <typename T, int kDim>
+__device__ __noinline__ void sum_again(const AttentionParams& p, int64_t b, const Request request, int n, int head, float top,
+                                       float scale) {
+    constexpr int kVectors = kDim / (4 * kJoinLanes);
+    const int lane = static_cast<int>(lane_id()) % kJoinLanes;
+    const uint32_t eight = 0xffu << (lane_id() & ~7u);
+    const int kv_head = head / p.group;
+    const int64_t at = n - request.begin, reach = p.table_width * p.page_size;
+    const int64_t before = static_cast<int64_t>(request.length) - request.fresh + 1;
+    int64_t seen = before + at < reach ? before + at : reach;
+    if (seen < 0) seen = 0;
+    const int64_t row_tile = (at * p.group + head - kv_head * p.group) / (2 * kRows);
+    int64_t last = before + last_token(row_tile, request.fresh, p.group);
+    if (last > reach) last = reach;
+    if (last < p.shared) last = p.shared;
+    const int64_t own = p.rows ? load_index(p.rows, p.rows_es, b) : b;
+    const int own_row = own >= 0 && own < p.table_rows ? static_cast<int>(own) : -1;
+    const auto slot_at = [&](int64_t j) {
+        return slot_of(p, look_up(p, j < p.shared ? static_cast<int>(p.source_row) : own_row, static_cast<uint32_t>(j)));
+    };
+    const auto load = [&](const void* plane, int64_t offset, float4* to) {
+        const T* from = static_cast<const T*>(plane) + offset + 4 * lane;
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            const uint2 raw = *reinterpret_cast<const uint2*>(from + v * 4 * kJoinLanes);
+            const float2 low = Kind<T>::unpack(raw.x), high = Kind<T>::unpack(raw.y);
+            to[v] = make_float4(low.x, low.y, high.x, high.y);
+        }
+    };
+    float4 row[kVectors];
+    bool found = false;
+    for (int64_t j = seen; j < last && !found; ++j) {
+        const int slot = slot_at(j);
+        if (slot < 0) continue;
+        load(p.v_plane, slot * p.v_slot + kv_head * p.v_head, row);
+        bool odd = false;
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) odd |= !finite(row[v]);
+        found = __any_sync(eight, odd);
+    }
+    if (!found) return;
+    float4 query[kVectors], acc[kVectors];
+    load(p.query, n * p.q_token + head * p.q_head, query);
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int64_t j = 0; j < seen; ++j) {
+        const int slot = slot_at(j);
+        if (slot < 0) continue;
+        load(p.k_plane, slot * p.k_slot + kv_head * p.k_head, row);
+        float score = 0.f;
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            score += query[v].x * row[v].x + query[v].y * row[v].y + query[v].z * row[v].z + query[v].w * row[v].w;
+        }
+#pragma unroll
+        for (int d = 1; d < kJoinLanes; d <<= 1) score += __shfl_xor_sync(eight, score, d);
+        const float weight = exp2_approx(score * p.scale_log2 - top);
+        load(p.v_plane, slot * p.v_slot + kv_head * p.v_head, row);
+#pragma unroll
+        for (int v = 0; v < kVectors; ++v) {
+            acc[v].x = fmaf(weight, row[v].x, acc[v].x);
+            acc[v].y = fmaf(weight, row[v].y, acc[v].y);
+            acc[v].z = fmaf(weight, row[v].z, acc[v].z);
+            acc[v].w = fmaf(weight, row[v].w, acc[v].w);
+        }
+    }
+    write_row<T, kDim>(p, n, head, lane, acc, scale);
+}
+
 // Eight lanes a row: the parts (m_i, l_i, O_i) of a row join as
 // sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i with m = max m_i.  The blocks (or workers) that may hold a part
 // of an item lie next to each other: a lane looks at each, first those of the row's prefix item, then
@@ -1579,15 +1683,16 @@ __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_c
     }
     if (!active || mine_of) return;
     const float scale = bad ? NAN : (total == 0.f ? 0.f : 1.f / total);
-    T* o = static_cast<T*>(p.out) + n * p.o_token + head * p.o_head + 4 * lane;
-#pragma unroll
-    for (int v = 0; v < kVectors; ++v) {
-        *reinterpret_cast<uint2*>(o + v * 4 * kJoinLanes) = make_uint2(Kind<T>::pack(acc[v].x * scale, acc[v].y * scale),
-                                                                       Kind<T>::pack(acc[v].z * scale, acc[v].w * scale));
-    }
+    write_row<T, kDim>(p, n, head, lane, acc, scale);
     if (p.lse && lane == 0) {
         p.lse[n * p.lse_token + head * p.lse_head] =
             bad ? NAN : (total == 0.f ? -INFINITY : (top + log2f(total)) * 0.69314718055994531f);
+    }
+    bool odd = false;
+#pragma unroll
+    for (int v = 0; v < kVectors; ++v) odd |= !finite(acc[v]);
+    if (__any_sync(0xffu << (lane_id() & ~7u), odd) && !bad && isfinite(total)) {
+        sum_again<T, kDim>(p, b, request, n, head, top, scale);
     }
 }
 

@@ -32,17 +32,6 @@ __device__ __forceinline__ bool barrier_try(uint32_t barrier, uint32_t parity) {
     return done != 0;
 }
 
-// As barrier_try, which may suspend the thread for a while, but returns at once.
-__device__ __forceinline__ bool barrier_test(uint32_t barrier, uint32_t parity) {
-    uint32_t done;
-    asm volatile(
-        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
-        : "=r"(done)
-        : "r"(barrier), "r"(parity)
-        : "memory");
-    return done != 0;
-}
-
 __device__ __forceinline__ uint64_t device_nanoseconds() {
     uint64_t t;
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
@@ -125,13 +114,6 @@ __device__ __forceinline__ void tensor_load32(uint32_t address, uint32_t* r) {
         "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
         : EKV_R8(r, 0), EKV_R8(r, 8), EKV_R8(r, 16), EKV_R8(r, 24)
         : "r"(address));
-}
-__device__ __forceinline__ void tensor_store32(uint32_t address, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::EKV_I8(r, 0),
-        EKV_I8(r, 8), EKV_I8(r, 16), EKV_I8(r, 24), "r"(address)
-        : "memory");
 }
 __device__ __forceinline__ void tensor_load16(uint32_t address, uint32_t* r) {
     asm volatile(
@@ -227,13 +209,6 @@ __device__ __forceinline__ void mma_warp(float (&c)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// Largest over the warp.
-__device__ __forceinline__ float warp_max(float x) {
-    float y;
-    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(y) : "f"(x));
     return y;
 }
 

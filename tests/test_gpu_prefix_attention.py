@@ -201,6 +201,46 @@ def test_nothing_behind_a_request_is_read(cuda_device):
         compare(case.run(cuda_device), want, case.dtype, v_max, 128)
 
 
+@pytest.mark.parametrize("odd", [float("inf"), float("-inf"), float("nan")])
+@pytest.mark.parametrize("dtype,dim,shared,lengths,new,at", [
+    # Requests of several new tokens (group 4), from tiles of 256 rows to fewer than 16, `at` a new token's place.
+    (torch.bfloat16, 128, 40, [290, 100, 44], [200, 37, 2], [130, 61, 70, 90, 200, 289]),
+    (torch.float16, 64, 0, [70, 9, 1], [70, 3, 1], [0, 7, 64, 65]),
+    # Requests shorter than the prefix, few and many: `at` is a shared position that some see.
+    (torch.bfloat16, 64, 500, [3, 130, 400, 520], None, [130, 400, 401, 499]),
+    (torch.float16, 128, 300, [10 + 7 * i for i in range(48)], None, [9, 10, 200, 290]),
+])
+def test_infinities_and_nan_where_only_others_look(dtype, dim, shared, lengths, new, at, odd, cuda_device):
+    """An odd V value reaches the rows that see its position and no others; an odd K value likewise."""
+    case = Case(lengths=lengths, shared=shared, new=new, dtype=dtype, dim=dim)
+    source = case.tables[case.source]
+
+    def slot(request, position):
+        row = source if position < shared else case.tables[request]
+        return int(row[position // case.page]) * case.page + position % case.page
+
+    for plane in (case.v, case.k):
+        kept = plane.clone()
+        for i, position in enumerate(at):
+            if plane is case.k and position == 0:
+                continue  # a row may see nothing else: 0 / 0 if its score is minus infinity
+            for request in range(len(lengths)):
+                if position < max(lengths[request], shared) and not (position < shared and request):
+                    plane[slot(request, position), i % 2, 3 * i + 1] = odd
+        got = case.run(cuda_device)
+        with np.errstate(invalid="ignore"):
+            want = case.want()
+        plane.copy_(kept)
+        out, lse = _np(got[0]), _np(got[1])
+        bad = ~np.isfinite(want[0])
+        assert bad.any() and not bad.all()
+        assert (np.isfinite(out) == ~bad).all() and (np.isfinite(lse) == np.isfinite(want[1])).all()
+        for values in (want[0], want[2], out):
+            values[bad] = 0.0
+        with np.errstate(invalid="ignore"):  # rows of an odd key have no tolerance to speak of
+            compare((torch.from_numpy(out), torch.from_numpy(lse)), want, dtype, float(case.v.double().abs().max()), dim)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_sharp_and_growing_scores(dtype, cuda_device):
     """Scores whose maximum grows along the tokens (rescaling at every tile) and nearly one-hot rows."""
