@@ -49,11 +49,13 @@ def _vector(tensor: torch.Tensor, name: str, count: int | None) -> int:
     return index_esize(tensor, name)
 
 
+def _end(tensor: torch.Tensor) -> int:
+    last = sum((n - 1) * s for n, s in zip(tensor.shape, tensor.stride()))
+    return tensor.data_ptr() + (last + 1) * tensor.element_size()
+
+
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
-    if not a.numel() or not b.numel():
-        return False
-    start, other = a.data_ptr(), b.data_ptr()
-    return (start < other + b.numel() * b.element_size()) and (other < start + a.numel() * a.element_size())
+    return bool(a.numel() and b.numel()) and a.data_ptr() < _end(b) and b.data_ptr() < _end(a)
 
 
 def extend_block_tables(block_tables: torch.Tensor, lengths: torch.Tensor, new_tokens: torch.Tensor,
@@ -145,8 +147,8 @@ def append_rows(rows, slot_map: torch.Tensor, planes) -> None:
     shape and dtype (e.g. the new tokens' K and V, and a layer's K and V planes).  Rows are
     contiguous within; all ``rows`` share one stride between tokens and all ``planes`` one
     between slots, so the views of a fused projection need no copy.  Tokens whose slot is
-    negative or not below ``slots`` are skipped; slots must be distinct.  The payload is
-    copied bit for bit.
+    negative or not below ``slots`` are skipped; slots must be distinct, planes too, and
+    ``rows`` must not lie in them.  The payload is copied bit for bit.
     """
     rows, planes = list(rows), list(planes)
     fast = torch_binding()

@@ -1461,9 +1461,10 @@ __device__ __forceinline__ void write_row(const AttentionParams& p, int n, int h
 // A weight of 0 does not keep an infinity or NaN out of a product: a V row that a query row does not see
 // but another of its tile does (a later token of its request, a shared position behind a short request) may
 // leave one in its sum.  Such a row is summed again over the positions it sees, by the eight lanes that join it;
-// its maximum and sum stand, they come from the scores alone.  If what it does not see is finite, nothing is done.
+// its maximum and sum stand, they come from the scores alone.  False, and nothing is written, if what it does not
+// see is finite.  Its query is read before its output is written: they may be the same memory.
 template <typename T, int kDim>
-__device__ __noinline__ void sum_again(const AttentionParams& p, int64_t b, const Request request, int n, int head, float top,
+__device__ __noinline__ bool sum_again(const AttentionParams& p, int64_t b, const Request request, int n, int head, float top,
                                        float scale) {
     constexpr int kVectors = kDim / (4 * kJoinLanes);
     const int lane = static_cast<int>(lane_id()) % kJoinLanes;
@@ -1502,7 +1503,7 @@ __device__ __noinline__ void sum_again(const AttentionParams& p, int64_t b, cons
         for (int v = 0; v < kVectors; ++v) odd |= !finite(row[v]);
         found = __any_sync(eight, odd);
     }
-    if (!found) return;
+    if (!found) return false;
     float4 query[kVectors], acc[kVectors];
     load(p.query, n * p.q_token + head * p.q_head, query);
 #pragma unroll
@@ -1529,6 +1530,7 @@ __device__ __noinline__ void sum_again(const AttentionParams& p, int64_t b, cons
         }
     }
     write_row<T, kDim>(p, n, head, lane, acc, scale);
+    return true;
 }
 
 // Eight lanes a row: the parts (m_i, l_i, O_i) of a row join as
@@ -1683,7 +1685,6 @@ __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_c
     }
     if (!active || mine_of) return;
     const float scale = bad ? NAN : (total == 0.f ? 0.f : 1.f / total);
-    write_row<T, kDim>(p, n, head, lane, acc, scale);
     if (p.lse && lane == 0) {
         p.lse[n * p.lse_token + head * p.lse_head] =
             bad ? NAN : (total == 0.f ? -INFINITY : (top + log2f(total)) * 0.69314718055994531f);
@@ -1691,9 +1692,11 @@ __global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_c
     bool odd = false;
 #pragma unroll
     for (int v = 0; v < kVectors; ++v) odd |= !finite(acc[v]);
-    if (__any_sync(0xffu << (lane_id() & ~7u), odd) && !bad && isfinite(total)) {
-        sum_again<T, kDim>(p, b, request, n, head, top, scale);
+    if (__any_sync(0xffu << (lane_id() & ~7u), odd) && !bad && isfinite(total) &&
+        sum_again<T, kDim>(p, b, request, n, head, top, scale)) {
+        return;
     }
+    write_row<T, kDim>(p, n, head, lane, acc, scale);
 }
 
 // ---------------------------------------------------------------- host side

@@ -440,6 +440,13 @@ bool head_rows_ok(const at::Tensor& t, bool apart) {
 
 int64_t stride_of(const at::Tensor& t, int d) { return t.size(d) > 1 ? t.stride(d) : 0; }
 
+// Entries of `width` elements, [tokens, heads], of which no two overlap.
+bool entries_apart(const at::Tensor& t, int64_t width) {
+    const int64_t tokens = t.size(0), heads = t.size(1), token = stride_of(t, 0), head = stride_of(t, 1);
+    if ((heads > 1 && head < width) || (tokens > 1 && token < width)) return false;
+    return tokens <= 1 || heads <= 1 || token >= (heads - 1) * head + width || head >= (tokens - 1) * token + width;
+}
+
 // (status, out, lse or None)
 py::tuple shared_prefix_attention(const at::Tensor& query, const at::Tensor& k_plane, const at::Tensor& v_plane,
                                   const at::Tensor& tables, const at::Tensor& lengths, int64_t page_size,
@@ -461,10 +468,11 @@ py::tuple shared_prefix_attention(const at::Tensor& query, const at::Tensor& k_p
     }
     if (out && (out->scalar_type() != dtype || out->sizes() != query.sizes())) return status(kNotHandled);
     if (!head_rows_ok(query, false) || !head_rows_ok(k_plane, true) || !head_rows_ok(v_plane, true) ||
-        (out && !head_rows_ok(*out, true))) {
+        (out && (!head_rows_ok(*out, true) || !entries_apart(*out, dim)))) {
         return status(kNotHandled);
     }
-    if (lse && (lse->scalar_type() != at::kFloat || lse->dim() != 2 || lse->size(0) != tokens || lse->size(1) != heads)) {
+    if (lse && (lse->scalar_type() != at::kFloat || lse->dim() != 2 || lse->size(0) != tokens || lse->size(1) != heads ||
+                !entries_apart(*lse, 1))) {
         return status(kNotHandled);
     }
     if (page_size < 1 || page_size > kInt32Max || tables.dim() != 2 || (tables.size(1) > 1 && tables.stride(1) != 1) ||

@@ -36,9 +36,21 @@ def _rows_ok(tensor: torch.Tensor, name: str) -> None:
         raise ValueError(f"{name} must have 16-byte aligned rows")
 
 
+def _apart(shape, strides, width: int, name: str) -> None:
+    """Entries of ``width`` elements that do not overlap, the heads of a token side by side or the tokens of a head."""
+    (tokens, heads), (token, head) = shape, _strides_of(shape, strides)
+    if (heads > 1 and head < width) or (tokens > 1 and token < width) or (
+            tokens > 1 and heads > 1 and token < (heads - 1) * head + width and head < (tokens - 1) * token + width):
+        raise ValueError(f"{name} rows overlap")
+
+
+def _strides_of(shape, strides) -> tuple[int, int]:
+    return tuple(s if n > 1 else 0 for n, s in zip(shape, strides))
+
+
 def _strides(tensor: torch.Tensor) -> tuple[int, int]:
     """Strides of the first two dimensions; 0 for one of a single entry."""
-    return tuple(s if n > 1 else 0 for n, s in zip(tensor.shape[:2], tensor.stride()[:2]))
+    return _strides_of(tensor.shape[:2], tensor.stride()[:2])
 
 
 def _outputs(query, out, lse, return_lse):
@@ -74,11 +86,13 @@ def _bind(query, k_plane, v_plane, block_tables, lengths, page_size, shared_toke
     for tensor, name in ((k_plane, "k_plane"), (v_plane, "v_plane"), (out, "out")):
         if any(n > 1 and s < dim for n, s in zip(tensor.shape[:2], tensor.stride()[:2])):
             raise ValueError(f"{name} rows overlap")
+    _apart(out.shape[:2], out.stride()[:2], dim, "out")
     if lse is not None:
         if lse.dtype != torch.float32:
             raise TypeError("lse must be a float32 tensor")
         if lse.shape != (tokens, query_heads):
             raise ValueError("lse must be [tokens, query_heads]")
+        _apart(lse.shape, lse.stride(), 1, "lse")
     if type(page_size) is not int or not 1 <= page_size < 1 << 31:
         raise ValueError("page_size outside the supported range")
     if block_tables.dim() != 2 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
@@ -139,17 +153,19 @@ def shared_prefix_attention(query: torch.Tensor, k_plane: torch.Tensor, v_plane:
     ``query_starts`` request b has the one new token ``query[b]``; with it (int32 / int64
     [requests + 1], ascending) its new tokens are ``query[query_starts[b]:query_starts[b + 1]]``,
     the last of the request, and each sees the tokens up to itself.  Query tokens of no
-    request are left as they were in ``out`` and ``lse``.
+    request are left as they were in ``out`` and ``lse`` (``out`` may be ``query`` itself).
 
     Position t of request b is in slot ``page * page_size + t % page_size`` with ``page =
     block_tables[row, t // page_size]``, where ``row`` is ``source_row`` for the first
     ``shared_tokens`` positions and ``rows[b]`` (default b) behind them.  A position without a
     slot (a negative page, one outside the planes, past the table) is skipped.  A query token
-    that sees no position gets zeros and a log-sum-exp of minus infinity.
+    that sees no position gets zeros and a log-sum-exp of minus infinity.  Infinities and NaN
+    reach the query tokens that see their position, no others.
 
-    One call takes up to ``ATTENTION_MAX_ROW_TILES`` (1536) row tiles: one per request and 256 query rows of a KV head.
-    ``scale`` defaults to ``1 / sqrt(dim)``; ``lse`` is float32 [tokens, query_heads], the natural
-    logarithm of the sum of the exponentials.  Scores, maxima, sums and outputs are held in 32 bits.
+    One call takes up to ``ATTENTION_MAX_ROW_TILES`` (1536) row tiles: one per request and one per 256
+    query rows of a KV head.  ``scale`` defaults to ``1 / sqrt(dim)``; ``lse`` is float32
+    [tokens, query_heads], the natural logarithm of the sum of the exponentials.  Scores, maxima,
+    sums and outputs are held in 32 bits.  For serving: no gradients flow through it.
     """
     fast = torch_binding() if all(type(x) is int for x in (page_size, shared_tokens, source_row)) else None
     if fast is not None:

@@ -241,6 +241,56 @@ def test_infinities_and_nan_where_only_others_look(dtype, dim, shared, lengths, 
             compare((torch.from_numpy(out), torch.from_numpy(lse)), want, dtype, float(case.v.double().abs().max()), dim)
 
 
+def test_output_in_the_query(cuda_device):
+    """`out` may be `query` itself, rows that are summed again included; lse transposed."""
+    from ekv_b200.prefix_attention import shared_prefix_attention
+
+    case = Case(lengths=[60, 20, 300], new=[50, 3, 1], shared=30, tail=4)
+    slot = int(case.tables[0][50 // 16]) * 16 + 50 % 16
+    case.v[slot, 1, 7] = float("nan")  # a new token of request 0, seen by its last ten
+    apart = case.run(cuda_device)
+    query = case.query.to(cuda_device)
+    lse = torch.full((8, case.query.shape[0]), MARK, device=cuda_device).t()
+    out, _ = shared_prefix_attention(query, *(t.to(cuda_device) for t in (case.k, case.v, case.tables, case.lengths)),
+                                     page_size=16, shared_tokens=30, source_row=case.source, lse=lse,
+                                     query_starts=case.starts.to(cuda_device), out=query)
+    assert out.data_ptr() == query.data_ptr()
+    assert int(torch.isnan(out[:54]).sum()) == 10 * 4 and torch.equal(out[54:].cpu(), case.query[54:])
+    torch.testing.assert_close(out[:54], apart[0][:54], rtol=0, atol=0, equal_nan=True)
+    assert torch.equal(lse, apart[1])
+
+
+def test_more_query_heads_than_a_tile_has_rows(cuda_device):
+    check(Case(lengths=[70, 200], new=[3, 1], shared=50, heads=1, group=300, dim=64), cuda_device)
+
+
+def test_most_requests_of_one_call(cuda_device):
+    """1530 requests and their six tiles of 256 query rows: as many as one call takes."""
+    check(Case(lengths=[40 + b % 7 for b in range(1530)], shared=40, heads=1, group=1, dim=64), cuda_device)
+
+
+def test_calls_captured_without_a_plan(cuda_device):
+    """The function itself in two graphs of one pool, replayed in turn."""
+    from ekv_b200.prefix_attention import shared_prefix_attention
+
+    cases = [Case(lengths=[210 + 30 * b for b in range(6)], shared=200, seed=s) for s in (3, 4)]
+    dev = [[t.to(cuda_device) for t in (c.query, c.k, c.v, c.tables, c.lengths)] for c in cases]
+
+    def run(i):
+        return shared_prefix_attention(*dev[i], page_size=16, shared_tokens=200, source_row=6, return_lse=True)
+
+    run(0)
+    graphs, results, pool = [], [], torch.cuda.graph_pool_handle()
+    for i in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[i], pool=pool):
+            results.append(run(i))
+    for _ in range(2):
+        for i, c in enumerate(cases):
+            graphs[i].replay()
+            compare(results[i], c.want(), c.dtype, float(c.v.double().abs().max()), 128)
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 def test_sharp_and_growing_scores(dtype, cuda_device):
     """Scores whose maximum grows along the tokens (rescaling at every tile) and nearly one-hot rows."""

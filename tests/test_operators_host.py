@@ -64,6 +64,10 @@ def test_extend_refuses_outputs_that_do_not_match(host):
             host[0].extend_block_tables(**args, out=good._replace(**{name: tensor}))
     with pytest.raises(TypeError):
         host[0].extend_block_tables(**args, out=good._replace(positions=torch.zeros(8, dtype=torch.int64)))
+    wide = torch.zeros((3, 32), dtype=torch.int32)
+    with pytest.raises(ValueError, match="positions overlaps an input"):  # in the table's last row
+        host[0].extend_block_tables(**{**args, "block_tables": wide[:, 4:8]},
+                                    out=good._replace(positions=wide[2, :8]))
 
 
 @pytest.mark.parametrize("rows,slot_map,planes,error,match", [
@@ -102,7 +106,10 @@ def _attend():
     (dict(k_plane=torch.zeros(1, 2, 64, dtype=torch.bfloat16).expand(32, 2, 64)), ValueError, "overlap"),
     (dict(out=torch.zeros(3, 4, 32, dtype=torch.bfloat16)), ValueError, "out must have"),
     (dict(out=torch.zeros(3, 4, 64)), TypeError, "share one dtype"),
+    (dict(out=torch.zeros(6 * 64, dtype=torch.bfloat16).as_strided((3, 4, 64), (64, 64, 1))), ValueError, "out rows overlap"),
     (dict(lse=torch.zeros(4, 3)), ValueError, "lse"),
+    (dict(lse=torch.zeros(1, 4).expand(3, 4)), ValueError, "lse rows overlap"),
+    (dict(lse=torch.zeros(6).as_strided((3, 4), (1, 1))), ValueError, "lse rows overlap"),
     (dict(lse=torch.zeros(3, 4).double()), TypeError, "float32"),
     (dict(page_size=0), ValueError, "page_size"),
     (dict(page_size=1 << 29), ValueError, "2\\^31"),
