@@ -1538,9 +1538,10 @@ __device__ __noinline__ bool sum_again(const AttentionParams& p, int64_t b, cons
 // of an item lie next to each other: a lane looks at each, first those of the row's prefix item, then
 // those of its own.  Bound by instructions for many rows (eight lanes a row take a quarter of what a warp
 // a row takes: 8 x 8001 prompts 20 us against 42); by the latency of dependent loads for few, so
-// then the four eights of a warp (kSplit) share one row's parts and join at the end.
+// then the four eights of a warp (kSplit) share one row's parts and join at the end.  Many rows: six blocks an
+// SM (eight, with less than 64 registers a thread, took 2 us more for 8192 rows of 128 requests).
 template <typename T, int kDim, int kSplit>
-__global__ void __launch_bounds__(32 * kJoinWarps) combine_kernel(const __grid_constant__ AttentionParams p) {
+__global__ void __launch_bounds__(32 * kJoinWarps, kSplit == 1 ? 6 : 1) combine_kernel(const __grid_constant__ AttentionParams p) {
     constexpr int kVectors = kDim / (4 * kJoinLanes);  // of four values, of a row, in a lane
     constexpr int kAtOnce = kSplit == 1 ? 2 : 4;       // parts whose loads are on their way together
     constexpr uint32_t kAll = 0xffffffffu;
