@@ -20,11 +20,11 @@
 // requests), so lengths may change under a captured graph and nothing is read back.
 //
 // attention_kernel, one tile: S = Q K^T and O += P V on the tensor cores (tcgen05, 128 rows, 32-bit sums
-// in tensor memory), a softmax thread per row between them.  The two halves of a tile follow one
-// another: the softmax of one runs beside the second product of the other and, right behind it, the first
+// in tensor memory), a softmax thread per row between them.  The two halves (64 positions) of a tile
+// follow one another: the softmax of one runs beside the second product of the other and, right behind it, the first
 // product of that half of the next tile, whose scores take the place of its weights.  (A first product of 64
 // columns runs at half the tensor cores' rate, since its 128 rows come from shared memory each time; waiting
-// for products of whole tiles cost more: 8 prompts of 8001 tokens 372 us against 343.)
+// for products of whole tiles cost more: 8 requests of up to 400 new tokens over 8001 shared ones 372 us against 343.)
 // Roles by warp: 0-3 and 4-7 softmax of the halves ("slots") 0 and 1 of a row tile; 8-11 copy the K rows,
 // 12-15 the V rows into swizzled shared memory (cp.async, 16 bytes a lane, whole rows; slots resolved
 // through the table, zeros for positions without one); 16 and 17 issue the products of slots 0 and 1
@@ -37,7 +37,7 @@
 // they are written); with few tiles, items alternate between the slots (kSingle).
 // What bounds it: the instructions of the softmax warps (128 x 256 exponentials a tile), beside which
 // eight copying warps run; the tensor cores are busy 40 % of the time.  256 requests of 64 heads over 32768
-// shared tokens and 1 to 256 own ones: 375 us for 279 GFLOP, 0.44 of the measured matrix peak.
+// shared tokens and up to 900 own ones: 375 us for 279 GFLOP, 0.44 of the measured matrix peak.
 //
 // The maximum a row's weights refer to is raised only when the scores' maximum passes it by 2^8
 // (kRaise), which makes rescaling O rare; weights are then at most 2^8.  They are rounded to the 16-bit type
@@ -1537,7 +1537,7 @@ __device__ __noinline__ bool sum_again(const AttentionParams& p, int64_t b, cons
 // sum 2^(m_i - m) O_i / sum 2^(m_i - m) l_i with m = max m_i.  The blocks (or workers) that may hold a part
 // of an item lie next to each other: a lane looks at each, first those of the row's prefix item, then
 // those of its own.  Bound by instructions for many rows (eight lanes a row take a quarter of what a warp
-// a row takes: 8 x 8001 prompts 20 us against 42); by the latency of dependent loads for few, so
+// a row takes: 8 prompts of up to 400 tokens, 51,000 rows, 20 us against 42); by the latency of dependent loads for few, so
 // then the four eights of a warp (kSplit) share one row's parts and join at the end.  Many rows: six blocks an
 // SM (eight, with less than 64 registers a thread, took 2 us more for 8192 rows of 128 requests).
 template <typename T, int kDim, int kSplit>
