@@ -610,7 +610,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             barrier_init(k_empty(s), 2);  // both slots, or one of them and the warp that passes on
             barrier_init(v_landed(s), 16 * kGatherWarps);
             barrier_init(v_full(s), 1);
-            barrier_init(v_empty(s), 2);
+            barrier_init(v_empty(s), 2);  // both slots
         }
         for (int s = 0; s < 2; ++s) {
             barrier_init(q_landed(s), kRows);
@@ -959,19 +959,31 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             const uint64_t all_values = shared_operand(base + L::kValues, L::kBlock);
             uint32_t uses = 0, q_uses = 0, p_uses = 0;
             bool fine = true;
+            const auto parity = [&](uint32_t use) { return (use / L::kStages) & 1; };
+            // A barrier tells apart only the phase under way and the one before, so a slot waits for every V
+            // tile in turn and lets those go that the other slot multiplies.  (K tiles need no such wait: the
+            // queries of an item are passed on behind the K tiles of the items before.)
+            const auto let_go = [&](uint32_t use) {
+                if (!barrier_wait(v_full(use % L::kStages), parity(use), failed)) return false;
+                barrier_arrive(v_empty(use % L::kStages));
+                return true;
+            };
             while (fine && next(true)) {
                 const bool pair = item.mode == kPair;
                 const uint32_t before = uses - item.low;  // tile t of the item is the block's tile before + t
+                const uint32_t first_use = uses;
                 uses += item.high - item.low;
                 if (item.mode == kSingle) {
                     const int owner = turn;
                     turn ^= 1;
-                    if (owner != slot) continue;
+                    if (owner != slot) {
+                        for (uint32_t use = first_use; fine && use < uses; ++use) fine = let_go(use);
+                        continue;
+                    }
                 }
                 const int low = item.low + (pair ? slot : 0), high = item.high, step = pair ? 2 : 1;
                 if (!(fine = barrier_wait(q_full(slot), q_uses & 1, failed))) break;
                 ++q_uses;
-                const auto parity = [&](uint32_t use) { return (use / L::kStages) & 1; };
                 // Scores of half a tile; then, as soon as the weights of a half are there, their product
                 // with V, and right behind it the scores of that half of the next tile, so that
                 // the softmax of one half runs beside the products of the other.
@@ -994,6 +1006,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                     const int stage = use % L::kStages;
                     const uint32_t next_use = use + step;
                     const bool more = t + step < high;
+                    if (pair && slot && !(fine = let_go(use - 1))) break;
                     if (!(fine = barrier_wait(v_full(stage), parity(use), failed))) break;
 #pragma unroll 1
                     for (int half = 0; half < 2; ++half) {
@@ -1016,7 +1029,10 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                         if (half) mma_commit(k_empty(next_use % L::kStages));
                     }
                     if (!fine) break;
+                    if (pair && !slot && t + 1 < high && !(fine = let_go(use + 1))) break;
                 }
+                // The last of an odd number of tiles is slot 0's.
+                if (fine && pair && slot && (high - item.low) % 2) fine = let_go(uses - 1);
                 if (fine) mma_commit(o_full(slot));
             }
             // Nothing may still use tensor memory when it is freed, whatever happened above.
@@ -1040,8 +1056,8 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                     const uint32_t parity = (uses / L::kStages) & 1;
                     fine = keys ? pass_on(k_landed(stage), k_full(stage), parity)
                                 : pass_on(v_landed(stage), v_full(stage), parity);
-                    // For the slot that has no use for the tile.
-                    if (fine && its.mode != kBoth) barrier_arrive(keys ? k_empty(stage) : v_empty(stage));
+                    // For the slot that has no use for the K tile.
+                    if (fine && keys && its.mode != kBoth) barrier_arrive(k_empty(stage));
                 }
                 return fine;
             };

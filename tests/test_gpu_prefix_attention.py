@@ -241,6 +241,22 @@ def test_infinities_and_nan_where_only_others_look(dtype, dim, shared, lengths, 
             compare((torch.from_numpy(out), torch.from_numpy(lse)), want, dtype, float(case.v.double().abs().max()), dim)
 
 
+@pytest.mark.parametrize("dim,page", [(128, 1), (64, 1), (128, 16), (64, 3)])
+def test_many_short_items(dim, page, cuda_device):
+    """Requests of 17 to 72 new tokens between decoding ones: items of one to four tiles that take turns on the
+    two halves of a block, among larger ones, with holes in the table (whose rows take the slower copy)."""
+    gen = torch.Generator().manual_seed(9)
+    new = [21, 5, 0, 1, 0, 5, 2, 1, 0, 2, 5, 0, 5, 1, 1, 25, 41, 72, 1, 1, 17, 12, 5, 44, 5, 62, 1, 17, 0, 1, 5, 1, 5, 64, 1, 1, 1, 30]
+    own = torch.randint(0, 420, (len(new),), generator=gen).tolist()
+    case = Case(lengths=[max(70 + n, w) for n, w in zip(own, new)], shared=70, page=page, heads=8, group=5, dim=dim, new=new)
+    for holes in range(3):
+        case.tables[torch.rand(case.tables.shape, generator=gen) < 0.1 * holes] = -1
+        first = check(case, cuda_device)
+        for _ in range(4):
+            again = case.run(cuda_device)
+            assert torch.equal(first[0], again[0]) and torch.equal(first[1], again[1])
+
+
 def test_output_in_the_query(cuda_device):
     """`out` may be `query` itself, rows that are summed again included; lse transposed."""
     from ekv_b200.prefix_attention import shared_prefix_attention
