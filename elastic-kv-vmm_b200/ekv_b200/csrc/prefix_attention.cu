@@ -542,7 +542,7 @@ struct Layout {
     // Six of each stage, nine of each slot, two of each place in the item ring, one where the slots of a pair meet.
     static constexpr int kBarrierCount = 6 * kStages + 9 * 2 + 2 * kItemRing + 1;
     static constexpr uint32_t kTail = kBarriers + kBarrierCount * 8;
-    static constexpr uint32_t kBytes = kTail + 16;  // tensor-memory address, failed flag
+    static constexpr uint32_t kBytes = kTail + 16;  // tensor-memory address, failed flag, V tiles passed on
 };
 
 template <typename T>
@@ -601,6 +601,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
     const auto drain = [&](int s) { return slot_barrier(8, s); };
     const auto item_full = [&](int i) { return barriers + 8 * (6 * L::kStages + 18 + i); };
     const auto item_empty = [&](int i) { return barriers + 8 * (6 * L::kStages + 18 + kItemRing + i); };
+    const uint32_t v_count = base + L::kTail + 8;  // V tiles that are passed on
     const uint32_t meet = barriers + 8 * (L::kBarrierCount - 1);
 
     if (threadIdx.x == 0) {
@@ -610,7 +611,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             barrier_init(k_empty(s), 2);  // both slots, or one of them and the warp that passes on
             barrier_init(v_landed(s), 16 * kGatherWarps);
             barrier_init(v_full(s), 1);
-            barrier_init(v_empty(s), 2);  // both slots
+            barrier_init(v_empty(s), 2);
         }
         for (int s = 0; s < 2; ++s) {
             barrier_init(q_landed(s), kRows);
@@ -629,6 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             barrier_init(item_empty(i), 8 + kGatherWarps + 3);  // every warp but the one that walks
         }
         *failed = 0;
+        count_store(v_count, 0);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_shared();
     }
@@ -960,26 +962,21 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             uint32_t uses = 0, q_uses = 0, p_uses = 0;
             bool fine = true;
             const auto parity = [&](uint32_t use) { return (use / L::kStages) & 1; };
-            // A barrier tells apart only the phase under way and the one before, so a slot waits for every V
-            // tile in turn and lets those go that the other slot multiplies.  (K tiles need no such wait: the
-            // queries of an item are passed on behind the K tiles of the items before.)
-            const auto let_go = [&](uint32_t use) {
-                if (!barrier_wait(v_full(use % L::kStages), parity(use), failed)) return false;
-                barrier_arrive(v_empty(use % L::kStages));
-                return true;
+            // A barrier tells apart only the phase under way and the one before, but a slot may come to a V tile
+            // while one of the other slot's is awaited at the same stage; so it first sees that one passed on.
+            // (K tiles need no such wait: an item's queries are passed on behind the K tiles of the items before.)
+            const auto values_there = [&](uint32_t use) {
+                return (use < L::kStages || count_wait(v_count, use - L::kStages + 1, failed)) &&
+                       barrier_wait(v_full(use % L::kStages), parity(use), failed);
             };
             while (fine && next(true)) {
                 const bool pair = item.mode == kPair;
                 const uint32_t before = uses - item.low;  // tile t of the item is the block's tile before + t
-                const uint32_t first_use = uses;
                 uses += item.high - item.low;
                 if (item.mode == kSingle) {
                     const int owner = turn;
                     turn ^= 1;
-                    if (owner != slot) {
-                        for (uint32_t use = first_use; fine && use < uses; ++use) fine = let_go(use);
-                        continue;
-                    }
+                    if (owner != slot) continue;
                 }
                 const int low = item.low + (pair ? slot : 0), high = item.high, step = pair ? 2 : 1;
                 if (!(fine = barrier_wait(q_full(slot), q_uses & 1, failed))) break;
@@ -1006,8 +1003,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                     const int stage = use % L::kStages;
                     const uint32_t next_use = use + step;
                     const bool more = t + step < high;
-                    if (pair && slot && !(fine = let_go(use - 1))) break;
-                    if (!(fine = barrier_wait(v_full(stage), parity(use), failed))) break;
+                    if (!(fine = values_there(use))) break;
 #pragma unroll 1
                     for (int half = 0; half < 2; ++half) {
                         const uint64_t values = all_values + stage * (L::kOperand >> 4) + half * (64 * 128 >> 4);
@@ -1029,10 +1025,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                         if (half) mma_commit(k_empty(next_use % L::kStages));
                     }
                     if (!fine) break;
-                    if (pair && !slot && t + 1 < high && !(fine = let_go(use + 1))) break;
                 }
-                // The last of an odd number of tiles is slot 0's.
-                if (fine && pair && slot && (high - item.low) % 2) fine = let_go(uses - 1);
                 if (fine) mma_commit(o_full(slot));
             }
             // Nothing may still use tensor memory when it is freed, whatever happened above.
@@ -1056,8 +1049,9 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                     const uint32_t parity = (uses / L::kStages) & 1;
                     fine = keys ? pass_on(k_landed(stage), k_full(stage), parity)
                                 : pass_on(v_landed(stage), v_full(stage), parity);
-                    // For the slot that has no use for the K tile.
-                    if (fine && keys && its.mode != kBoth) barrier_arrive(k_empty(stage));
+                    if (fine && !keys) count_store(v_count, uses + 1);
+                    // For the slot that has no use for the tile.
+                    if (fine && its.mode != kBoth) barrier_arrive(keys ? k_empty(stage) : v_empty(stage));
                 }
                 return fine;
             };

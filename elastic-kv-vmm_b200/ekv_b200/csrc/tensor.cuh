@@ -59,6 +59,26 @@ __device__ __forceinline__ bool barrier_wait(uint32_t barrier, uint32_t parity, 
     return true;
 }
 
+// A count in shared memory that one thread raises, and a wait until it is at least `target`, bounded as above.
+__device__ __forceinline__ void count_store(uint32_t address, uint32_t value) {
+    asm volatile("st.release.cta.shared::cta.b32 [%0], %1;" ::"r"(address), "r"(value) : "memory");
+}
+__device__ __forceinline__ bool count_wait(uint32_t address, uint32_t target, volatile uint32_t* failed) {
+    uint64_t begin = 0;
+#pragma unroll 1
+    while (true) {
+        uint32_t value;
+        asm volatile("ld.acquire.cta.shared::cta.b32 %0, [%1];" : "=r"(value) : "r"(address) : "memory");
+        if (value >= target) return true;
+        const uint64_t now = device_nanoseconds();
+        if (!begin) begin = now;
+        if (*failed || now - begin > kWaitLimit) {
+            *failed = 1;
+            return false;
+        }
+    }
+}
+
 // ---------------------------------------------------------------- proxies and asynchronous copies
 
 __device__ __forceinline__ void fence_async_shared() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
