@@ -1817,7 +1817,8 @@ extern "C" int ekv_shared_prefix_attention(
         require(dtype == EKV_BF16 || dtype == EKV_FP16, "dtype must be EKV_BF16 or EKV_FP16");
         check_shape(tokens, batch, query_heads, kv_heads, head_dim);
         require(page_size >= 1 && page_size <= INT32_MAX, "page_size outside [1, 2^31)");
-        require(table_width <= INT32_MAX / page_size, "a table row covers more than 2^31 - 1 positions");
+        // The end of the last tile is held in 32 bits too.
+        require(table_width <= (INT32_MAX - 255) / page_size, "a table row covers more than 2^31 - 256 positions");
         require(shared_tokens >= 0 && shared_tokens <= table_width * page_size,
                 "shared_tokens outside the table's positions");
         require(!shared_tokens || (source_row >= 0 && source_row < table_rows), "source row is outside the block table");

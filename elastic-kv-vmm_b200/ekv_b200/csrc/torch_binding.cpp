@@ -476,7 +476,7 @@ py::tuple shared_prefix_attention(const at::Tensor& query, const at::Tensor& k_p
         return status(kNotHandled);
     }
     if (page_size < 1 || page_size > kInt32Max || tables.dim() != 2 || (tables.size(1) > 1 && tables.stride(1) != 1) ||
-        !index_size(tables) || tables.size(1) > kInt32Max / page_size || shared_tokens < 0 ||
+        !index_size(tables) || tables.size(1) > (kInt32Max - 255) / page_size || shared_tokens < 0 ||
         shared_tokens > tables.size(1) * page_size ||
         (shared_tokens && (source_row < 0 || source_row >= tables.size(0))) || lengths.dim() != 1) {
         return status(kNotHandled);

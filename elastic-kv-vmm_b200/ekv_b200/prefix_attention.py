@@ -99,8 +99,8 @@ def _bind(query, k_plane, v_plane, block_tables, lengths, page_size, shared_toke
         raise ValueError("block_tables must be [rows, width] with contiguous rows")
     table_es = index_esize(block_tables, "block_tables")
     table_rows, table_width = block_tables.shape
-    if table_width * page_size >= 1 << 31:
-        raise ValueError("a table row covers more than 2^31 - 1 positions")
+    if table_width * page_size > (1 << 31) - 256:
+        raise ValueError("a table row covers more than 2^31 - 256 positions")
     if type(shared_tokens) is not int or not 0 <= shared_tokens <= table_width * page_size:
         raise ValueError("shared_tokens outside the table's positions")
     if type(source_row) is not int or (shared_tokens and not 0 <= source_row < table_rows):
@@ -162,10 +162,11 @@ def shared_prefix_attention(query: torch.Tensor, k_plane: torch.Tensor, v_plane:
     that sees no position gets zeros and a log-sum-exp of minus infinity.  Infinities and NaN
     reach the query tokens that see their position, no others.
 
-    One call takes up to ``ATTENTION_MAX_ROW_TILES`` (1536) row tiles: one per request and one per 256
-    query rows of a KV head.  ``scale`` defaults to ``1 / sqrt(dim)``; ``lse`` is float32
-    [tokens, query_heads], the natural logarithm of the sum of the exponentials.  Scores, maxima,
-    sums and outputs are held in 32 bits.  For serving: no gradients flow through it.
+    A table row covers up to 2^31 - 256 positions.  One call takes up to
+    ``ATTENTION_MAX_ROW_TILES`` (1536) row tiles: one per request and one per 256 query rows of a
+    KV head.  ``scale`` defaults to ``1 / sqrt(dim)``; ``lse`` is float32 [tokens, query_heads],
+    the natural logarithm of the sum of the exponentials.  Scores, maxima, sums and outputs are
+    held in 32 bits.  For serving: no gradients flow through it.
     """
     fast = torch_binding() if all(type(x) is int for x in (page_size, shared_tokens, source_row)) else None
     if fast is not None:

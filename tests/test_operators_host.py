@@ -113,6 +113,7 @@ def _attend():
     (dict(lse=torch.zeros(3, 4).double()), TypeError, "float32"),
     (dict(page_size=0), ValueError, "page_size"),
     (dict(page_size=1 << 29), ValueError, "2\\^31"),
+    (dict(block_tables=torch.zeros((3, 1), dtype=torch.int32), page_size=(1 << 31) - 255), ValueError, "2\\^31 - 256"),
     (dict(shared_tokens=17), ValueError, "shared_tokens"),
     (dict(shared_tokens=-1), ValueError, "shared_tokens"),
     (dict(source_row=3), ValueError, "source row"),
