@@ -74,7 +74,7 @@ def extend_block_tables(block_tables: torch.Tensor, lengths: torch.Tensor, new_t
     ``block_tables`` is written in place (only the entries of taken pages); nothing else
     among the inputs changes, so the step can be repeated.  Active requests must have
     distinct rows.  ``out`` takes the tensors of an earlier result again; they must not
-    overlap the inputs (copy ``out.lengths`` to the next step's lengths instead).
+    overlap the inputs or one another (copy ``out.lengths`` to the next step's lengths instead).
     """
     fast = torch_binding() if out is None and type(page_size) is int and type(max_tokens) is int else None
     if fast is not None:
@@ -118,6 +118,9 @@ def extend_block_tables(block_tables: torch.Tensor, lengths: torch.Tensor, new_t
             _vector(tensor, name, count)
             if any(_overlap(tensor, t) for t in inputs):
                 raise ValueError(f"{name} overlaps an input")
+        spans = sorted((tensor.data_ptr(), _end(tensor)) for tensor in out if tensor.numel())
+        if any(end > start for (_, end), (start, _) in zip(spans, spans[1:])):
+            raise ValueError("the tensors of out overlap")
     call(
         "ekv_extend_block_tables",
         block_tables.data_ptr(), block_tables.shape[0], block_tables.shape[1], block_tables.stride(0),

@@ -70,6 +70,18 @@ def test_extend_refuses_outputs_that_do_not_match(host):
                                     out=good._replace(positions=wide[2, :8]))
 
 
+@pytest.mark.parametrize("change", [
+    lambda flat: dict(positions=flat[8:16]),    # the slot map's
+    lambda flat: dict(positions=flat[15:23]),   # its last entry
+    lambda flat: dict(pages_used=flat[3:4]),    # the starts' last entry
+])
+def test_extend_refuses_outputs_that_overlap_one_another(change, host):
+    flat = torch.zeros(64, dtype=torch.int32)
+    good = host[0].TableExtension(flat[:4], flat[8:16], flat[16:24], flat[24:27], flat[27:28])
+    with pytest.raises(ValueError, match="tensors of out overlap"):
+        host[0].extend_block_tables(**_tables(), out=good._replace(**change(flat)))
+
+
 @pytest.mark.parametrize("rows,slot_map,planes,error,match", [
     ([torch.zeros(3, 2, 8)], torch.zeros(3, dtype=torch.int32), [], ValueError, "length"),
     ([torch.zeros(3, 2, 8)] * 257, torch.zeros(3, dtype=torch.int32), [torch.zeros(5, 2, 8)] * 257, ValueError, "MAX_PLANES"),
