@@ -166,7 +166,7 @@ __global__ void __launch_bounds__(kTableThreads) extend_tables_kernel(const __gr
         }
         tokens_before += tile_tokens;
         pages_before += tile_pages;
-        open = !closed;
+        open = open && !closed;  // a pass behind the closing one grants nothing, so none in it is refused
         __syncthreads();
     }
     for (int64_t t = (tokens_before > begin ? tokens_before : begin) + threadIdx.x; t < end; t += kTableThreads) {

@@ -182,3 +182,22 @@ def test_refusals_on_the_device(cuda_device):
         append_rows([torch.zeros((2, 2, 8), device=cuda_device).half()], two, [plane])
     with pytest.raises(ValueError, match="overlap"):
         append_rows([torch.zeros((2, 2, 8), device=cuda_device)], two, [plane[:1].expand(4, 2, 8)])
+
+
+@pytest.mark.parametrize("short", ["pages", "tokens"])
+@pytest.mark.parametrize("requests,closing", [(2049, 500), (2049, 1024), (2049, 2048), (3100, 1023), (3100, 1500),
+                                              (5000, 3), (5000, 2500), (5000, 4999)])
+def test_nothing_is_granted_behind_a_large_request(short, requests, closing, cuda_device):
+    """One request needs more than is left and the small ones behind it would not: they get nothing either,
+    however many passes of 1024 requests lie between."""
+    page = 4
+    tables, lengths, new, free, rows = _extend_case(requests + closing, requests, page, 64, 100, 3, 4 * requests)
+    new[closing] = 120
+    need = lambda n: int((-(-(lengths + new) // page) + -lengths // page)[:n].sum())  # noqa: E731
+    if short == "pages":
+        free, most = free[:need(closing) + 20], int(new.sum())
+    else:
+        most = int(new[:closing].sum()) + 100
+    got = _check(cuda_device, tables, lengths, new, free, rows, page, most)
+    assert int(got.query_starts[-1]) == int(new[:closing].sum()) and int(got.pages_used) == need(closing)
+    np.testing.assert_array_equal(got.lengths.cpu().numpy()[closing:], lengths[closing:])
