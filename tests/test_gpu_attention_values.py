@@ -1,0 +1,58 @@
+"""Shared-prefix attention on the device: values that the sums have to hold.
+
+Every comparison here also asks that a result is finite where the definition is (a comparison with NaN
+is false, so an error bound alone lets one pass).
+"""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import prefix_attention as opa
+from test_gpu_prefix_attention import E, MARK, Case, compare
+
+pytestmark = pytest.mark.gpu
+
+# What each takes through the kernels: requests of few rows alone; a prefix in tiles of up to 128 rows and
+# of more; new tokens of 17 rows and more, up to several tiles of rows.
+SHAPES = {
+    "decode": dict(lengths=[900, 65, 2049], shared=0, group=4),
+    "decode, 16 rows": dict(lengths=[700, 1300], shared=0, group=16),
+    "short prefix, few rows": dict(lengths=[1030, 1025], shared=1024, group=4),
+    "prefix, 48 rows": dict(lengths=[1290 + 3 * b for b in range(12)], shared=1280, group=4),
+    "prefix, 320 rows": dict(lengths=[1025 + b for b in range(40)], shared=1024, group=8),
+    "drafts": dict(lengths=[400, 333, 290], new=[5, 5, 5], shared=256, group=4),
+    "prompts": dict(lengths=[700, 500, 900], new=[130, 70, 300], shared=200, group=3),
+    "prompts, no prefix": dict(lengths=[300, 20, 129], new=[300, 20, 129], shared=0, group=2),
+}
+
+
+def _np(tensor):
+    return tensor.detach().double().cpu().numpy()
+
+
+def _slots(case, request, count):
+    """Slots of the first ``count`` positions of a request."""
+    position, slots = np.arange(count), case.k.shape[0]
+    own = opa.slots_of(case.tables[request].numpy(), position, case.page, slots)
+    donor = opa.slots_of(case.tables[case.source].numpy(), position, case.page, slots)
+    return torch.from_numpy(np.where(position < case.shared, donor, own))
+
+
+def finite_where_defined(got, want):
+    out, lse = _np(got[0]), _np(got[1])
+    held = ~np.isnan(want[0]).all((1, 2))
+    assert np.isfinite(out[held]).all()
+    assert (np.isfinite(lse[held]) == np.isfinite(want[1][held])).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_results_are_finite(shape, dim, dtype, cuda_device):
+    case = Case(**SHAPES[shape], heads=2, dim=dim, dtype=dtype, tail=3 if "new" in SHAPES[shape] else 0)
+    got, want = case.run(cuda_device), case.want()
+    finite_where_defined(got, want)
+    compare(got, want, dtype, float(case.v.double().abs().max()), dim)
