@@ -827,11 +827,14 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
             tensor_fence_after();
             float sum = total.x + total.y, factor = 1.f, other = 0.f;
             if (pair) {
-                // The slots exchange their maxima and sums; each then joins half of the columns.
+                // The slots exchange their maxima and sums; each then joins half of the columns, reading the other
+                // slot's too: what that one's products and rescaling have written lies before the meeting.
                 stats[slot * kRows + r] = make_float2(top, sum);
+                tensor_fence_before();
                 __syncwarp();
                 if (lane == 0) barrier_arrive(meet);
                 if (!__all_sync(0xffffffffu, barrier_wait(meet, meetings & 1, failed))) goto finish;
+                tensor_fence_after();
                 ++meetings;
                 const float2 its = stats[(slot ^ 1) * kRows + r];
                 const float higher = fmaxf(top, its.x);

@@ -56,3 +56,22 @@ def test_results_are_finite(shape, dim, dtype, cuda_device):
     got, want = case.run(cuda_device), case.want()
     finite_where_defined(got, want)
     compare(got, want, dtype, float(case.v.double().abs().max()), dim)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_items_that_the_halves_of_a_block_share(dim, dtype, cuda_device):
+    """Items of 20 and 60 rows, eight tiles of them a block: its halves take the tiles in turn and each joins half of the
+    columns of both.  Scores grow along the positions, so that either half has rescaled its sums just before."""
+    case = Case(lengths=[9000, 8033, 9900], shared=4000, heads=8, group=20, dim=dim, dtype=dtype, page=64, spread=0.5)
+    for request, length in enumerate(case.lengths.tolist()):
+        slots = _slots(case, request, length)
+        ramp = torch.linspace(0.2, 8.0, length)[:, None, None]
+        head = case.query[request].reshape(8, 20, dim)[:, 0].float()
+        case.k[slots] = (case.k[slots].float() * 0.2 + head[None] * ramp).to(dtype)
+    got, want = case.run(cuda_device), case.want()
+    finite_where_defined(got, want)
+    compare(got, want, dtype, float(case.v.double().abs().max()), dim)
+    for _ in range(5):
+        again = case.run(cuda_device)
+        assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1])
