@@ -634,10 +634,11 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         fence_async_shared();
     }
-    if (warp == kIssueWarp) tensor_alloc(base + L::kTail, 512);
     grid_dependency_wait();
-    tensor_fence_before();
     allow_dependents();  // rows_kernel needs nothing of this one: its blocks begin where this one's leave room
+    // Behind the wait: a block of the kernel before may still need tensor memory on this SM.
+    if (warp == kIssueWarp) tensor_alloc(base + L::kTail, 512);
+    tensor_fence_before();
     build_plan(p, plan);  // ends with __syncthreads
     tensor_fence_after();
     const uint32_t tensor = *reinterpret_cast<volatile uint32_t*>(shared + L::kTail);

@@ -75,3 +75,36 @@ def test_items_that_the_halves_of_a_block_share(dim, dtype, cuda_device):
     for _ in range(5):
         again = case.run(cuda_device)
         assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1])
+
+
+def test_between_matrix_products(cuda_device):
+    """Calls right behind and before library products on one stream, eagerly and in a graph: tensor memory that either
+    holds is free again when the other takes it."""
+    from ekv_b200.prefix_attention import SharedPrefixAttention
+
+    case = Case(**SHAPES["prefix, 320 rows"], heads=2, dim=128)
+    dev = [t.to(cuda_device) for t in (case.query, case.k, case.v, case.tables, case.lengths)]
+    plan = SharedPrefixAttention(*dev, page_size=case.page, shared_tokens=case.shared, source_row=case.source, return_lse=True)
+    small, large = (torch.randn(n, n, device=cuda_device).bfloat16() for n in (512, 4096))
+
+    def step():
+        products = []
+        for matrix in (small, large, small):
+            products.append(matrix @ matrix)
+            plan()
+        return products
+
+    first = step()
+    want = plan.out.clone(), plan.lse.clone()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = step()
+    for _ in range(5):
+        again = step()
+        assert torch.equal(plan.out, want[0]) and torch.equal(plan.lse, want[1])
+        plan.out.zero_()
+        graph.replay()
+        assert torch.equal(plan.out, want[0]) and torch.equal(plan.lse, want[1])
+        for products in (again, captured):
+            assert all(torch.equal(a, b) for a, b in zip(products, first))
+    compare((plan.out, plan.lse), case.want(), case.dtype, float(case.v.double().abs().max()), 128)
