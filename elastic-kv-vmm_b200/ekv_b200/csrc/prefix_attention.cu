@@ -80,6 +80,10 @@ enum Mode { kSingle = 0, kBoth = 1, kPair = 2 };
 constexpr int kMaskRing = 16;
 constexpr int kItemRing = 8, kItemsAhead = 5;
 constexpr float kRaise = 8.f;
+// A row's maximum is a product of score and scale rounded to 32 bits, its weights are taken of the exact one.  Below
+// kLarge the two differ by 2^-5 at most; from there on, where they come to differ by more than an exponent holds, the
+// scores are rounded in the same way first.
+constexpr float kLarge = 1048576.f;
 
 struct AttentionParams {
     const void* query;
@@ -777,7 +781,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                             }
                         }
                         const float most = fmaxf(fmaxf(highs[0], highs[1]), fmaxf(highs[2], highs[3])) * p.scale_log2;
-                        const bool raise = present && (most > top + kRaise || (top == -INFINITY && most > -INFINITY));
+                        const bool raise = present && most - top > kRaise;  // exact where it matters, as top + kRaise is not
                         if (__any_sync(0xffffffffu, raise)) {
                             const float before = top;
                             if (raise) top = most;
@@ -801,6 +805,12 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                             }
                         }
                         const float shift = top == -INFINITY ? 0.f : -top;
+                        float scale = p.scale_log2;
+                        if (__any_sync(0xffffffffu, fabsf(shift) >= kLarge)) {
+#pragma unroll
+                            for (int j = 0; j < 64; ++j) s[j] = __float_as_uint(__fmul_rn(__uint_as_float(s[j]), scale));
+                            scale = 1.f;
+                        }
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
                             uint32_t weights[16];
@@ -808,7 +818,7 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                             for (int j = 0; j < 32; j += 2) {
                                 const int at = 32 * c + j;
                                 float2 x = fma2(make_float2(__uint_as_float(s[at]), __uint_as_float(s[at + 1])),
-                                                make_float2(p.scale_log2, p.scale_log2), make_float2(shift, shift));
+                                                make_float2(scale, scale), make_float2(shift, shift));
                                 x.x = exp2_approx(x.x);
                                 x.y = exp2_approx(x.y);
                                 total = add2(total, x);
@@ -1353,7 +1363,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) rows_kernel(const __grid_co
                         for (int i = 0; i < 4; ++i) {
                             const int at = m * 16 + (lane >> 2) + (i >> 1) * 8;
                             const bool visible = (seen_now >> at & 1u) && position + at < sees[n][i & 1];
-                            score[m][n][i] = visible ? score[m][n][i] * p.scale_log2 : -INFINITY;
+                            score[m][n][i] = visible ? __fmul_rn(score[m][n][i], p.scale_log2) : -INFINITY;
                             most[n][i & 1] = fmaxf(most[n][i & 1], score[m][n][i]);
                         }
                     }
@@ -1361,7 +1371,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) rows_kernel(const __grid_co
                     for (int j = 0; j < 2; ++j) {
 #pragma unroll
                         for (int d = 4; d < 32; d <<= 1) most[n][j] = fmaxf(most[n][j], __shfl_xor_sync(0xffffffffu, most[n][j], d));
-                        raise |= most[n][j] > top[n][j] + kRaise || (top[n][j] == -INFINITY && most[n][j] > -INFINITY);
+                        raise |= most[n][j] - top[n][j] > kRaise;
                     }
                 }
                 if (__any_sync(0xffffffffu, raise)) {
@@ -1533,7 +1543,7 @@ __device__ __noinline__ bool sum_again(const AttentionParams& p, int64_t b, cons
         }
 #pragma unroll
         for (int d = 1; d < kJoinLanes; d <<= 1) score += __shfl_xor_sync(eight, score, d);
-        const float weight = exp2_approx(score * p.scale_log2 - top);
+        const float weight = exp2_approx(__fmul_rn(score, p.scale_log2) - top);
         load(p.v_plane, slot * p.v_slot + kv_head * p.v_head, row);
 #pragma unroll
         for (int v = 0; v < kVectors; ++v) {

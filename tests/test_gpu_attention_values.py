@@ -108,3 +108,50 @@ def test_between_matrix_products(cuda_device):
         for products in (again, captured):
             assert all(torch.equal(a, b) for a, b in zip(products, first))
     compare((plan.out, plan.lse), case.want(), case.dtype, float(case.v.double().abs().max()), 128)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_scores_far_beyond_the_exponent(shape, dim, dtype, cuda_device):
+    """Scores of 2^30 to 2^32, exact in 32 bits and further apart than any rounding: the mean of V over the
+    positions of the largest.  (A maximum rounded to 32 bits and an exact score differ by up to 2^8 here.)"""
+    gen = torch.Generator().manual_seed(dim)
+    case = Case(**SHAPES[shape], heads=1, dim=dim, dtype=dtype)
+    case.query.zero_()
+    case.k.zero_()
+    case.query[..., :16] = 2.0 ** 15
+    values = (1 + torch.randint(1, 100, (case.k.shape[0], 1, 1), generator=gen) / 128) * 2.0 ** 15
+    values[torch.rand(values.shape, generator=gen) < 0.3] *= -1
+    case.k[..., :16] = values.to(dtype)
+    got, want = case.run(cuda_device, scale=0.125), case.want(scale=0.125)
+    finite_where_defined(got, want)
+    expected, lse, weight, _, seen = want
+    # Weights are 1 and 0: what is rounded are the sums and the result, and the maximum of lse.
+    tolerance = 2.0 ** -8 if dtype == torch.bfloat16 else 2.0 ** -11
+    tolerance = tolerance * np.abs(expected) + (2 * seen[:, None, None] + 8) * E * weight + 2.0 ** -25
+    assert (np.abs(_np(got[0]) - expected) <= tolerance).all()
+    assert (np.abs(_np(got[1]) - lse) <= 8 * E * np.abs(lse)).all()
+
+
+@pytest.mark.parametrize("shape", SHAPES)
+@pytest.mark.parametrize("power,dtype", [*((n, t) for n in (20, 24, 26, 27, 28, 30) for t in (torch.bfloat16, torch.float16)),
+                                         (34, torch.bfloat16)])
+def test_large_scores_stay_a_mean_of_v(power, shape, dtype, cuda_device):
+    """Scores about 2^power that grow by a step of their 32 bits from position to position: which of the last takes
+    the weight is rounding's choice, but the result is a mean of V."""
+    case = Case(**SHAPES[shape], heads=1, dim=64, dtype=dtype)
+    case.query.zero_()
+    case.k.zero_()
+    base, step = 2.0 ** (power // 2), max(2.0 ** (power - 23), 1.0)
+    case.query[..., 0], case.query[..., 1] = base, 1.0
+    case.k[..., 0] = 1.25 * 2.0 ** (power - power // 2)
+    for b, length in enumerate(case.lengths.tolist()):
+        case.k[_slots(case, b, length), :, 1] = (step * (torch.arange(length) % 250)[:, None]).clamp(max=60000).to(dtype)
+    got, want = case.run(cuda_device, scale=1.0), case.want(scale=1.0)
+    finite_where_defined(got, want)
+    largest = float(case.v.double().abs().max())
+    out = _np(got[0])
+    assert (np.abs(out) <= largest * (1 + 2.0 ** -7)).all(), np.abs(out).max()
+    # The maximum is the scores', off by the rounding of a sum of two, of the scale and of the product.
+    assert (np.abs(_np(got[1]) - want[1]) <= 8 * E * np.abs(want[1]) + 1e-3).all()
