@@ -41,7 +41,9 @@
 //
 // The maximum a row's weights refer to is raised only when the scores' maximum passes it by 2^8
 // (kRaise), which makes rescaling O rare; weights are then at most 2^8.  They are rounded to the 16-bit type
-// for the second product (its operand type); the row sum is taken of the unrounded ones.
+// for the second product (its operand type); the row sum is taken of the unrounded ones.  fp16 holds nothing below
+// 2^-25, so its weights are 2^7 times as large (kShift), at most 2^15: what is lost of a long flat tail is then below
+// 2^-32 of the maximum's weight.  Sums and outputs carry the factor up to the join, where it cancels.
 #include "tensor.cuh"
 
 #include <cuda_bf16.h>
@@ -554,6 +556,7 @@ struct Kind;
 template <>
 struct Kind<__nv_bfloat16> {
     static constexpr bool kBf16 = true;
+    static constexpr float kShift = 0.f, kFactor = 1.f;  // of the weights: 2^kShift
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&v);
@@ -565,6 +568,7 @@ struct Kind<__nv_bfloat16> {
 template <>
 struct Kind<__half> {
     static constexpr bool kBf16 = false;
+    static constexpr float kShift = 7.f, kFactor = 128.f;
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
         const __half2 v = __floats2half2_rn(a, b);
         return *reinterpret_cast<const uint32_t*>(&v);
@@ -804,12 +808,15 @@ __global__ void __launch_bounds__(kThreads, 1) attention_kernel(const __grid_con
                                 }
                             }
                         }
-                        const float shift = top == -INFINITY ? 0.f : -top;
-                        float scale = p.scale_log2;
+                        float shift = top == -INFINITY ? 0.f : Kind<T>::kShift - top, scale = p.scale_log2;
                         if (__any_sync(0xffffffffu, fabsf(shift) >= kLarge)) {
+                            const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
-                            for (int j = 0; j < 64; ++j) s[j] = __float_as_uint(__fmul_rn(__uint_as_float(s[j]), scale));
+                            for (int j = 0; j < 64; ++j) {
+                                s[j] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(s[j]), scale), base));
+                            }
                             scale = 1.f;
+                            shift = Kind<T>::kShift;
                         }
 #pragma unroll
                         for (int c = 0; c < 2; ++c) {
@@ -1401,7 +1408,7 @@ __global__ void __launch_bounds__(32 * kFewWarps, 2) rows_kernel(const __grid_co
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
                             const float base = top[n][i & 1] == -INFINITY ? 0.f : top[n][i & 1];
-                            w[i] = exp2_approx(score[m][n][i] - base);
+                            w[i] = exp2_approx(score[m][n][i] - base + Kind<T>::kShift);
                             sum[n][i & 1] += w[i];
                         }
                         weights[m][n][0] = transpose_block(Kind<T>::pack(w[0], w[1]));
@@ -1485,7 +1492,7 @@ __device__ __forceinline__ void write_row(const AttentionParams& p, int n, int h
 // A weight of 0 does not keep an infinity or NaN out of a product: a V row that a query row does not see
 // but another of its tile does (a later token of its request, a shared position behind a short request) may
 // leave one in its sum.  Such a row is summed again over the positions it sees, by the eight lanes that join it;
-// its maximum and sum stand, they come from the scores alone.  False, and nothing is written, if what it does not
+// its maximum and sum stand, they come from the scores alone (`scale` is one over the sum, without kFactor).  False, and nothing is written, if what it does not
 // see is finite.  Its query is read before its output is written: they may be the same memory.
 template <typename T, int kDim>
 __device__ __noinline__ bool sum_again(const AttentionParams& p, int64_t b, const Request request, int n, int head, float top,
@@ -1712,13 +1719,13 @@ __global__ void __launch_bounds__(32 * kJoinWarps, kSplit == 1 ? 6 : 1) combine_
     const float scale = bad ? NAN : (total == 0.f ? 0.f : 1.f / total);
     if (p.lse && lane == 0) {
         p.lse[n * p.lse_token + head * p.lse_head] =
-            bad ? NAN : (total == 0.f ? -INFINITY : (top + log2f(total)) * 0.69314718055994531f);
+            bad ? NAN : (total == 0.f ? -INFINITY : (top + log2f(total * (1.f / Kind<T>::kFactor))) * 0.69314718055994531f);
     }
     bool odd = false;
 #pragma unroll
     for (int v = 0; v < kVectors; ++v) odd |= !finite(acc[v]);
     if (__any_sync(0xffu << (lane_id() & ~7u), odd) && !bad && isfinite(total) &&
-        sum_again<T, kDim>(p, b, request, n, head, top, scale)) {
+        sum_again<T, kDim>(p, b, request, n, head, top, scale * Kind<T>::kFactor)) {
         return;
     }
     write_row<T, kDim>(p, n, head, lane, acc, scale);

@@ -155,3 +155,31 @@ def test_large_scores_stay_a_mean_of_v(power, shape, dtype, cuda_device):
     assert (np.abs(out) <= largest * (1 + 2.0 ** -7)).all(), np.abs(out).max()
     # The maximum is the scores', off by the rounding of a sum of two, of the scale and of the product.
     assert (np.abs(_np(got[1]) - want[1]) <= 8 * E * np.abs(want[1]) + 1e-3).all()
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("shape", SHAPES)
+def test_a_flat_tail_keeps_its_weight_in_fp16(shape, dim, cuda_device):
+    """The first position of every 128 has V = 0 and takes all but 2^-26 of each other one's weight, whose V is
+    large.  fp16 holds weights down to steps of 2^-24; they refer to 2^-7 of the maximum (or less), so each is off by
+    2^-32 of the largest, beside half a step of its own."""
+    case = Case(**SHAPES[shape], heads=1, dim=dim, dtype=torch.float16)
+    case.query.zero_()
+    case.query[..., 0] = 4.0
+    case.k.zero_()
+    case.v[:] = (case.v.float().abs() * 64 + 512).half()
+    for b, length in enumerate(case.lengths.tolist()):
+        sharp = _slots(case, b, length)[::128]
+        case.k[sharp, :, 0] = 4.5  # 18 = 25.97 log 2
+        case.v[sharp] = 0.0
+    got, want = case.run(cuda_device, scale=1.0), case.want(scale=1.0)
+    finite_where_defined(got, want)
+    expected, lse, weight, _, seen = want
+    v_max, u = float(case.v.double().max()), 2.0 ** -11
+    total = np.exp(lse - 18.0)[..., None]  # the sum of the weights, the largest 1
+    # Scores are exact (one product); an exponent of 26 is off by 4 e of itself, the sums by n e.
+    inner = (2 * seen[:, None, None] + 200) * E
+    tolerance = u * (weight + np.abs(expected)) * (1 + 2 * u) + inner * weight
+    tolerance = tolerance + seen[:, None, None] * 2.0 ** -32 * v_max / total + 2.0 ** -25
+    excess = np.abs(_np(got[0]) - expected) - tolerance
+    assert excess.max() <= 0, (excess.max(), float((np.abs(_np(got[0]) - expected) / tolerance).max()))
