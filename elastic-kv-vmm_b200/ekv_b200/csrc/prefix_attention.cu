@@ -1489,6 +1489,34 @@ __device__ __forceinline__ void write_row(const AttentionParams& p, int n, int h
     }
 }
 
+// The table row behind the shared positions, -1 for none; the slot of position j.
+__device__ __forceinline__ int own_row_of(const AttentionParams& p, int64_t b) {
+    const int64_t row = p.rows ? load_index(p.rows, p.rows_es, b) : b;
+    return row >= 0 && row < p.table_rows ? static_cast<int>(row) : -1;
+}
+__device__ __forceinline__ int slot_at(const AttentionParams& p, int own_row, int64_t j) {
+    return slot_of(p, look_up(p, j < p.shared ? static_cast<int>(p.source_row) : own_row, static_cast<uint32_t>(j)));
+}
+
+// Positions that query token n sees.
+__device__ __forceinline__ int64_t seen_by(const AttentionParams& p, const Request& request, int n) {
+    const int64_t reach = p.table_width * p.page_size, seen = request.length - request.fresh + 1 + n - request.begin;
+    return seen < 0 ? 0 : (seen < reach ? seen : reach);
+}
+
+// A row whose weights are all 0 sees no position with a slot (its result is 0), or its scores are all minus infinity (0 / 0).
+__device__ __noinline__ bool sees_any(const AttentionParams& p, int64_t b, const Request request, int n) {
+    const int lane = static_cast<int>(lane_id()) % kJoinLanes;
+    const uint32_t eight = 0xffu << (lane_id() & ~7u);
+    const int64_t seen = seen_by(p, request, n);
+    const int own_row = own_row_of(p, b);
+    bool found = false;
+    for (int64_t j = 0; j < seen && !found; j += kJoinLanes) {
+        found = __any_sync(eight, j + lane < seen && slot_at(p, own_row, j + lane) >= 0);
+    }
+    return found;
+}
+
 // A weight of 0 does not keep an infinity or NaN out of a product: a V row that a query row does not see
 // but another of its tile does (a later token of its request, a shared position behind a short request) may
 // leave one in its sum.  Such a row is summed again over the positions it sees, by the eight lanes that join it;
@@ -1501,19 +1529,12 @@ __device__ __noinline__ bool sum_again(const AttentionParams& p, int64_t b, cons
     const int lane = static_cast<int>(lane_id()) % kJoinLanes;
     const uint32_t eight = 0xffu << (lane_id() & ~7u);
     const int kv_head = head / p.group;
-    const int64_t at = n - request.begin, reach = p.table_width * p.page_size;
-    const int64_t before = static_cast<int64_t>(request.length) - request.fresh + 1;
-    int64_t seen = before + at < reach ? before + at : reach;
-    if (seen < 0) seen = 0;
+    const int64_t at = n - request.begin, reach = p.table_width * p.page_size, seen = seen_by(p, request, n);
     const int64_t row_tile = (at * p.group + head - kv_head * p.group) / (2 * kRows);
-    int64_t last = before + last_token(row_tile, request.fresh, p.group);
+    int64_t last = request.length - request.fresh + 1 + last_token(row_tile, request.fresh, p.group);
     if (last > reach) last = reach;
     if (last < p.shared) last = p.shared;
-    const int64_t own = p.rows ? load_index(p.rows, p.rows_es, b) : b;
-    const int own_row = own >= 0 && own < p.table_rows ? static_cast<int>(own) : -1;
-    const auto slot_at = [&](int64_t j) {
-        return slot_of(p, look_up(p, j < p.shared ? static_cast<int>(p.source_row) : own_row, static_cast<uint32_t>(j)));
-    };
+    const int own_row = own_row_of(p, b);
     const auto load = [&](const void* plane, int64_t offset, float4* to) {
         const T* from = static_cast<const T*>(plane) + offset + 4 * lane;
 #pragma unroll
@@ -1526,7 +1547,7 @@ __device__ __noinline__ bool sum_again(const AttentionParams& p, int64_t b, cons
     float4 row[kVectors];
     bool found = false;
     for (int64_t j = seen; j < last && !found; ++j) {
-        const int slot = slot_at(j);
+        const int slot = slot_at(p, own_row, j);
         if (slot < 0) continue;
         load(p.v_plane, slot * p.v_slot + kv_head * p.v_head, row);
         bool odd = false;
@@ -1540,7 +1561,7 @@ __device__ __noinline__ bool sum_again(const AttentionParams& p, int64_t b, cons
 #pragma unroll
     for (int v = 0; v < kVectors; ++v) acc[v] = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int64_t j = 0; j < seen; ++j) {
-        const int slot = slot_at(j);
+        const int slot = slot_at(p, own_row, j);
         if (slot < 0) continue;
         load(p.k_plane, slot * p.k_slot + kv_head * p.k_head, row);
         float score = 0.f;
@@ -1716,7 +1737,8 @@ __global__ void __launch_bounds__(32 * kJoinWarps, kSplit == 1 ? 6 : 1) combine_
         }
     }
     if (!active || mine_of) return;
-    const float scale = bad ? NAN : (total == 0.f ? 0.f : 1.f / total);
+    float scale = bad ? NAN : (total == 0.f ? 0.f : 1.f / total);
+    if (total == 0.f && sees_any(p, b, request, n)) scale = NAN;
     if (p.lse && lane == 0) {
         p.lse[n * p.lse_token + head * p.lse_head] =
             bad ? NAN : (total == 0.f ? -INFINITY : (top + log2f(total * (1.f / Kind<T>::kFactor))) * 0.69314718055994531f);

@@ -159,7 +159,8 @@ def shared_prefix_attention(query: torch.Tensor, k_plane: torch.Tensor, v_plane:
     block_tables[row, t // page_size]``, where ``row`` is ``source_row`` for the first
     ``shared_tokens`` positions and ``rows[b]`` (default b) behind them.  A position without a
     slot (a negative page, one outside the planes, past the table) is skipped.  A query token
-    that sees no position gets zeros and a log-sum-exp of minus infinity.  Infinities and NaN
+    that sees no position gets zeros and a log-sum-exp of minus infinity (one whose scores are all
+    minus infinity NaN and minus infinity, as 0 / 0 and log 0 are).  Infinities and NaN
     reach the query tokens that see their position, no others.
 
     A table row covers up to 2^31 - 256 positions.  One call takes up to

@@ -183,3 +183,34 @@ def test_a_flat_tail_keeps_its_weight_in_fp16(shape, dim, cuda_device):
     tolerance = tolerance + seen[:, None, None] * 2.0 ** -32 * v_max / total + 2.0 ** -25
     excess = np.abs(_np(got[0]) - expected) - tolerance
     assert excess.max() <= 0, (excess.max(), float((np.abs(_np(got[0]) - expected) / tolerance).max()))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_rows_whose_scores_are_all_minus_infinity(dtype, cuda_device):
+    """By the definition 0 / 0, with a log-sum-exp of minus infinity; a row that sees no position has zeros, and one
+    finite score is enough for a result."""
+    # Decode: all of it odd; one finite; nothing seen; a table row that holds no page; odd shared positions.
+    case = Case(lengths=[40, 41, 0, 37, 90], shared=0, dtype=dtype, heads=1, group=4, dim=64)
+    case.query.abs_().clamp_(min=0.5)
+    case.tables[3] = -1
+    for request, count in ((0, 40), (1, 40)):
+        case.k[_slots(case, request, count), :, 3] = -float("inf")
+    out, lse = (_np(t) for t in case.run(cuda_device))
+    assert np.isnan(out[0]).all() and np.isneginf(lse[0]).all()
+    assert np.isfinite(out[[1, 4]]).all() and np.isfinite(lse[[1, 4]]).all()
+    np.testing.assert_allclose(out[1], np.broadcast_to(_np(case.v[_slots(case, 1, 41)[40]]), out[1].shape), rtol=2.0 ** -7)
+    assert (out[[2, 3]] == 0).all() and np.isneginf(lse[[2, 3]]).all()
+    # Prompts: the first 30 tokens of request 0 see odd keys only.
+    case = Case(lengths=[200, 150], new=[200, 100], shared=0, dtype=dtype, heads=1, group=4, dim=64)
+    case.query.abs_().clamp_(min=0.5)
+    case.k[_slots(case, 0, 30), :, 5] = -float("inf")
+    out, lse = (_np(t) for t in case.run(cuda_device))
+    assert np.isnan(out[:30]).all() and np.isneginf(lse[:30]).all()
+    assert np.isfinite(out[30:]).all() and np.isfinite(lse[30:]).all()
+    # A prefix of odd keys: the request inside it sees nothing else, those behind it do.
+    case = Case(lengths=[300, 301, 350] + [310] * 9, shared=300, dtype=dtype, heads=1, group=4, dim=64)
+    case.query.abs_().clamp_(min=0.5)
+    case.k[_slots(case, 0, 300), :, 7] = -float("inf")
+    out, lse = (_np(t) for t in case.run(cuda_device))
+    assert np.isnan(out[0]).all() and np.isneginf(lse[0]).all()
+    assert np.isfinite(out[1:]).all() and np.isfinite(lse[1:]).all()
