@@ -1865,7 +1865,8 @@ extern "C" int ekv_shared_prefix_attention(
         require(shared_tokens >= 0 && shared_tokens <= table_width * page_size,
                 "shared_tokens outside the table's positions");
         require(!shared_tokens || (source_row >= 0 && source_row < table_rows), "source row is outside the block table");
-        require(scale > 0.f && scale <= 3.4e38f, "scale must be positive and finite");
+        // The kernels' factor, scale * log2(e), has to be finite too.
+        require(scale > 0.f && scale <= 2.3e38f, "scale must lie in (0, 2.3e38]");
         require(query_starts || tokens == batch, "without query_starts every request has one query token");
         if (!tokens || !batch) return;
         require(query && out && lengths && (block_tables || !table_rows || !table_width) &&

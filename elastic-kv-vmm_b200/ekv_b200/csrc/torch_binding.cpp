@@ -489,7 +489,7 @@ py::tuple shared_prefix_attention(const at::Tensor& query, const at::Tensor& k_p
         return status(kNotHandled);
     }
     const double factor = scale ? *scale : 1.0 / std::sqrt(static_cast<double>(dim));
-    if (!(factor > 0.0 && factor < 3.0e38)) return status(kNotHandled);
+    if (!(factor >= 1.5e-45 && factor <= 2.3e38)) return status(kNotHandled);
     if (!out) out = at::empty(query.sizes(), query.options());
     if (!lse && want_lse) lse = at::empty({tokens, heads}, query.options().dtype(at::kFloat));
     int64_t bytes = 0;

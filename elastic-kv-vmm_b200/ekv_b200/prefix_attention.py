@@ -25,6 +25,8 @@ from .block_tables import _vector
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}  # EKV_BF16, EKV_FP16
 HEAD_DIMS = (64, 128)
+# A positive number in 32 bits, whose product with log2(e) is finite there.
+_LEAST_SCALE, _MOST_SCALE = 1.5e-45, 2.3e38
 
 
 def _rows_ok(tensor: torch.Tensor, name: str) -> None:
@@ -114,8 +116,8 @@ def _bind(query, k_plane, v_plane, block_tables, lengths, page_size, shared_toke
     if batch + -(-tokens * query_heads // kv_heads // 256) > ATTENTION_MAX_ROW_TILES:
         raise ValueError("more requests and query tokens than one call takes")
     scale = 1.0 / math.sqrt(dim) if scale is None else float(scale)
-    if not 0.0 < scale < 3.0e38:
-        raise ValueError("scale must be positive and finite")
+    if not _LEAST_SCALE <= scale <= _MOST_SCALE:
+        raise ValueError("scale must lie in [1.5e-45, 2.3e38]")
     return (
         query.data_ptr(), *_strides(query), k_plane.data_ptr(), *_strides(k_plane),
         v_plane.data_ptr(), *_strides(v_plane), slots,
@@ -165,7 +167,7 @@ def shared_prefix_attention(query: torch.Tensor, k_plane: torch.Tensor, v_plane:
 
     A table row covers up to 2^31 - 256 positions.  One call takes up to
     ``ATTENTION_MAX_ROW_TILES`` (1536) row tiles: one per request and one per 256 query rows of a
-    KV head.  ``scale`` defaults to ``1 / sqrt(dim)``; ``lse`` is float32 [tokens, query_heads],
+    KV head.  ``scale`` (1.5e-45 to 2.3e38) defaults to ``1 / sqrt(dim)``; ``lse`` is float32 [tokens, query_heads],
     the natural logarithm of the sum of the exponentials.  Scores, maxima, sums and outputs are
     held in 32 bits.  For serving: no gradients flow through it.
     """

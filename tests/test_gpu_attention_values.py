@@ -214,3 +214,19 @@ def test_rows_whose_scores_are_all_minus_infinity(dtype, cuda_device):
     out, lse = (_np(t) for t in case.run(cuda_device))
     assert np.isnan(out[0]).all() and np.isneginf(lse[0]).all()
     assert np.isfinite(out[1:]).all() and np.isfinite(lse[1:]).all()
+
+
+@pytest.mark.parametrize("scale", [2.3e38, 1.5e-45])
+@pytest.mark.parametrize("shape", ["decode", "prefix, 48 rows", "prompts"])
+def test_the_ends_of_the_scales(shape, scale, cuda_device):
+    """Scores of 0 at the largest scale, and any at the smallest, weigh every position alike."""
+    case = Case(**SHAPES[shape], heads=1, dim=64)
+    if scale > 1:
+        case.query.zero_()
+    got, want = case.run(cuda_device, scale=scale), case.want(scale=scale)
+    finite_where_defined(got, want)
+    compare(got, want, case.dtype, float(case.v.double().abs().max()), 64)
+    with pytest.raises(ValueError, match="scale"):
+        case.run(cuda_device, scale=2.4e38)
+    with pytest.raises(ValueError, match="scale"):
+        case.run(cuda_device, scale=1e-46)

@@ -222,3 +222,27 @@ def test_restatement_known_answers():
     out, lse, *_ = opa.attend(query, keys, values, np.array([[1, 0]]), [3], page_size=2, scale=1.0)
     np.testing.assert_allclose(out[0, 0], (values[2, 0] + values[3, 0] + values[0, 0]) / 3)
     np.testing.assert_allclose(lse, np.log(3.0))
+
+
+@pytest.mark.parametrize("scale", [2.4e38, 2.99e38, 1e-46, -1.0, -0.0])
+def test_attention_refuses_scales_that_32_bits_do_not_hold(scale, host, library_path):
+    """scale * log2(e), the factor of the kernels, has to be a positive number of 32 bits."""
+    from ekv_b200 import _lib
+
+    with pytest.raises(ValueError, match="scale"):
+        host[1].shared_prefix_attention(**_attend(), scale=scale)
+    with pytest.raises(ValueError, match="scale"):
+        host[1].SharedPrefixAttention(**_attend(), scale=scale)
+    lib = _lib.library(str(library_path))
+    assert lib.ekv_shared_prefix_attention(*_attention_args(scale=scale, tokens=0, batch=0)) == -1
+    assert b"scale" in lib.ekv_error()
+
+
+@pytest.mark.parametrize("scale", [2.3e38, 1.5e-45])
+def test_the_ends_of_the_scales_are_taken(scale, host, library_path):
+    from ekv_b200 import _lib
+
+    with pytest.raises(AssertionError, match="was launched"):
+        host[1].shared_prefix_attention(**_attend(), scale=scale)
+    assert _lib.library(str(library_path)).ekv_shared_prefix_attention(*_attention_args(scale=scale, tokens=0, batch=0)) == 0
+    assert np.isfinite(np.float32(scale) * np.float32(1.4426950408889634)) and np.float32(scale) > 0
