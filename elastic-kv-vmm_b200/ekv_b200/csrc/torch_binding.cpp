@@ -22,6 +22,7 @@
 #include <cstdint>
 #include <limits>
 #include <optional>
+#include <utility>
 #include <vector>
 
 #include "ekv_kernels.h"
@@ -447,6 +448,59 @@ bool entries_apart(const at::Tensor& t, int64_t width) {
     return tokens <= 1 || heads <= 1 || token >= (heads - 1) * head + width || head >= (tokens - 1) * token + width;
 }
 
+// The addresses a tensor spans; empty for one without elements.
+struct Extent {
+    int64_t begin = 0, end = 0;
+    Extent() = default;
+    explicit Extent(const at::Tensor* t) {
+        if (!t || !t->numel()) return;
+        const at::IntArrayRef sizes = t->sizes(), strides = t->strides();
+        int64_t last = 0;
+        for (size_t d = 0; d < sizes.size(); ++d) last += (sizes[d] - 1) * strides[d];
+        begin = static_cast<int64_t>(reinterpret_cast<uintptr_t>(t->const_data_ptr()));
+        end = begin + (last + 1) * static_cast<int64_t>(t->element_size());
+    }
+    bool meets(const Extent& other) const {
+        return begin < end && other.begin < other.end && begin < other.end && other.begin < end;
+    }
+};
+
+// Whether [tokens, heads(, dim)] tensors share an element: exact where their strides agree, by extents otherwise.
+bool collide(const at::Tensor& a, const at::Tensor& b) {
+    if (!Extent(&a).meets(Extent(&b))) return false;
+    const int64_t size_a = a.element_size(), size_b = b.element_size();
+    const int64_t width_a = (a.dim() == 3 ? a.size(2) : 1) * size_a, width_b = (b.dim() == 3 ? b.size(2) : 1) * size_b;
+    struct Axis {
+        int64_t step, of_a, of_b;
+    } axes[2];
+    for (int d = 0; d < 2; ++d) {
+        const int64_t step_a = a.stride(d) * size_a, step_b = b.stride(d) * size_b;
+        if (a.size(d) > 1 && b.size(d) > 1 && step_a != step_b) return true;
+        axes[d] = {a.size(d) > 1 ? step_a : (b.size(d) > 1 ? step_b : 0), a.size(d), b.size(d)};
+    }
+    if (axes[0].step < axes[1].step) std::swap(axes[0], axes[1]);
+    const int64_t most[2] = {std::max(axes[0].of_a, axes[0].of_b), std::max(axes[1].of_a, axes[1].of_b)};
+    const int64_t width = std::max(width_a, width_b);
+    if ((most[1] > 1 && axes[1].step < width) || (most[0] > 1 && axes[0].step < (most[1] - 1) * axes[1].step + width)) {
+        return true;
+    }
+    const int64_t delta = static_cast<int64_t>(reinterpret_cast<uintptr_t>(b.data_ptr())) -
+                          static_cast<int64_t>(reinterpret_cast<uintptr_t>(a.data_ptr()));
+    // Quotients are rounded towards 0 here: one more candidate on the low side.
+    const auto first = [](int64_t x, int64_t step) { return step ? x / step - 2 : 0; };
+    const auto last = [](int64_t x, int64_t step) { return step ? x / step + 2 : 0; };
+    for (int64_t i = first(delta, axes[0].step); i <= last(delta, axes[0].step); ++i) {
+        if (i <= -axes[0].of_b || i >= axes[0].of_a) continue;
+        const int64_t left = delta - i * axes[0].step;
+        for (int64_t j = first(left, axes[1].step); j <= last(left, axes[1].step); ++j) {
+            if (j <= -axes[1].of_b || j >= axes[1].of_a) continue;
+            const int64_t apart = left - j * axes[1].step;
+            if (-width_b < apart && apart < width_a) return true;
+        }
+    }
+    return false;
+}
+
 // (status, out, lse or None)
 py::tuple shared_prefix_attention(const at::Tensor& query, const at::Tensor& k_plane, const at::Tensor& v_plane,
                                   const at::Tensor& tables, const at::Tensor& lengths, int64_t page_size,
@@ -488,6 +542,23 @@ py::tuple shared_prefix_attention(const at::Tensor& query, const at::Tensor& k_p
         batch + (tokens * heads / kv_heads + 255) / 256 > EKV_ATTENTION_MAX_ROW_TILES) {
         return status(kNotHandled);
     }
+    if (out || lse) {
+        // Extents first: the exact answer is needed only where they meet.
+        const Extent results[2] = {Extent(optional_tensor(out)), Extent(optional_tensor(lse))};
+        for (const at::Tensor* read : {&query, &k_plane, &v_plane}) {
+            const Extent its(read);
+            if (lse && results[1].meets(its) && collide(*lse, *read)) return status(kNotHandled);
+            if (!out || !results[0].meets(its)) continue;
+            const bool query_itself = read == &query && out->const_data_ptr() == query.const_data_ptr() &&
+                                      stride_of(*out, 0) == stride_of(query, 0) && stride_of(*out, 1) == stride_of(query, 1);
+            if (!query_itself && collide(*out, *read)) return status(kNotHandled);
+        }
+        for (const at::Tensor* read : {&tables, &lengths, optional_tensor(rows), optional_tensor(starts)}) {
+            const Extent its(read);
+            if (results[0].meets(its) || results[1].meets(its)) return status(kNotHandled);
+        }
+        if (out && lse && results[0].meets(results[1]) && collide(*out, *lse)) return status(kNotHandled);
+    }
     const double factor = scale ? *scale : 1.0 / std::sqrt(static_cast<double>(dim));
     if (!(factor >= 1.5e-45 && factor <= 2.3e38)) return status(kNotHandled);
     if (!out) out = at::empty(query.sizes(), query.options());
@@ -524,6 +595,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
     m.def("extend_block_tables", &extend_block_tables);
     m.def("append_rows", &append_rows);
     m.def("shared_prefix_attention", &shared_prefix_attention);
+    m.def("collide", &collide);
     m.attr("NOT_HANDLED") = kNotHandled;
     m.attr("KERNEL_ERROR") = kKernelError;
 }

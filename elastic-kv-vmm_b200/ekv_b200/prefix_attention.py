@@ -21,7 +21,7 @@ import math
 import torch
 
 from ._lib import ATTENTION_MAX_ROW_TILES, call, index_esize, last_error, require_cuda, stream_handle, torch_binding
-from .block_tables import _vector
+from .block_tables import _overlap, _vector
 
 _DTYPES = {torch.bfloat16: 0, torch.float16: 1}  # EKV_BF16, EKV_FP16
 HEAD_DIMS = (64, 128)
@@ -53,6 +53,38 @@ def _strides_of(shape, strides) -> tuple[int, int]:
 def _strides(tensor: torch.Tensor) -> tuple[int, int]:
     """Strides of the first two dimensions; 0 for one of a single entry."""
     return _strides_of(tensor.shape[:2], tensor.stride()[:2])
+
+
+def _collide(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether two tensors [tokens, heads] or [tokens, heads, dim] share an element.
+
+    Exact for views of one buffer whose strides agree (slices of a fused projection, say); others count as sharing
+    when their extents do.
+    """
+    if not _overlap(a, b):
+        return False
+    width_a, width_b = ((t.shape[2] if t.dim() == 3 else 1) * t.element_size() for t in (a, b))
+    steps, counts = [], []
+    for d in range(2):
+        of_a, of_b = a.stride(d) * a.element_size(), b.stride(d) * b.element_size()
+        if a.shape[d] > 1 and b.shape[d] > 1 and of_a != of_b:
+            return True
+        steps.append(of_a if a.shape[d] > 1 else of_b if b.shape[d] > 1 else 0)
+        counts.append((a.shape[d], b.shape[d]))
+    (large, of_large), (small, of_small) = sorted(zip(steps, counts), reverse=True)
+    width = max(width_a, width_b)
+    if max(of_small) > 1 and small < width or max(of_large) > 1 and large < (max(of_small) - 1) * small + width:
+        return True
+    # Rows of b lie at delta - i * large - j * small from those of a, with i and j differences of their indices.
+    delta = b.data_ptr() - a.data_ptr()
+    near = lambda x, step, of: [  # noqa: E731
+        i for i in (range(x // step - 1, x // step + 3) if step else (0,)) if -of[1] < i < of[0]]
+    return any(-width_b < delta - i * large - j * small < width_a
+               for i in near(delta, large, of_large) for j in near(delta - i * large, small, of_small))
+
+
+def _same(a: torch.Tensor, b: torch.Tensor) -> bool:
+    return a.data_ptr() == b.data_ptr() and _strides(a) == _strides(b)
 
 
 def _outputs(query, out, lse, return_lse):
@@ -95,6 +127,18 @@ def _bind(query, k_plane, v_plane, block_tables, lengths, page_size, shared_toke
         if lse.shape != (tokens, query_heads):
             raise ValueError("lse must be [tokens, query_heads]")
         _apart(lse.shape, lse.stride(), 1, "lse")
+    outputs = [(out, "out")] if lse is None else [(out, "out"), (lse, "lse")]
+    for tensor, name in outputs:
+        if tensor is out and _same(out, query):
+            pass
+        elif _collide(tensor, query):
+            raise ValueError(f"{name} overlaps query" + (" (it may be query itself)" if tensor is out else ""))
+        if _collide(tensor, k_plane) or _collide(tensor, v_plane):
+            raise ValueError(f"{name} overlaps a plane")
+        if any(t is not None and _overlap(tensor, t) for t in (block_tables, lengths, rows, query_starts)):
+            raise ValueError(f"{name} overlaps an index tensor")
+    if lse is not None and _collide(out, lse):
+        raise ValueError("out and lse overlap")
     if type(page_size) is not int or not 1 <= page_size < 1 << 31:
         raise ValueError("page_size outside the supported range")
     if block_tables.dim() != 2 or (block_tables.shape[1] > 1 and block_tables.stride(1) != 1):
@@ -155,7 +199,8 @@ def shared_prefix_attention(query: torch.Tensor, k_plane: torch.Tensor, v_plane:
     ``query_starts`` request b has the one new token ``query[b]``; with it (int32 / int64
     [requests + 1], ascending) its new tokens are ``query[query_starts[b]:query_starts[b + 1]]``,
     the last of the request, and each sees the tokens up to itself.  Query tokens of no
-    request are left as they were in ``out`` and ``lse`` (``out`` may be ``query`` itself).
+    request are left as they were in ``out`` and ``lse``.  ``out`` may be ``query`` itself; otherwise the outputs
+    share no memory with the inputs or one another (interleaved views of one buffer are fine).
 
     Position t of request b is in slot ``page * page_size + t % page_size`` with ``page =
     block_tables[row, t // page_size]``, where ``row`` is ``source_row`` for the first

@@ -552,14 +552,15 @@ int ekv_append_rows(
  *     lse[n, h] = log sum_t exp(scale * q.k_t)          (lse may be NULL)
  * and 0 / -infinity for a token that sees nothing (NaN / -infinity for one whose scores
  * are all -infinity); infinities and NaN reach the tokens that see their position only.
- * Tokens of no request are not written.  out may be query (same strides).  dtype is that
- * of query, planes and out; head_dim 64 or 128; 0 < scale <= 2.3e38; strides in elements,
- * the head dimension contiguous, every row 16-byte aligned.  batch + ceil(tokens *
- * query_heads / kv_heads / 256) is at most EKV_ATTENTION_MAX_ROW_TILES; table_width *
- * page_size <= 2^31 - 256. workspace: ekv_shared_prefix_workspace's bytes of 256-byte
- * aligned device memory that no other call uses at the same time; its content need not be
- * initialised or kept.  The waits inside the kernel are bounded (4 s); rows that one
- * running out affects are NaN.
+ * Tokens of no request are not written.  out may be query (same strides); otherwise out
+ * and lse share no memory with the inputs or one another.  dtype is that of query, planes
+ * and out; head_dim 64 or 128; 0 < scale <= 2.3e38; strides in elements, the head
+ * dimension contiguous, every row 16-byte aligned.  batch + ceil(tokens * query_heads /
+ * kv_heads / 256) is at most EKV_ATTENTION_MAX_ROW_TILES; table_width * page_size <= 2^31
+ * - 256. workspace: ekv_shared_prefix_workspace's bytes of 256-byte aligned device memory
+ * that no other call uses at the same time; its content need not be initialised or kept.
+ * The waits inside the kernel are bounded (4 s); rows that one running out affects are
+ * NaN.
  */
 #define EKV_BF16 0
 #define EKV_FP16 1

@@ -230,3 +230,26 @@ def test_the_ends_of_the_scales(shape, scale, cuda_device):
         case.run(cuda_device, scale=2.4e38)
     with pytest.raises(ValueError, match="scale"):
         case.run(cuda_device, scale=1e-46)
+
+
+def test_outputs_in_shared_buffers(cuda_device):
+    """Outputs interleaved with the query or the planes are taken, ones in memory that is read are refused."""
+    case = Case(lengths=[60, 20, 300], shared=30, heads=2, group=2, dim=64)
+    dev = [t.to(cuda_device) for t in (case.k, case.v, case.tables, case.lengths)]
+    fused = torch.full((3, 12, 64), MARK, dtype=case.dtype, device=cuda_device)
+    fused[:, 4:8] = case.query.to(cuda_device)
+    got = case.run(cuda_device)
+
+    def run(**args):
+        from ekv_b200.prefix_attention import shared_prefix_attention
+
+        return shared_prefix_attention(fused[:, 4:8], *dev, page_size=16, shared_tokens=30, source_row=case.source, **args)
+
+    assert torch.equal(run(out=fused[:, 8:]), got[0])
+    assert bool((fused[:, :4] == MARK).all()) and torch.equal(fused[:, 4:8].cpu(), case.query)
+    for out in (fused[:, 3:7], fused.view(-1)[:768].view(3, 4, 64), dev[0].view(-1)[:768].view(3, 4, 64)):
+        with pytest.raises(ValueError, match="out overlaps"):
+            run(out=out)
+    with pytest.raises(ValueError, match="out and lse overlap"):
+        run(out=fused[:, :4], lse=fused.view(-1)[:24].view(torch.float32).view(3, 4))
+    assert torch.equal(run(out=fused[:, 4:8]), got[0])

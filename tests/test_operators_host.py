@@ -246,3 +246,79 @@ def test_the_ends_of_the_scales_are_taken(scale, host, library_path):
         host[1].shared_prefix_attention(**_attend(), scale=scale)
     assert _lib.library(str(library_path)).ekv_shared_prefix_attention(*_attention_args(scale=scale, tokens=0, batch=0)) == 0
     assert np.isfinite(np.float32(scale) * np.float32(1.4426950408889634)) and np.float32(scale) > 0
+
+
+def _bf16(*shape):
+    return torch.zeros(shape, dtype=torch.bfloat16)
+
+
+def _sharing():
+    """Calls whose outputs share memory with an input or one another, and what the refusal says."""
+    tokens, wide = _bf16(4, 4, 64), _bf16(3, 8, 64)
+    flat, plane, words = _bf16(1024), _bf16(32, 2, 64), torch.zeros(64, dtype=torch.int32)
+    yield dict(query=tokens[:3], out=tokens[1:]), "out overlaps query"
+    yield dict(query=flat[:768].view(3, 4, 64), out=flat[8:776].view(3, 4, 64)), "out overlaps query"
+    yield dict(query=wide[:, :4], out=wide[:, 2:6]), "out overlaps query"
+    yield dict(query=wide[:, :4], out=wide.view(-1)[:768].view(3, 4, 64)), "out overlaps query"  # other strides
+    yield dict(query=tokens[:1].expand(3, -1, -1), out=tokens[:3]), "out overlaps query"
+    yield dict(k_plane=plane, out=plane.view(-1)[-768:].view(3, 4, 64)), "out overlaps a plane"
+    yield dict(v_plane=plane, out=plane.view(-1)[:768].view(3, 4, 64)), "out overlaps a plane"
+    yield dict(v_plane=plane, lse=plane.view(-1)[:24].view(torch.float32).view(3, 4)), "lse overlaps a plane"
+    yield dict(query=tokens[:3], lse=tokens.view(-1)[744:768].view(torch.float32).view(3, 4)), "lse overlaps query"
+    yield dict(out=tokens[:3], lse=tokens.view(-1)[744:768].view(torch.float32).view(3, 4)), "out and lse overlap"
+    yield dict(lengths=words[10:13], lse=words[2:14].view(torch.float32).view(3, 4)), "lse overlaps an index"
+    yield dict(block_tables=words[:12].view(3, 4), lse=words[11:23].view(torch.float32).view(3, 4)), "lse overlaps an index"
+    yield dict(rows=words[:3], lse=words[:12].view(torch.float32).view(3, 4)), "lse overlaps an index"
+    yield dict(query_starts=words[8:12], lse=words[:12].view(torch.float32).view(3, 4)), "lse overlaps an index"
+
+
+@pytest.mark.parametrize("change,match", list(_sharing()))
+def test_attention_refuses_outputs_in_memory_that_is_read(change, match, host):
+    with pytest.raises(ValueError, match=match):
+        host[1].shared_prefix_attention(**{**_attend(), **change})
+    with pytest.raises(ValueError, match=match):
+        host[1].SharedPrefixAttention(**{**_attend(), **change})
+
+
+def _beside():
+    tokens, wide, flat = _bf16(3, 4, 64), _bf16(3, 12, 64), torch.zeros(1024)
+    pool, words = _bf16(32, 3, 2, 64), torch.zeros(64, dtype=torch.int32)
+    yield dict(query=tokens, out=tokens)
+    yield dict(query=wide[:, :4], out=wide[:, :4])
+    yield dict(query=wide[:, :4], out=wide[:, 4:8])  # interleaved
+    yield dict(query=wide[:, 8:], out=wide[:, :4])
+    yield dict(query=wide[:, :2], out=wide[:, 3:5], k_plane=_bf16(32, 1, 64), v_plane=_bf16(32, 1, 64))
+    yield dict(k_plane=pool[:, 0], v_plane=pool[:, 1], query=_bf16(3, 2, 64), out=pool[:3, 2])  # a third plane of the pool
+    yield dict(out=flat[:384].view(torch.bfloat16).view(3, 4, 64), lse=flat[384:396].view(3, 4))
+    yield dict(lse=words[:12].view(torch.float32).view(4, 3).t(), lengths=words[12:15], rows=words[15:18])
+
+
+@pytest.mark.parametrize("change", list(_beside()))
+def test_attention_takes_outputs_beside_what_is_read(change, host):
+    with pytest.raises(AssertionError, match="was launched"):
+        host[1].shared_prefix_attention(**{**_attend(), **change})
+
+
+def test_shared_elements_are_found():
+    """Random views of one buffer against the set of their elements; the compiled form agrees."""
+    from ekv_b200 import _lib
+    from ekv_b200.prefix_attention import _collide
+
+    compiled = getattr(_lib.torch_binding(), "collide", _collide)
+    rng = np.random.default_rng(2)
+    buffer = torch.zeros(600, dtype=torch.int16)
+    shared = exact = 0
+    for _ in range(6000):
+        steps = rng.integers(1, 40, 2)
+        views = []
+        for _ in range(2):
+            if rng.random() < 0.2:
+                steps = rng.integers(0, 40, 2)
+            shape, width = rng.integers(1, 5, 2), int(rng.integers(1, 6))
+            views.append(buffer.as_strided((*shape, width), (*steps, 1), int(rng.integers(0, 250))))
+        a, b = ({int(e) for e in torch.arange(600).as_strided(v.shape, v.stride(), v.storage_offset()).reshape(-1)} for v in views)
+        found = _collide(*views)
+        assert found == compiled(*views) and (found or not a & b)
+        shared += bool(a & b)
+        exact += not found and max(min(a), min(b)) <= min(max(a), max(b))  # interleaved
+    assert shared > 500 and exact > 100
