@@ -71,9 +71,13 @@ def extend_block_tables(block_tables: torch.Tensor, lengths: torch.Tensor, new_t
     in the returned lengths.  A request whose tokens its table row cannot hold is passed over.
     A negative page, in the table or in ``free_pages``, gives its tokens slot -1.
 
+    Tokens that fill up a request's last page go to the page that its row names there.  A request that
+    begins with shared tokens which end inside a page must therefore have a page of its own in that entry:
+    with none its tokens get slot -1, and with the donor's all requests would write into that one.
+
     ``block_tables`` is written in place (only the entries of taken pages); nothing else
     among the inputs changes, so the step can be repeated.  Active requests must have
-    distinct rows.  ``out`` takes the tensors of an earlier result again; they must not
+    distinct rows, and no other input may lie in the entries that are written.  ``out`` takes the tensors of an earlier result again; they must not
     overlap the inputs or one another (copy ``out.lengths`` to the next step's lengths instead).
     """
     fast = torch_binding() if out is None and type(page_size) is int and type(max_tokens) is int else None

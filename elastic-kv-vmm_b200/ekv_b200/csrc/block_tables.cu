@@ -10,14 +10,14 @@
 // Bound by latency up to ~10^5 tokens: one launch in which EVERY block scans the
 // whole batch (1024 requests a pass; two dependent 4-byte loads and one block scan)
 // and then places only its own slice of tokens and pages, so no second launch or
-// grid-wide wait separates the scan from the placement: 6.4 us on the device for 8
-// requests, 8.3 us for 1024 requests of one token or 257,000 tokens of prompts; 13 us a
+// grid-wide wait separates the scan from the placement: 6.3 us on the device for 8
+// requests, 8.4 us for 1024 requests of one token or 257,000 tokens of prompts; 13 us a
 // call from Python, which binds it.
 //
 // append_rows_kernel.  plane[slot_map[i]] = row[i] for every plane: HBM-bound, one
 // read and one write of each row.  Rows are flattened to vectors (plane in grid.y) and
 // each thread keeps kAppendUnroll independent copies in flight: 65,536 tokens of 2 KB in K
-// and in V 84 us, 0.97 of the measured copy peak; 64 tokens 4.2 us (9 us a call).
+// and in V, one in 97 skipped, 84 us, 0.96 of the measured copy peak; 64 tokens 4.2 us (9 us a call).
 #include "common.cuh"
 
 namespace ekv {

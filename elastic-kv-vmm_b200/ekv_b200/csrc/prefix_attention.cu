@@ -24,7 +24,8 @@
 // follow one another: the softmax of one runs beside the second product of the other and, right behind it, the first
 // product of that half of the next tile, whose scores take the place of its weights.  (A first product of 64
 // columns runs at half the tensor cores' rate, since its 128 rows come from shared memory each time; waiting
-// for products of whole tiles cost more: 8 requests of up to 400 new tokens over 8001 shared ones 372 us against 343.)
+// for products of whole tiles cost more where the two were compared: 8 requests of up to 400 new tokens over 8001
+// shared ones 372 us against 343.)
 // Roles by warp: 0-3 and 4-7 softmax of the halves ("slots") 0 and 1 of a row tile; 8-11 copy the K rows,
 // 12-15 the V rows into swizzled shared memory (cp.async, 16 bytes a lane, whole rows; slots resolved
 // through the table, zeros for positions without one); 16 and 17 issue the products of slots 0 and 1
@@ -35,9 +36,10 @@
 // An item of more than 128 rows uses both slots on the same K and V (kBoth); a smaller one with many
 // tiles gives its even tiles to one slot and its odd ones to the other (kPair; the two join before
 // they are written); with few tiles, items alternate between the slots (kSingle).
-// What bounds it: the instructions of the softmax warps (128 x 256 exponentials a tile), beside which
-// eight copying warps run; the tensor cores are busy 40 % of the time.  256 requests of 64 heads over 32768
-// shared tokens and up to 900 own ones: 375 us for 279 GFLOP, 0.44 of the measured matrix peak.
+// What bounds it: no single unit.  Tensor cores (half of whose work runs at half rate), exponential unit and issue
+// slots, which eight copying warps share, are each busy 40 to 47 % of the time; the rest is each half waiting for the
+// chain of product, softmax and product.  256 requests of 64 heads over 32768 shared tokens and up to 900 own ones:
+// 373 us in graph replays for 279 GFLOP, 0.44 of the measured matrix peak.
 //
 // The maximum a row's weights refer to is raised only when the scores' maximum passes it by 2^8
 // (kRaise), which makes rescaling O rare; weights are then at most 2^8.  They are rounded to the 16-bit type
@@ -241,8 +243,9 @@ __device__ __forceinline__ uint32_t few_prefix_cost(const AttentionParams& p) {
 
 // Blocks (an SM each) that attention_kernel uses when both kernels have work: the two share the SMs in
 // proportion to their estimated times there (a unit of its cost takes about 0.37 us of an SM, one of
-// rows_kernel's 0.35 us), so that the memory-bound part runs beside the compute-bound one: 128 requests over
-// 16384 shared tokens 181 us against 217 one behind the other.
+// rows_kernel's 0.35 us, at heads of 128; heads of 64 go by the same numbers), so that the memory-bound part runs beside
+// the compute-bound one: 128 requests over 16384 shared tokens 181 us against 217 one behind the other where the two
+// were compared, 173 now.
 __device__ __forceinline__ int large_blocks(const AttentionParams& p, int64_t large, int64_t few) {
     if (!few || !large) return p.blocks;
     const int64_t mine = large * kLargeTime, its = few * kFewTime;
@@ -1137,7 +1140,8 @@ struct FewLayout {
 // units, but a share belongs to a WARP, which keeps to itself: it copies 16 or 32 positions of K and V at a
 // time into its own shared memory (the next keys while it weighs these, the next values while it
 // scores those) and multiplies them with mma.sync, positions by rows: S^T = K Q^T, O^T += V^T P^T,
-// so that up to 8 rows cost half of what 16 do.  Sixteen such warps an SM have about 128 KB on the way.
+// so that up to 8 rows cost half of what 16 do.  Sixteen such warps an SM have 128 KB of buffers, about half of
+// them on the way at a time.  (At heads of 128 a thread's 128 registers spill some 160 bytes.)
 template <typename T, int kDim>
 __global__ void __launch_bounds__(32 * kFewWarps, 2) rows_kernel(const __grid_constant__ AttentionParams p) {
     using L = FewLayout<kDim>;

@@ -199,12 +199,13 @@ def shared_prefix_attention(query: torch.Tensor, k_plane: torch.Tensor, v_plane:
     ``query_starts`` request b has the one new token ``query[b]``; with it (int32 / int64
     [requests + 1], ascending) its new tokens are ``query[query_starts[b]:query_starts[b + 1]]``,
     the last of the request, and each sees the tokens up to itself.  Query tokens of no
-    request are left as they were in ``out`` and ``lse``.  ``out`` may be ``query`` itself; otherwise the outputs
+    request are left as they were in ``out`` and ``lse`` (uninitialised in tensors that the call makes).  ``out`` may be ``query`` itself; otherwise the outputs
     share no memory with the inputs or one another (interleaved views of one buffer are fine).
 
     Position t of request b is in slot ``page * page_size + t % page_size`` with ``page =
     block_tables[row, t // page_size]``, where ``row`` is ``source_row`` for the first
-    ``shared_tokens`` positions and ``rows[b]`` (default b) behind them.  A position without a
+    ``shared_tokens`` positions and ``rows[b]`` (default b) behind them (where the shared positions end
+    inside a page, the request's own entry for that page is read from there on).  A position without a
     slot (a negative page, one outside the planes, past the table) is skipped.  A query token
     that sees no position gets zeros and a log-sum-exp of minus infinity (one whose scores are all
     minus infinity NaN and minus infinity, as 0 / 0 and log 0 are).  Infinities and NaN
@@ -214,7 +215,10 @@ def shared_prefix_attention(query: torch.Tensor, k_plane: torch.Tensor, v_plane:
     ``ATTENTION_MAX_ROW_TILES`` (1536) row tiles: one per request and one per 256 query rows of a
     KV head.  ``scale`` (1.5e-45 to 2.3e38) defaults to ``1 / sqrt(dim)``; ``lse`` is float32 [tokens, query_heads],
     the natural logarithm of the sum of the exponentials.  Scores, maxima, sums and outputs are
-    held in 32 bits.  For serving: no gradients flow through it.
+    held in 32 bits.  The weights are rounded to the inputs' type before they multiply V (half a step, up to 2^-8
+    of each in bfloat16 and 2^-11 in float16, which also loses what is below 2^-32 of the largest); their sum
+    is of the unrounded ones, and the result is rounded once more.  Sums are of weights up to 2^8 (2^15 in
+    float16) times V, so a V above 2^100 may overflow them.  For serving: no gradients flow through it.
     """
     fast = torch_binding() if all(type(x) is int for x in (page_size, shared_tokens, source_row)) else None
     if fast is not None:
@@ -243,7 +247,7 @@ class SharedPrefixAttention:
     Each call only launches; the tensors must outlive the object and keep their storage.
     The results are in ``out`` and ``lse`` (None unless given or asked for).  The object owns its
     workspace, so its calls must not overlap one another: two graphs that capture the same
-    object must not replay at the same time.
+    object must not replay at the same time.  The object must outlive the graphs that capture it.
     """
 
     def __init__(self, query, k_plane, v_plane, block_tables, lengths, *, page_size, shared_tokens=0, source_row=0,

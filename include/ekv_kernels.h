@@ -557,10 +557,12 @@ int ekv_append_rows(
  * and out; head_dim 64 or 128; 0 < scale <= 2.3e38; strides in elements, the head
  * dimension contiguous, every row 16-byte aligned.  batch + ceil(tokens * query_heads /
  * kv_heads / 256) is at most EKV_ATTENTION_MAX_ROW_TILES; table_width * page_size <= 2^31
- * - 256. workspace: ekv_shared_prefix_workspace's bytes of 256-byte aligned device memory
+ * - 256.  workspace: ekv_shared_prefix_workspace's bytes of 256-byte aligned device memory
  * that no other call uses at the same time; its content need not be initialised or kept.
  * The waits inside the kernel are bounded (4 s); rows that one running out affects are
- * NaN.
+ * NaN.  Scores, maxima, sums and outputs are held in 32 bits; the weights are rounded to
+ * dtype before they multiply v (their sum is of the unrounded ones), and the result once
+ * more.
  */
 #define EKV_BF16 0
 #define EKV_FP16 1
