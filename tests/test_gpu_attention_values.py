@@ -253,3 +253,44 @@ def test_outputs_in_shared_buffers(cuda_device):
     with pytest.raises(ValueError, match="out and lse overlap"):
         run(out=fused[:, :4], lse=fused.view(-1)[:24].view(torch.float32).view(3, 4))
     assert torch.equal(run(out=fused[:, 4:8]), got[0])
+
+
+@pytest.mark.parametrize("new", [None, [1, 5, 0, 20]])
+def test_query_rows_far_behind_the_last_token(new, cuda_device):
+    """A step captured for 600 tokens that holds a few: NaN behind the last query, outputs there left alone."""
+    from ekv_b200.prefix_attention import SharedPrefixAttention
+
+    case = Case(lengths=[310, 330, 300, 420], shared=300, new=new or [1] * 4, heads=2, group=4, dim=64)
+    count = case.query.shape[0]
+    query = torch.full((600, *case.query.shape[1:]), float("nan"), dtype=case.dtype, device=cuda_device)
+    query[:count] = case.query.to(cuda_device)
+    out, lse = torch.full_like(query, MARK), torch.full(query.shape[:2], MARK, device=cuda_device)
+    dev = [t.to(cuda_device) for t in (case.k, case.v, case.tables, case.lengths)]
+    plan = SharedPrefixAttention(query, *dev, page_size=16, shared_tokens=300, source_row=case.source,
+                                 query_starts=case.starts.to(cuda_device), out=out, lse=lse)
+    graph = torch.cuda.CUDAGraph()
+    plan()
+    with torch.cuda.graph(graph):
+        plan()
+    out.fill_(MARK)
+    lse.fill_(MARK)
+    graph.replay()
+    assert bool((out[count:] == MARK).all()) and bool((lse[count:] == MARK).all())
+    got, want = (out[:count], lse[:count]), case.want()
+    finite_where_defined(got, want)
+    compare(got, want, case.dtype, float(case.v.double().abs().max()), 64)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("lengths,heads,group,dim,new", [
+    ([131072], 1, 4, 128, None), ([32768, 40001, 3], 1, 1, 64, None), ([33000, 20000], 2, 4, 128, [3, 1]),
+    ([40000, 9000], 1, 4, 64, [30, 2]),
+])
+def test_long_own_contexts_in_few_heads(lengths, heads, group, dim, new, dtype, cuda_device):
+    """One request spread over all warps or blocks, whose parts the join walks one by one; without a prefix."""
+    case = Case(lengths=lengths, shared=0, heads=heads, group=group, dim=dim, dtype=dtype, new=new, page=64, spread=3.0)
+    got, want = case.run(cuda_device), case.want()
+    finite_where_defined(got, want)
+    compare(got, want, dtype, float(case.v.double().abs().max()), dim)
+    again = case.run(cuda_device)
+    assert torch.equal(again[0], got[0]) and torch.equal(again[1], got[1])
